@@ -52,6 +52,29 @@ Checker& Checker::buffers(const Span* spans, size_t count, size_t outputs) {
     return *this;
 }
 
+bool View::meets(const View& o) const {
+    const Span a = span(), b = o.span();
+    if (a.bytes == 0 || b.bytes == 0 || !a.meets(b)) return false;
+    if (stride == 0 || stride != o.stride || value != o.value) return true;
+    // o's columns in this view's rows start at column `from`.
+    const size_t row = stride * value;
+    const size_t ahead = a.begin() % row, behind = b.begin() % row;
+    const size_t from = (behind + row - ahead) % row;
+    return !(from >= width * value && from + o.width * value <= row);
+}
+
+Checker& Checker::views(std::initializer_list<View> views, size_t outputs) {
+    for (const View& v : views)
+        for (int kind : {kNull, kAlign, kWrap}) one(v.span(), kind);
+    for (size_t i = 0; i < outputs && i < views.size(); ++i)
+        for (size_t j = i + 1; j < views.size(); ++j) {
+            const View& a = views.begin()[i];
+            const View& b = views.begin()[j];
+            require(!a.meets(b), "%s and %s overlap", a.name, b.name);
+        }
+    return *this;
+}
+
 Checker& Checker::apart(const Span& first, std::initializer_list<Span> others) {
     for (const Span& o : others) require(!first.meets(o), "%s and %s overlap", first.name, o.name);
     return *this;

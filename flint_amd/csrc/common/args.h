@@ -35,6 +35,23 @@ struct Span {
     }
 };
 
+// One device buffer of rows `stride` values apart, `width` of them the call's
+// own (a column slice of a wider tensor), or with stride 0 one run of `width`
+// values; `value` bytes each.
+struct View {
+    const char* name;
+    const void* at;
+    size_t rows, width, stride;
+    size_t value;
+
+    Span span() const {
+        return {name, at, rows == 0 ? 0 : ((rows - 1) * stride + width) * value};
+    }
+    // Whether some byte is in both. Slices of rows of one stride whose columns
+    // are apart interleave without meeting.
+    bool meets(const View& o) const;
+};
+
 class Checker {
 public:
     explicit Checker(const char* function) : function_(function) {}
@@ -54,6 +71,9 @@ public:
     Checker& buffers(std::initializer_list<Span> spans, size_t outputs) {
         return buffers(spans.begin(), spans.size(), outputs);
     }
+
+    // The same for views, whose column slices may interleave.
+    Checker& views(std::initializer_list<View> views, size_t outputs);
 
     // "<first> and <other> overlap" for the first `other` that meets `first`.
     Checker& apart(const Span& first, std::initializer_list<Span> others);

@@ -1,0 +1,167 @@
+// Tiles of 64 rows of one head (64 or 128 halves a row) in LDS, and the MFMA
+// fragments read from them, for the attention over packed sequences (packed.hip)
+// and over a paged cache (paged.hip). The layouts are attention.hip's: scores
+// transposed (a lane holds one query), probabilities used as the next product's
+// operand straight from their registers.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "kernels/gemm_common.h"
+
+namespace flint {
+namespace {
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc_of(const void* base, unsigned bytes) {
+    const uint64_t v = reinterpret_cast<uint64_t>(base);
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(v));
+    const uint32_t hi = __builtin_amdgcn_readfirstlane(uint32_t(v >> 32));
+    void* p = reinterpret_cast<void*>((uint64_t(hi) << 32) | lo);
+    return __builtin_amdgcn_make_buffer_rsrc(p, 0, __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
+}
+
+// lgkmcnt(0): the transposing reads are inline asm, invisible to the
+// compiler's wait insertion.
+__device__ __forceinline__ void wait_lds() {
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The value of lane ^ 32 (the other half of the wave holds the same query).
+__device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
+
+// A tile holds rows of HD halves back to back, 16-byte chunk c of row r at
+// chunk position c ^ key(r). Two reads have to spread over the banks: the 16
+// lanes of a row fragment take one chunk of 16 consecutive rows, those of a
+// transposing read two neighbouring chunks of 4 consecutive rows. A row of 128
+// halves covers all 64 banks, so its 16 rows need 16 keys; one of 64 covers
+// half of them, so pairs of rows share 8 keys. Rotating the row bits left by
+// one makes the keys of 4 neighbouring rows differ above bit 0, which keeps
+// their chunk pairs apart.
+template <int HD>
+struct Tile {
+    static_assert(HD == 64 || HD == 128, "head widths");
+    static constexpr int kHalves = 64 * HD;
+    static constexpr int kChunks = HD / 8;          // of a row
+    static constexpr int kLoadRows = 64 / kChunks;  // rows of one load: 64 lanes, 16 bytes each
+    static constexpr int kLoads = 64 / kLoadRows;   // loads of a tile
+
+    static __device__ __forceinline__ int key(int row) {
+        if constexpr (HD == 64) {
+            const int r = (row >> 1) & 7;
+            return ((r << 1) | (r >> 2)) & 7;
+        } else {
+            const int r = row & 15;
+            return ((r << 1) | (r >> 3)) & 15;
+        }
+    }
+};
+
+// Rows 0 .. 63 at `from` (rows `stride` halves apart; those from `left` on read
+// as zeros) into a tile by direct-to-LDS loads, shared out over WAVES waves.
+template <int HD, int WAVES>
+__device__ __forceinline__ void load_tile(_Float16* tile, const _Float16* from, int left, int stride,
+                                          int wave, int lane) {
+    using T = Tile<HD>;
+    const int rows = min(left, 64);
+    const auto rs = rsrc_of(from, rows <= 0 ? 0u : unsigned((rows - 1) * stride + HD) * 2u);
+#pragma unroll
+    for (int i = 0; i < T::kLoads / WAVES; ++i) {
+        const int u = wave + WAVES * i;
+        const int row = u * T::kLoadRows + lane / T::kChunks;
+        const unsigned voff =
+            unsigned(row * stride + (((lane % T::kChunks) ^ T::key(row)) * 8)) * 2u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(lds_half*)(tile + u * 512), 16, voff, 0, 0,
+            0);
+    }
+}
+
+// Per-lane byte offsets of the fragment reads, kept in registers (an empty asm
+// makes them opaque, so they are not recomputed per read). Rows 16 and 32 apart
+// have one key, so they are immediate offsets from these.
+template <int HD>
+struct Frags {
+    unsigned rows[HD / 16];
+    unsigned tr[HD / 32][2];
+
+    __device__ __forceinline__ explicit Frags(int lane) {
+        using T = Tile<HD>;
+        const int fr = lane & 31, h = lane >> 5, j = lane & 15;
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) {
+            rows[kk] = unsigned((fr * HD + (((2 * kk + h) ^ T::key(fr)) * 8)) * 2);
+            asm volatile("" : "+v"(rows[kk]));
+        }
+#pragma unroll
+        for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int row = 4 * h + (j >> 2) + 8 * t;
+                const int col = 32 * db + 16 * ((lane >> 4) & 1) + 4 * (j & 3);
+                tr[db][t] = unsigned((row * HD + (((col >> 3) ^ T::key(row)) * 8) + (col & 7)) * 2);
+                asm volatile("" : "+v"(tr[db][t]));
+            }
+    }
+
+    // An MFMA operand with tile rows as its rows and d as k: lane l gets row
+    // 32 hb + l % 32, halves 16 kk + 8 (l / 32) .. + 8.
+    __device__ __forceinline__ f16x8 row(const _Float16* tile, int hb, int kk) const {
+        return *reinterpret_cast<const f16x8*>(reinterpret_cast<const char*>(tile) + rows[kk] +
+                                               64 * HD * hb);
+    }
+
+    // An MFMA operand with d as its rows and tile rows as k, in the order the
+    // probabilities' registers hold them: lane l (d = 32 db + l % 32, h = l /
+    // 32) gets tile rows 16 cs + 4h .. + 3 (k 0..3) and 16 cs + 8 + 4h .. + 3
+    // (k 4..7) of column d. wait_lds before the first use.
+    template <int CS>
+    __device__ __forceinline__ TrFrag transposed(const _Float16* tile, int db) const {
+        const unsigned base = unsigned(reinterpret_cast<uintptr_t>((lds_half*)tile));
+        TrFrag f;
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
+                     : "=v"(f.lo) : "v"(base + tr[db][0]), "i"(32 * HD * CS));
+        asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2"
+                     : "=v"(f.hi) : "v"(base + tr[db][1]), "i"(32 * HD * CS));
+        return f;
+    }
+    // For a slice known once the loops are unrolled.
+    __device__ __forceinline__ TrFrag transposed(const _Float16* tile, int cs, int db) const {
+        switch (cs) {
+        case 0: return transposed<0>(tile, db);
+        case 1: return transposed<1>(tile, db);
+        case 2: return transposed<2>(tile, db);
+        default: return transposed<3>(tile, db);
+        }
+    }
+};
+
+__device__ __forceinline__ f32x16 mfma(const f16x8& a, const f16x8& b, const f32x16& c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// The row (0..31) of an MFMA result that register r of a lane in half h holds.
+__device__ __forceinline__ constexpr int result_row(int r, int h) {
+    return 8 * (r >> 2) + 4 * h + (r & 3);
+}
+
+// A lane's part of a result transposed to rows (one query or key of the lane,
+// HD values scaled by `by`) written to `row` as FP16.
+template <int HD>
+__device__ __forceinline__ void store_row(_Float16* row, const f32x16* acc, float by, int h) {
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const f16x4 v = {_Float16(acc[db][4 * a] * by), _Float16(acc[db][4 * a + 1] * by),
+                             _Float16(acc[db][4 * a + 2] * by), _Float16(acc[db][4 * a + 3] * by)};
+            *reinterpret_cast<f16x4*>(row + 32 * db + 8 * a + 4 * h) = v;
+        }
+}
+
+}  // namespace
+}  // namespace flint

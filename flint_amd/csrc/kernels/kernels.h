@@ -8,6 +8,8 @@
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
+#include "flint/flint_packed.h"
+#include "flint/flint_paged.h"
 #include "flint/flint_train.h"
 
 namespace flint {
@@ -157,6 +159,47 @@ hipError_t launch_attention_backward(void* dq, void* dk, void* dv, const void* d
                                      const void* k, const void* v, const void* o, const void* lse,
                                      void* dsum, size_t batches, size_t length, float scale,
                                      hipStream_t stream, AttnLayout layout = {});
+// Causal attention over packed sequences (packed.hip): blocks of kPackedBlock
+// queries of one sequence, listed longest first by the plan (PackedItem, at
+// most packed_items of them, behind one 16-byte header holding their count).
+constexpr size_t kPackedMaxTokens = size_t{1} << 26;
+constexpr size_t kPackedMaxSequences = size_t{1} << 20;
+constexpr size_t kHeadsMax = 1024;
+constexpr size_t kStrideMax = size_t{1} << 23;
+constexpr size_t kPackedMaxBlocks = size_t{1} << 23;   // workgroups: below 2^32 threads
+constexpr int kPackedBlock = 128;
+struct PackedItem {
+    int begin, end;   // the sequence's rows
+    int block;        // queries (or keys) begin + 128 block on
+    int pad;
+};
+inline size_t packed_items(const flint_packed_shape& s) {
+    return s.tokens / kPackedBlock + s.sequences;
+}
+inline size_t packed_plan_bytes(const flint_packed_shape& s) {
+    return (packed_items(s) + 1) * sizeof(PackedItem);
+}
+size_t packed_backward_workspace(const flint_packed_shape& s);
+hipError_t launch_packed_plan(void* plan, const void* offsets, const flint_packed_shape& s,
+                              hipStream_t stream);
+hipError_t launch_packed_forward(void* o, void* lse, const void* q, const void* k, const void* v,
+                                 const void* plan, const flint_packed_shape& s, float scale,
+                                 hipStream_t stream);
+hipError_t launch_packed_backward(void* dq, void* dk, void* dv, const void* dout, const void* q,
+                                  const void* k, const void* v, const void* o, const void* lse,
+                                  const void* plan, const flint_packed_shape& s, float scale,
+                                  void* workspace, hipStream_t stream);
+// Attention of new tokens over a paged cache (paged.hip).
+constexpr size_t kPagedMaxTokens = size_t{1} << 20;
+constexpr size_t kPagedMaxSequences = 65535;
+constexpr size_t kPagedMaxPageSize = 65536;
+constexpr size_t kPagedMaxPositions = size_t{1} << 30;
+size_t paged_workspace(const flint_paged_shape& s);
+hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const void* q,
+                                  const void* k, const void* v, const void* offsets,
+                                  const void* cached, const void* table,
+                                  const flint_paged_shape& s, float scale, void* workspace,
+                                  hipStream_t stream);
 // Rows of a causal tile and the k-step both divide this: a causal softmax
 // writing its zeros up to the end of each such block covers what the causal
 // GEMMs read.
@@ -284,6 +327,16 @@ hipError_t launch_attn_scores_softmax_backward(void* ds, const void* p, const vo
 hipError_t launch_softmax_cross_entropy(void* dlogits, void* row_loss, const void* logits,
                                         const void* targets, float scale, size_t rows,
                                         size_t vocab, size_t cols, hipStream_t stream);
+// Log probabilities of given tokens (logprobs.hip).
+constexpr size_t kLogprobsMaxTop = 64;
+hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, void* top_ids,
+                                   void* top_logprobs, const void* logits, const void* targets,
+                                   float scale, size_t rows, size_t vocab, size_t cols, size_t top,
+                                   hipStream_t stream);
+hipError_t launch_logprobs_backward(void* dlogits, const void* dlogprob, const void* dentropy,
+                                    const void* logits, const void* targets, const void* entropy,
+                                    const void* stats, float scale, size_t rows, size_t vocab,
+                                    size_t cols, hipStream_t stream);
 
 // Data movement.
 constexpr size_t kEmbeddingMaxWidth = size_t{1} << 24;

@@ -1,0 +1,554 @@
+// Causal attention over packed sequences for gfx950: sequences of different
+// lengths one after another in the token rows, grouped heads, head widths 64
+// and 128; forward, and backward to dQ, dK and dV.
+//
+// Per query t of a sequence, over its keys t' <= t: S = c q k^T (c = scale
+// log2 e), P = 2^(S - m) / l with the running maximum m and sum l, O = P V,
+// lse = (m + log2 l) ln 2. Backward, with P recomputed from lse and D = sum
+// dO O: dV = P^T dO, dS = P (dO V^T - D), dQ = scale dS K, dK = scale dS^T Q.
+//
+// A workgroup owns 128 queries (dK/dV: keys) of one sequence and head and walks
+// the sequence's tiles of 64 keys (queries). Which, the plan says: a list of
+// blocks, longest first, made once a batch on the device. The work of a block
+// grows with its place in its sequence, so the list's order is what balances
+// the GPU; the kernels' grids are the largest number of blocks that tokens and
+// sequences allow, and workgroups past the list's end leave at once.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <type_traits>
+
+#include "common/common.h"
+#include "kernels/attention_tiles.h"
+#include "kernels/kernels.h"
+
+namespace flint {
+namespace {
+
+constexpr int kThreads = 256;   // 4 waves of 32 queries (keys)
+// How far (log2 units) a query's scores may rise above the running maximum
+// before O and l are rescaled: P <= 2^8 until then, far inside FP16.
+constexpr float kRescale = 8.0f;
+
+// ---------------------------------------------------------------- plan
+
+constexpr int kPlanThreads = 1024;
+constexpr int kBuckets = 1024;
+
+// One workgroup. The blocks of a sequence of n blocks have places 0 .. n - 1;
+// bucket b holds the places b << shift .. and comes before bucket b - 1. A
+// counting sort: full[b] counts the sequences whose last, partly filled bucket
+// is b, part[b] their places in it; the items of b are part[b] + (full[b + 1] +
+// full[b + 2] + ...) << shift. Within a bucket the order is the arrival's: it
+// changes which workgroup takes which block and no result.
+__global__ void __launch_bounds__(kPlanThreads)
+packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequences, int tokens,
+            int capacity, int shift) {
+    __shared__ int full[kBuckets], part[kBuckets], next[kBuckets];
+    const int tid = threadIdx.x;
+    full[tid] = part[tid] = 0;
+    __syncthreads();
+    auto rows_of = [&](int s, int* begin) {
+        const int a = min(max(offsets[s], 0), tokens), b = min(max(offsets[s + 1], a), tokens);
+        *begin = a;
+        return b;
+    };
+    const int low = (1 << shift) - 1;
+    for (int s = tid; s < sequences; s += kPlanThreads) {
+        int begin;
+        const int end = rows_of(s, &begin);
+        const int n = (end - begin + kPackedBlock - 1) / kPackedBlock;
+        if (n == 0) continue;
+        atomicAdd(&full[n >> shift], 1);
+        atomicAdd(&part[n >> shift], n & low);
+    }
+    __syncthreads();
+    // items[b], then its sum over the buckets after b.
+    __shared__ int sums[2][kBuckets];
+    auto after = [&](int own) {   // sum of `own` over the threads after this one
+        int at = 0;
+        sums[0][tid] = own;
+        __syncthreads();
+        for (int d = 1; d < kBuckets; d *= 2) {
+            const int v = sums[at][tid] + (tid + d < kBuckets ? sums[at][tid + d] : 0);
+            sums[at ^ 1][tid] = v;
+            at ^= 1;
+            __syncthreads();
+        }
+        const int total = sums[at][tid] - own;
+        __syncthreads();
+        return total;
+    };
+    const int longer = after(full[tid]);
+    const int items = part[tid] + (longer << shift);
+    const int first = after(items);
+    next[tid] = first;
+    if (tid == 0) plan[0] = int4{min(first + items, capacity), 0, 0, 0};
+    __syncthreads();
+    // A sequence of many blocks is written by its whole wave.
+    const int lane = tid & 63;
+    for (int base = 0; base < sequences; base += kPlanThreads) {
+        const int s = base + tid;
+        int begin = 0, end = 0;
+        if (s < sequences) end = rows_of(s, &begin);
+        const int n = (end - begin + kPackedBlock - 1) / kPackedBlock;
+        auto put = [&](int b0, int e0, int block) {
+            const int at = atomicAdd(&next[min(block >> shift, kBuckets - 1)], 1);
+            if (at < capacity) plan[1 + at] = int4{b0, e0, block, 0};
+        };
+        if (n <= 16)
+            for (int b = 0; b < n; ++b) put(begin, end, b);
+        for (unsigned long long many = __ballot(n > 16); many != 0; many &= many - 1) {
+            const int from = __ffsll(many) - 1;
+            const int b0 = __shfl(begin, from), e0 = __shfl(end, from), n0 = __shfl(n, from);
+            for (int b = lane; b < n0; b += 64) put(b0, e0, b);
+        }
+    }
+}
+
+// The block that rank `rank` of `heads` heads works on; false past the list. A
+// plan of other sequences gives wrong rows, but none outside the tokens.
+struct Work {
+    int begin, length, block, head;
+};
+__device__ __forceinline__ bool work_of(const int4* plan, int rank, int heads, int tokens,
+                                        Work* w) {
+    const int item = rank / heads;
+    if (item >= plan[0].x) return false;
+    const int4 it = plan[1 + item];
+    w->begin = min(max(it.x, 0), tokens);
+    w->length = min(max(it.y, w->begin), tokens) - w->begin;
+    w->block = it.z;
+    w->head = rank - item * heads;
+    return it.z >= 0 && it.z <= (w->length - 1) / kPackedBlock && w->length > 0;
+}
+
+// Fragments of rows `row0 + l % 32` of a head's matrix (zeros from `left` on):
+// 16-byte chunks 2 kk + l / 32.
+template <int HD>
+__device__ __forceinline__ void load_frags(f16x8 (&f)[HD / 16], const _Float16* base, int row,
+                                           int left, int stride, int h) {
+    const _Float16* at = base + size_t(row) * stride + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+        f[kk] = row < left ? *reinterpret_cast<const f16x8*>(at + 16 * kk) : f16x8{};
+}
+
+struct Strides {
+    int q, kv, o;
+};
+
+// ---------------------------------------------------------------- forward
+
+template <int HD, bool NEG>
+__global__ void __launch_bounds__(kThreads, HD == 64 ? 3 : 2)
+packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float16* __restrict__ q,
+               const _Float16* __restrict__ k, const _Float16* __restrict__ v,
+               const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
+               float c) {
+    constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    Work w;
+    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, h = lane >> 5;
+    const Frags<HD> fo(lane);
+    const int length = w.length;
+    const _Float16* qb = q + size_t(w.begin) * st.q + size_t(w.head) * HD;
+    const _Float16* kb = k + size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
+    const _Float16* vb = v + size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
+    const int q0 = w.block * kPackedBlock + wave * 32;
+    const int qi = q0 + fr;
+
+    f16x8 qf[KK];
+    load_frags<HD>(qf, qb, qi, length, st.q, h);
+    float m = -INFINITY, l = 0.0f;
+    f32x16 acc[DB] = {};
+    const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
+    const int tiles = q_last / 64 + 1;
+    auto load = [&](int j) {
+        _Float16* t = lds + (j & 1) * 2 * kTile;
+        const size_t at = size_t(64 * j) * st.kv;
+        load_tile<HD, 4>(t, kb + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, 4>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
+    };
+    load(0);
+    for (int j = 0; j < tiles; ++j) {
+        wait_vmcnt<0>();
+        block_sync();
+        const _Float16* kt = lds + (j & 1) * 2 * kTile;
+        const _Float16* vt = kt + kTile;
+        if (j + 1 < tiles) load(j + 1);
+        const int kbase = 64 * j;
+        if (kbase > q0 + 31) continue;          // every key after every query of the wave
+        f32x16 s[2] = {};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb) s[hb] = mfma(fo.row(kt, hb, kk), qf[kk], s[hb]);
+        // The tile's largest scaled score. Tiles that hold keys after a query
+        // scale first and mask (a uniform branch); the others take c max(s), or
+        // c min(s) for c < 0, and scale inside the exponent's FMA below.
+        float mx = -INFINITY, ce = c;
+        if (kbase + 63 > q0) {
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float t = s[hb][r] * c;
+                    if (kbase + 32 * hb + result_row(r, h) > qi) t = -INFINITY;
+                    s[hb][r] = t;
+                    mx = fmaxf(mx, t);
+                }
+            ce = 1.0f;
+        } else {
+#pragma unroll
+            for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, NEG ? -s[hb][r] : s[hb][r]);
+            mx *= NEG ? -c : c;
+        }
+        mx = fmaxf(mx, xor32(mx));
+        // m moves only when some query passes it by more than kRescale.
+        const float m_new = fmaxf(m, mx);
+        if (__any(m_new > m + kRescale)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+            m = m_new;
+        }
+        float sum = 0.0f;
+        f16x8 pf[4];
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hb][r], ce, -m));
+                pf[2 * hb + (r >> 3)][r & 7] = _Float16(p);
+                sum += p;
+            }
+        l += sum + xor32(sum);
+        // O^T += V^T P^T, a 16-key slice at a time (two for 64-wide heads).
+        constexpr int kSlices = HD == 64 ? 2 : 1;
+#pragma unroll
+        for (int cs = 0; cs < 4; cs += kSlices) {
+            TrFrag vf[kSlices][DB];
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) vf[i][db] = fo.transposed(vt, cs + i, db);
+            wait_lds();
+#pragma unroll
+            for (int i = 0; i < kSlices; ++i)
+#pragma unroll
+                for (int db = 0; db < DB; ++db)
+                    acc[db] = mfma(as_f16x8(vf[i][db]), pf[cs + i], acc[db]);
+        }
+    }
+    if (qi < length) {
+        store_row<HD>(out + size_t(w.begin + qi) * st.o + size_t(w.head) * HD, acc, 1.0f / l, h);
+        if (h == 0)
+            lse[size_t(w.head) * tokens + w.begin + qi] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+}
+
+// ---------------------------------------------------------------- backward: dQ (and D)
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, HD == 64 ? 3 : 2)
+packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
+                   const _Float16* __restrict__ q, const _Float16* __restrict__ k,
+                   const _Float16* __restrict__ v, const _Float16* __restrict__ o,
+                   const _Float16* __restrict__ dout, const float* __restrict__ lse,
+                   const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
+                   float c, float scale) {
+    constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    Work w;
+    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, h = lane >> 5;
+    const Frags<HD> fo(lane);
+    const int length = w.length;
+    const size_t o_at = size_t(w.begin) * st.o + size_t(w.head) * HD;
+    const size_t kv_at = size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
+    const size_t q_at = size_t(w.begin) * st.q + size_t(w.head) * HD;
+    const int q0 = w.block * kPackedBlock + wave * 32;
+    const int qi = q0 + fr;
+
+    f16x8 qf[KK], df[KK];
+    load_frags<HD>(qf, q + q_at, qi, length, st.q, h);
+    load_frags<HD>(df, dout + o_at, qi, length, st.o, h);
+    float dd = 0.0f;
+    {
+        f16x8 of[KK];
+        load_frags<HD>(of, o + o_at, qi, length, st.o, h);
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                dd = __builtin_fmaf(float(df[kk][e]), float(of[kk][e]), dd);
+    }
+    dd += xor32(dd);
+    const size_t row_at = size_t(w.head) * tokens + w.begin + qi;
+    const float lse2 = qi < length ? lse[row_at] * kLog2e : 0.0f;
+    if (qi < length && h == 0) dsum[row_at] = dd;
+
+    f32x16 acc[DB] = {};   // dQ^T[d][q]
+    const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
+    const int tiles = q_last / 64 + 1;
+    auto load = [&](int j) {
+        _Float16* t = lds + (j & 1) * 2 * kTile;
+        const size_t at = kv_at + size_t(64 * j) * st.kv;
+        load_tile<HD, 4>(t, k + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, 4>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
+    };
+    load(0);
+    for (int j = 0; j < tiles; ++j) {
+        wait_vmcnt<0>();
+        block_sync();
+        const _Float16* kt = lds + (j & 1) * 2 * kTile;
+        const _Float16* vt = kt + kTile;
+        if (j + 1 < tiles) load(j + 1);
+        const int kbase = 64 * j;
+        if (kbase > q0 + 31) continue;
+        const bool masked = kbase + 63 > q0;
+        // Two halves of 32 keys, each through all of its products before the
+        // next (fewer registers live at once).
+#pragma unroll
+        for (int hb = 0; hb < 2; ++hb) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                s = mfma(fo.row(kt, hb, kk), qf[kk], s);
+                dp = mfma(fo.row(vt, hb, kk), df[kk], dp);
+            }
+            f16x8 sf[2];
+            auto form = [&](auto mask) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    float p = __builtin_amdgcn_exp2f(s[r] * c - lse2);
+                    if constexpr (mask)
+                        if (kbase + 32 * hb + result_row(r, h) > qi) p = 0.0f;
+                    sf[r >> 3][r & 7] = _Float16(p * (dp[r] - dd));
+                }
+            };
+            if (masked) form(std::true_type{});
+            else form(std::false_type{});
+            // dQ^T += K^T dS^T.
+#pragma unroll
+            for (int cs = 0; cs < 2; ++cs) {
+                TrFrag kf[DB];
+#pragma unroll
+                for (int db = 0; db < DB; ++db) kf[db] = fo.transposed(kt, 2 * hb + cs, db);
+                wait_lds();
+#pragma unroll
+                for (int db = 0; db < DB; ++db) acc[db] = mfma(as_f16x8(kf[db]), sf[cs], acc[db]);
+            }
+        }
+    }
+    if (qi < length) store_row<HD>(dq + q_at + size_t(qi) * st.q, acc, scale, h);
+}
+
+// ---------------------------------------------------------------- backward: dK, dV
+
+// 128 keys (32 a wave) of one head of k and v; walks the 64-query tiles at or
+// after its first key, of each query head of the group in turn. A lane holds
+// one key and 16 queries per 32-query half, whose lse and D come from LDS.
+template <int HD>
+__global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1)
+packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
+                     const _Float16* __restrict__ q, const _Float16* __restrict__ k,
+                     const _Float16* __restrict__ v, const _Float16* __restrict__ dout,
+                     const float* __restrict__ lse, const float* __restrict__ dsum,
+                     const int4* __restrict__ plan, int tokens, int kv_heads, int group, Strides st,
+                     float c, float scale) {
+    constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][Q, dO]
+    __shared__ __attribute__((aligned(16))) float rowstat[2][2][64];       // [buf][lse, D]
+    Work w;
+    if (!work_of(plan, int(blockIdx.x), kv_heads, tokens, &w)) return;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, h = lane >> 5;
+    const Frags<HD> fo(lane);
+    const int length = w.length;
+    // The list's long blocks are the last of their sequences; as keys the first
+    // ones have the most queries.
+    const int block = (length + kPackedBlock - 1) / kPackedBlock - 1 - w.block;
+    const size_t kv_at = size_t(w.begin) * st.kv + size_t(w.head) * HD;
+    const int k0 = block * kPackedBlock + wave * 32;
+    const int ki = k0 + fr;
+
+    f16x8 kf[KK], vf[KK];
+    load_frags<HD>(kf, k + kv_at, ki, length, st.kv, h);
+    load_frags<HD>(vf, v + kv_at, ki, length, st.kv, h);
+    f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
+    const int first = block * kPackedBlock / 64;
+    const int per_head = (length + 63) / 64 - first;
+    const int steps = per_head * group;
+    auto stage = [&](int i) {
+        const int buf = i & 1, g = i / per_head, tile = first + i - g * per_head;
+        const int head = w.head * group + g;
+        _Float16* t = lds + buf * 2 * kTile;
+        const int qq = 64 * tile + lane;
+        float lv = 0.0f, dv0 = 0.0f;
+        if (wave == 0 && qq < length) {
+            const size_t at = size_t(head) * tokens + w.begin + qq;
+            lv = lse[at];
+            dv0 = dsum[at];
+        }
+        const size_t row = size_t(w.begin) + 64 * tile;
+        load_tile<HD, 4>(t, q + row * st.q + size_t(head) * HD, length - 64 * tile, st.q, wave, lane);
+        load_tile<HD, 4>(t + kTile, dout + row * st.o + size_t(head) * HD, length - 64 * tile, st.o,
+                         wave, lane);
+        if (wave == 0) {
+            rowstat[buf][0][lane] = lv * kLog2e;
+            rowstat[buf][1][lane] = dv0;
+        }
+    };
+    stage(0);
+    int tile = first;
+    for (int i = 0; i < steps; ++i) {
+        const int buf = i & 1;
+        wait_vmcnt<0>();
+        __syncthreads();
+        const _Float16* qt = lds + buf * 2 * kTile;
+        const _Float16* gt = qt + kTile;
+        const float* l2 = rowstat[buf][0];
+        const float* dd = rowstat[buf][1];
+        if (i + 1 < steps) stage(i + 1);
+        const int qbase = 64 * tile;
+        tile = tile + 1 == first + per_head ? first : tile + 1;
+        if (qbase + 63 < k0) continue;        // every query before every key of the wave
+        const bool masked = qbase < k0 + 31 || qbase + 63 >= length;
+#pragma unroll
+        for (int qh = 0; qh < 2; ++qh) {
+            f32x16 s = {}, dp = {};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                s = mfma(fo.row(qt, qh, kk), kf[kk], s);
+                dp = mfma(fo.row(gt, qh, kk), vf[kk], dp);
+            }
+            f16x8 pf[2], sf[2];
+            auto form = [&](auto mask) {
+#pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    const int qr = 32 * qh + 8 * a + 4 * h;   // query row in the tile, + e
+                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(l2 + qr);
+                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(dd + qr);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * a + e;
+                        float p = __builtin_amdgcn_exp2f(s[r] * c - l4[e]);
+                        if constexpr (mask) {
+                            if (ki > qbase + qr + e || qbase + qr + e >= length) p = 0.0f;
+                        }
+                        pf[a >> 1][4 * (a & 1) + e] = _Float16(p);
+                        sf[a >> 1][4 * (a & 1) + e] = _Float16(p * (dp[r] - d4[e]));
+                    }
+                }
+            };
+            if (masked) form(std::true_type{});
+            else form(std::false_type{});
+            // dV^T += dO^T P^T and dK^T += Q^T dS^T, a 16-query slice at a time.
+#pragma unroll
+            for (int cs = 0; cs < 2; ++cs) {
+                TrFrag gf[DB], tf[DB];
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    gf[db] = fo.transposed(gt, 2 * qh + cs, db);
+                    tf[db] = fo.transposed(qt, 2 * qh + cs, db);
+                }
+                wait_lds();
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    dva[db] = mfma(as_f16x8(gf[db]), pf[cs], dva[db]);
+                    dka[db] = mfma(as_f16x8(tf[db]), sf[cs], dka[db]);
+                }
+            }
+        }
+    }
+    if (ki < length) {
+        const size_t at = kv_at + size_t(ki) * st.kv;
+        store_row<HD>(dk + at, dka, scale, h);
+        store_row<HD>(dv + at, dva, 1.0f, h);
+    }
+}
+
+template <int HD>
+hipError_t forward(void* o, void* lse, const void* q, const void* k, const void* v,
+                   const void* plan, const flint_packed_shape& s, float scale,
+                   hipStream_t stream) {
+    auto* const kernel = scale < 0.0f ? packed_forward<HD, true> : packed_forward<HD, false>;
+    hipLaunchKernelGGL(kernel, dim3(unsigned(packed_items(s) * s.heads)), dim3(kThreads), 0, stream,
+                       static_cast<_Float16*>(o), static_cast<float*>(lse),
+                       static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
+                       static_cast<const _Float16*>(v), static_cast<const int4*>(plan),
+                       int(s.tokens), int(s.heads), int(s.heads / s.kv_heads),
+                       Strides{int(s.q_stride), int(s.kv_stride), int(s.o_stride)},
+                       scale * kLog2e);
+    return hipGetLastError();
+}
+
+template <int HD>
+hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* q, const void* k,
+                    const void* v, const void* o, const void* lse, const void* plan,
+                    const flint_packed_shape& s, float scale, void* workspace, hipStream_t stream) {
+    const Strides st{int(s.q_stride), int(s.kv_stride), int(s.o_stride)};
+    auto* dsum = static_cast<float*>(workspace);
+    const int group = int(s.heads / s.kv_heads);
+    hipLaunchKernelGGL(packed_backward_dq<HD>, dim3(unsigned(packed_items(s) * s.heads)),
+                       dim3(kThreads), 0, stream, static_cast<_Float16*>(dq), dsum,
+                       static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
+                       static_cast<const _Float16*>(v), static_cast<const _Float16*>(o),
+                       static_cast<const _Float16*>(dout), static_cast<const float*>(lse),
+                       static_cast<const int4*>(plan), int(s.tokens), int(s.heads), group, st,
+                       scale * kLog2e, scale);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(packed_items(s) * s.kv_heads)),
+                       dim3(kThreads), 0, stream, static_cast<_Float16*>(dk),
+                       static_cast<_Float16*>(dv), static_cast<const _Float16*>(q),
+                       static_cast<const _Float16*>(k), static_cast<const _Float16*>(v),
+                       static_cast<const _Float16*>(dout), static_cast<const float*>(lse),
+                       static_cast<const float*>(dsum), static_cast<const int4*>(plan),
+                       int(s.tokens), int(s.kv_heads), group, st, scale * kLog2e, scale);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+// D, one FP32 value a query and head.
+size_t packed_backward_workspace(const flint_packed_shape& s) { return s.heads * s.tokens * 4; }
+
+hipError_t launch_packed_plan(void* plan, const void* offsets, const flint_packed_shape& s,
+                              hipStream_t stream) {
+    // The longest possible sequence's blocks fit the buckets.
+    int shift = 0;
+    while (((s.tokens / kPackedBlock + 1) >> shift) >= size_t(kBuckets)) ++shift;
+    hipLaunchKernelGGL(packed_plan, dim3(1), dim3(kPlanThreads), 0, stream,
+                       static_cast<int4*>(plan), static_cast<const int*>(offsets),
+                       int(s.sequences), int(s.tokens), int(packed_items(s)), shift);
+    return hipGetLastError();
+}
+
+hipError_t launch_packed_forward(void* o, void* lse, const void* q, const void* k, const void* v,
+                                 const void* plan, const flint_packed_shape& s, float scale,
+                                 hipStream_t stream) {
+    return s.head_width == 64 ? forward<64>(o, lse, q, k, v, plan, s, scale, stream)
+                              : forward<128>(o, lse, q, k, v, plan, s, scale, stream);
+}
+
+hipError_t launch_packed_backward(void* dq, void* dk, void* dv, const void* dout, const void* q,
+                                  const void* k, const void* v, const void* o, const void* lse,
+                                  const void* plan, const flint_packed_shape& s, float scale,
+                                  void* workspace, hipStream_t stream) {
+    return s.head_width == 64
+               ? backward<64>(dq, dk, dv, dout, q, k, v, o, lse, plan, s, scale, workspace, stream)
+               : backward<128>(dq, dk, dv, dout, q, k, v, o, lse, plan, s, scale, workspace, stream);
+}
+
+}  // namespace flint

@@ -21,6 +21,9 @@ HEADER = ROOT / "include" / "flint" / "flint.h"
 TRAIN_HEADER = ROOT / "include" / "flint" / "flint_train.h"
 NOALLOC_HEADER = ROOT / "include" / "flint" / "flint_noalloc.h"
 ATTENTION_HEADER = ROOT / "include" / "flint" / "flint_attention.h"
+PACKED_HEADER = ROOT / "include" / "flint" / "flint_packed.h"
+PAGED_HEADER = ROOT / "include" / "flint" / "flint_paged.h"
+LOGPROBS_HEADER = ROOT / "include" / "flint" / "flint_logprobs.h"
 TUNING_HEADER = ROOT / "include" / "flint" / "flint_tuning.h"
 LIBRARY = ROOT / "build" / "release" / "bin" / "libflint.so"
 
@@ -71,6 +74,19 @@ class TrainState(ctypes.Structure):
                 ("found_inf", ctypes.c_int), ("grad_norm", ctypes.c_double), ("clip_coef", ctypes.c_double)]
 
 
+class PackedShape(ctypes.Structure):
+    """flint_packed_shape (include/flint/flint_packed.h)."""
+    _fields_ = [("tokens", Z), ("sequences", Z), ("heads", Z), ("kv_heads", Z), ("head_width", Z),
+                ("q_stride", Z), ("kv_stride", Z), ("o_stride", Z)]
+
+
+class PagedShape(ctypes.Structure):
+    """flint_paged_shape (include/flint/flint_paged.h)."""
+    _fields_ = [("tokens", Z), ("sequences", Z), ("max_new", Z), ("heads", Z), ("kv_heads", Z),
+                ("head_width", Z), ("q_stride", Z), ("kv_stride", Z), ("o_stride", Z), ("pages", Z),
+                ("page_size", Z), ("max_pages", Z)]
+
+
 SIGNATURES = {
     "flint_version": (ctypes.c_char_p, []),
     "flint_status_string": (ctypes.c_char_p, [I]),
@@ -98,6 +114,19 @@ SIGNATURES = {
     "flint_attention_backward": (I, [P, P, P, P, P, P, P, P, P, Z, Z, Z, F, P, Z, P]),
     "flint_gpt2_bytes_fused": (I, [ctypes.POINTER(Gpt2Config), ctypes.POINTER(Z)]),
     "flint_gpt2_create_fused": (I, [ctypes.POINTER(Gpt2Config), ctypes.POINTER(P)]),
+    # flint_packed.h (no counterpart in the reference)
+    "flint_attention_packed_plan_bytes": (I, [ctypes.POINTER(PackedShape), ctypes.POINTER(Z)]),
+    "flint_attention_packed_plan": (I, [P, P, ctypes.POINTER(PackedShape), P]),
+    "flint_attention_packed_forward": (I, [P, P, P, P, P, P, ctypes.POINTER(PackedShape), F, P]),
+    "flint_attention_packed_backward_workspace": (I, [ctypes.POINTER(PackedShape),
+                                                      ctypes.POINTER(Z)]),
+    "flint_attention_packed_backward": (I, [P] * 10 + [ctypes.POINTER(PackedShape), F, P, Z, P]),
+    # flint_paged.h (no counterpart in the reference)
+    "flint_attention_paged_workspace": (I, [ctypes.POINTER(PagedShape), ctypes.POINTER(Z)]),
+    "flint_attention_paged": (I, [P] * 9 + [ctypes.POINTER(PagedShape), F, P, Z, P]),
+    # flint_logprobs.h (no counterpart in the reference)
+    "flint_logprobs_forward": (I, [P] * 7 + [F, Z, Z, Z, Z, P]),
+    "flint_logprobs_backward": (I, [P] * 7 + [F, Z, Z, Z, P]),
     # flint_tuning.h (no counterpart in the reference)
     "flint_set_tuning": (I, [ctypes.c_char_p, ctypes.c_char_p]),
     "flint_gemm_nt_batched": (I, [P, P, P, Z, Z, Z, Z, F, P]),
@@ -364,6 +393,75 @@ class Flint:
             pointer(v), pointer(o), pointer(lse), batches, length, head_width, scale,
             pointer(workspace), workspace_bytes, stream_handle(stream)))
 
+    # -- attention over packed sequences (flint_packed.h) ----------------------
+    @staticmethod
+    def packed_shape(tokens, sequences, heads, kv_heads, head_width, q_stride=None, kv_stride=None,
+                     o_stride=None):
+        """A flint_packed_shape; a stride left out is the tensor's own width."""
+        return PackedShape(tokens, sequences, heads, kv_heads, head_width,
+                           heads * head_width if q_stride is None else q_stride,
+                           kv_heads * head_width if kv_stride is None else kv_stride,
+                           heads * head_width if o_stride is None else o_stride)
+
+    def attention_packed_plan_bytes(self, shape):
+        out = Z(0)
+        self.check(self.lib.flint_attention_packed_plan_bytes(shape, ctypes.byref(out)))
+        return out.value
+
+    def attention_packed_plan(self, plan, offsets, shape, stream=None):
+        self.check(self.lib.flint_attention_packed_plan(pointer(plan), pointer(offsets), shape,
+                                                        stream_handle(stream)))
+
+    def attention_packed_forward(self, o, lse, q, k, v, plan, shape, scale, stream=None):
+        self.check(self.lib.flint_attention_packed_forward(
+            pointer(o), pointer(lse), pointer(q), pointer(k), pointer(v), pointer(plan), shape,
+            scale, stream_handle(stream)))
+
+    def attention_packed_backward_workspace(self, shape):
+        out = Z(0)
+        self.check(self.lib.flint_attention_packed_backward_workspace(shape, ctypes.byref(out)))
+        return out.value
+
+    def attention_packed_backward(self, dq, dk, dv, dout, q, k, v, o, lse, plan, shape, scale,
+                                  workspace=None, workspace_bytes=None, stream=None):
+        if workspace is None:
+            import torch
+
+            workspace = torch.empty(max(self.attention_packed_backward_workspace(shape), 16),
+                                    dtype=torch.uint8, device="cuda")
+        if workspace_bytes is None:
+            workspace_bytes = workspace.numel() * workspace.element_size()
+        self.check(self.lib.flint_attention_packed_backward(
+            pointer(dq), pointer(dk), pointer(dv), pointer(dout), pointer(q), pointer(k),
+            pointer(v), pointer(o), pointer(lse), pointer(plan), shape, scale,
+            pointer(workspace), workspace_bytes, stream_handle(stream)))
+
+    # -- attention over a paged cache (flint_paged.h) --------------------------
+    @staticmethod
+    def paged_shape(tokens, sequences, max_new, heads, kv_heads, head_width, q_stride, kv_stride,
+                    o_stride, pages, page_size, max_pages):
+        return PagedShape(tokens, sequences, max_new, heads, kv_heads, head_width, q_stride,
+                          kv_stride, o_stride, pages, page_size, max_pages)
+
+    def attention_paged_workspace(self, shape):
+        out = Z(0)
+        self.check(self.lib.flint_attention_paged_workspace(shape, ctypes.byref(out)))
+        return out.value
+
+    def attention_paged(self, o, k_pages, v_pages, q, k, v, offsets, cached, table, shape, scale,
+                        workspace=None, workspace_bytes=None, stream=None):
+        if workspace is None:
+            import torch
+
+            workspace = torch.empty(max(self.attention_paged_workspace(shape), 16),
+                                    dtype=torch.uint8, device="cuda")
+        if workspace_bytes is None:
+            workspace_bytes = workspace.numel() * workspace.element_size()
+        self.check(self.lib.flint_attention_paged(
+            pointer(o), pointer(k_pages), pointer(v_pages), pointer(q), pointer(k), pointer(v),
+            pointer(offsets), pointer(cached), pointer(table), shape, scale, pointer(workspace),
+            workspace_bytes, stream_handle(stream)))
+
     def bias_gradient_noalloc(self, dbias, dy, rows, cols, accumulate=False, stream=None):
         """flint_bias_gradient with the library's own scratch array (no workspace)."""
         self.check(self.lib.flint_bias_gradient_noalloc(pointer(dbias), pointer(dy), rows, cols,
@@ -423,6 +521,21 @@ class Flint:
         self.check(self.lib.flint_softmax_cross_entropy(pointer(dlogits), pointer(row_loss),
                                                         pointer(logits), pointer(targets), scale,
                                                         rows, vocab, cols, stream_handle(stream)))
+
+    # -- log probabilities (flint_logprobs.h) ----------------------------------
+    def logprobs_forward(self, logprob, entropy, stats, top_ids, top_logprobs, logits, targets,
+                         scale, rows, vocab, cols, top=0, stream=None):
+        self.check(self.lib.flint_logprobs_forward(
+            pointer(logprob), pointer(entropy), pointer(stats), pointer(top_ids),
+            pointer(top_logprobs), pointer(logits), pointer(targets), scale, rows, vocab, cols, top,
+            stream_handle(stream)))
+
+    def logprobs_backward(self, dlogits, dlogprob, dentropy, logits, targets, entropy, stats, scale,
+                          rows, vocab, cols, stream=None):
+        self.check(self.lib.flint_logprobs_backward(
+            pointer(dlogits), pointer(dlogprob), pointer(dentropy), pointer(logits),
+            pointer(targets), pointer(entropy), pointer(stats), scale, rows, vocab, cols,
+            stream_handle(stream)))
 
     # -- data movement --------------------------------------------------------
     def fp32_to_fp16(self, y, x, count, stream=None):
@@ -556,10 +669,11 @@ class Gpt2:
 
 def declared_functions(header=None):
     """Names of every FLINT_API function a header declares; by default those of
-    flint.h and of the training-step extension, flint_train.h."""
+    flint.h and of every additive header."""
     import re
 
     headers = ([header] if header is not None
-               else [HEADER, TRAIN_HEADER, NOALLOC_HEADER, ATTENTION_HEADER, TUNING_HEADER])
+               else [HEADER, TRAIN_HEADER, NOALLOC_HEADER, ATTENTION_HEADER, PACKED_HEADER,
+                     PAGED_HEADER, LOGPROBS_HEADER, TUNING_HEADER])
     text = "".join(Path(h).read_text() for h in headers)
     return re.findall(r"FLINT_API\s+[^;(]*?\b(flint_\w+)\s*\(", text)
