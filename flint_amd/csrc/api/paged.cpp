@@ -35,6 +35,13 @@ Checker& paged_sizes(Checker& c, const flint_paged_shape* s) {
                  s->pages, size_t{0x7fffffff})
         .require(s->max_pages != 0 && s->max_pages <= columns, "max_pages (%zu) must be from 1 to %zu",
                  s->max_pages, columns);
+    if (c.ok())
+        c.require(s->tokens * s->heads <= flint::kPagedMaxRows,
+                  "tokens x heads (%zu) can be up to %zu", s->tokens * s->heads,
+                  flint::kPagedMaxRows)
+            .require(s->sequences * s->kv_heads <= flint::kPagedMaxRows / 8,
+                     "sequences x kv_heads (%zu) can be up to %zu", s->sequences * s->kv_heads,
+                     flint::kPagedMaxRows / 8);
     const struct {
         const char* name;
         size_t stride, width;

@@ -2,7 +2,21 @@
 // cached positions of its sequence and the sequence's new tokens up to itself;
 // the new rows of k and v go into their pages in the same launch, and are read
 // from k and v here, so no workgroup waits for another's store.
+//
+// The rows that share a head of K and V are taken together: row r of a sequence
+// and kv head is new token r / group, query head r % group of the group. A work
+// item is a block of such rows and a part of the sequence's 64- or 32-key tiles;
+// the parts are joined by a second, small launch. Two kernels:
+//  * few rows (up to 32: generation). Reading the cache bounds it: 2 values of
+//    K and V a key and column against 4 FLOPs a row. Each of the four waves
+//    streams tiles of its own through LDS, two in flight, with no barrier until
+//    the waves' results are joined at the end.
+//  * many rows (chunks of prompts). Each wave takes 32 of 128 rows, and the four
+//    share the tiles, as in packed.hip.
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "common/common.h"
 #include "kernels/attention_tiles.h"
@@ -11,14 +25,39 @@
 namespace flint {
 namespace {
 
+constexpr int kThreads = 256;   // 4 waves
+constexpr float kRescale = 8.0f;
+// A running maximum below every score: a tile may hold no visible key, and
+// exp2(-inf - kFloor) is 0.
+constexpr float kFloor = -3e38f;
+constexpr int kFewRows = 32, kManyRows = 128;
+// Workgroups aimed at, and the fewest tiles that a part of a sequence takes.
+constexpr int kFewTarget = 512, kManyTarget = 512;
+constexpr int kFewTiles = 8, kManyTiles = 4;
+
+template <int HD, bool MANY>
+struct Plan {
+    static constexpr int kRows = MANY ? kManyRows : kFewRows;
+    static constexpr int kKeys = MANY || HD == 64 ? 64 : 32;   // of a tile
+    static constexpr int kLeast = MANY ? kManyTiles : kFewTiles;
+};
+
 struct PagedArgs {
     _Float16 *o, *k_pages, *v_pages;
     const _Float16 *q, *k, *v;
     const int *offsets, *cached, *table;
-    int tokens, sequences, max_new, heads, kv_heads;
+    int tokens, sequences, max_new, heads, kv_heads, group;
     int q_stride, kv_stride, o_stride;
     int pages, page_size, max_pages;
-    float c;   // scale log2 e
+    unsigned long long magic;   // column of position p: (p magic) >> shift
+    int shift;
+    float c;       // |scale| log2 e
+    int negative;  // scale < 0: q enters negated
+    int target;    // items a kv head aimed at
+    int slots;     // parts that the workspace holds, a kv head
+    int2* splits;  // [sequences]: first slot, parts
+    float2* sums;  // [slots][kv_heads][rows]: maximum (log2 units), sum
+    float* parts;  // [slots][kv_heads][rows][HD]
 };
 
 // Sequence s: its new tokens' first row and count, and its cached positions.
@@ -33,109 +72,548 @@ __device__ __forceinline__ Sequence sequence_of(const PagedArgs& a, int s) {
     return q;
 }
 
-// The page of position p of sequence s, or -1.
-__device__ __forceinline__ int page_of(const PagedArgs& a, int s, int p) {
-    const int column = p / a.page_size;
-    if (column >= a.max_pages) return -1;
-    const int page = a.table[size_t(s) * a.max_pages + column];
-    return page >= 0 && page < a.pages ? page : -1;
-}
-template <int HD>
-__device__ __forceinline__ size_t row_in_pages(const PagedArgs& a, int page, int head, int p) {
-    return ((size_t(page) * a.kv_heads + head) * a.page_size + p % a.page_size) * HD;
+// The table column of a position: an exact division by page_size, as a product
+// (positions stay below 2^31).
+__device__ __forceinline__ int column_of(const PagedArgs& a, int p) {
+    return int((unsigned long long)(unsigned(p)) * a.magic >> a.shift);
 }
 
-// One wave a token and head: a lane takes a key of each 64, then a column of V.
+template <class T>
+__device__ __forceinline__ T wave_sum(T v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ int wave_scan(int v, int lane) {   // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int w = __shfl_up(v, d);
+        if (lane >= d) v += w;
+    }
+    return v;
+}
+
+// Item `idx` of a kv head. Every item takes about the same number of tiles,
+// total / target: the sequences' lengths are known only here, so each wave adds
+// them up (64 sequences a step) and finds its item by a prefix sum.
+struct Item {
+    Sequence seq;
+    int s, block, part, parts, slot;   // slot of the block's part 0 (parts > 1)
+};
+template <int HD, bool MANY>
+__device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane, Item* it) {
+    using P = Plan<HD, MANY>;
+    auto blocks_of = [&](const Sequence& q) { return (q.count * a.group + P::kRows - 1) / P::kRows; };
+    auto tiles_of = [&](const Sequence& q) {
+        return q.count == 0 ? 0 : int(unsigned(q.cached + q.count + P::kKeys - 1) / P::kKeys);
+    };
+    long long total = 0;
+    Sequence q{};
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        q = Sequence{};
+        if (s0 + lane < a.sequences) q = sequence_of(a, s0 + lane);
+        total += (long long)(blocks_of(q)) * tiles_of(q);
+    }
+    total = wave_sum(total);
+    const int each = max(P::kLeast, int((total + a.target - 1) / a.target));
+    int before = 0, slots = 0;
+    for (int s0 = 0; s0 < a.sequences; s0 += 64) {
+        if (a.sequences > 64) {
+            q = Sequence{};
+            if (s0 + lane < a.sequences) q = sequence_of(a, s0 + lane);
+        }
+        const int parts = (tiles_of(q) + each - 1) / each;
+        const int items = blocks_of(q) * parts;
+        const int upto = wave_scan(items, lane);
+        const int held = wave_scan(parts > 1 ? items : 0, lane);
+        const unsigned long long past = __ballot(before + upto > idx);
+        if (past != 0) {
+            const int at = __ffsll(past) - 1;
+            auto get = [&](int v) { return __builtin_amdgcn_readlane(v, at); };
+            it->s = s0 + at;
+            it->seq = {get(q.first), get(q.count), get(q.cached)};
+            it->parts = get(parts);
+            const int in = idx - before - get(upto - items);
+            it->block = in / it->parts;
+            it->part = in - it->block * it->parts;
+            it->slot = slots + get(held) - get(parts > 1 ? items : 0) + it->block * it->parts;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+        slots += __builtin_amdgcn_readlane(held, 63);
+    }
+    return false;
+}
+
+// Reads the rows of K and V of one sequence and kv head, wherever they lie.
 template <int HD>
-__global__ void __launch_bounds__(256) paged_rows(PagedArgs a) {
-    const int lane = threadIdx.x & 63;
-    const int head = (blockIdx.x * 4 + (threadIdx.x >> 6)) % a.heads;
-    const int place = (blockIdx.x * 4 + (threadIdx.x >> 6)) / a.heads;
-    const int s = blockIdx.y;
-    const Sequence sq = sequence_of(a, s);
-    if (place >= sq.count) return;
-    const int group = a.heads / a.kv_heads, kv = head / group;
-    const _Float16* qr = a.q + size_t(sq.first + place) * a.q_stride + size_t(head) * HD;
-    if (head % group == 0) {
-        const int page = page_of(a, s, sq.cached + place);
-        const size_t from = size_t(sq.first + place) * a.kv_stride + size_t(kv) * HD;
-        if (page >= 0) {
-            const size_t to = row_in_pages<HD>(a, page, kv, sq.cached + place);
-            for (int d = lane; d < HD; d += 64) {
-                a.k_pages[to + d] = a.k[from + d];
-                a.v_pages[to + d] = a.v[from + d];
-            }
-        }
+struct Reader {
+    using T = Tile<HD>;
+    const PagedArgs& a;
+    const int* table;
+    int kv, cached, total;
+    const _Float16 *k, *v;   // the sequence's first new row of this head
+    int row, lane;           // this lane's row of a load
+
+    __device__ __forceinline__ Reader(const PagedArgs& args, const Item& it, int head, int lane_)
+        : a(args), table(args.table + size_t(it.s) * args.max_pages), kv(head),
+          cached(it.seq.cached), total(it.seq.cached + it.seq.count),
+          k(args.k + size_t(it.seq.first) * args.kv_stride + size_t(head) * HD),
+          v(args.v + size_t(it.seq.first) * args.kv_stride + size_t(head) * HD),
+          row(lane_ / T::kChunks), lane(lane_) {}
+
+    static __device__ __forceinline__ void into(_Float16* lds, __amdgpu_buffer_rsrc_t rs,
+                                                unsigned at) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rs, (__attribute__((address_space(3))) void*)(lds_half*)lds, 16, at, 0, 0, 0);
     }
-    const int keys = sq.cached + place + 1;
-    float m = -3e38f, l = 0.0f, acc[HD / 64] = {};
-    for (int base = 0; base < keys; base += 64) {
-        const int p = base + lane;
-        const _Float16 *kr = nullptr, *vr = nullptr;
-        if (p < keys) {
-            if (p >= sq.cached) {
-                const size_t at = size_t(sq.first + p - sq.cached) * a.kv_stride + size_t(kv) * HD;
-                kr = a.k + at;
-                vr = a.v + at;
-            } else if (const int page = page_of(a, s, p); page >= 0) {
-                const size_t at = row_in_pages<HD>(a, page, kv, p);
-                kr = a.k_pages + at;
-                vr = a.v_pages + at;
-            }
+
+    // Load u of a tile of K and of V, its rows the positions p0 on: one load
+    // each at least. Rows of no position, or of no page, are zeros. Whether the
+    // cached positions among them have a page.
+    __device__ __forceinline__ bool load(_Float16* kt, _Float16* vt, int p0, int u) const {
+        const int chunk = (lane % T::kChunks) ^ T::key(u * T::kLoadRows + row);
+        const int column = column_of(a, p0);
+        const int page = p0 < cached ? table[column] : -1;   // cached ends inside the table
+        const bool ok = page >= 0 && page < a.pages;
+        const unsigned held = ok ? unsigned(min(cached - p0, T::kLoadRows)) * HD * 2 : 0u;
+        const size_t from =
+            ((size_t(ok ? page : 0) * a.kv_heads + kv) * a.page_size + (p0 - column * a.page_size)) *
+            HD;
+        const unsigned at = unsigned(row * HD + chunk * 8) * 2;
+        if (p0 + T::kLoadRows <= cached || p0 >= total) {
+            into(kt + u * 512, rsrc_of(a.k_pages + (ok ? from : 0), held), at);
+            into(vt + u * 512, rsrc_of(a.v_pages + (ok ? from : 0), held), at);
+        } else if (p0 + row < cached) {
+            into(kt + u * 512, rsrc_of(a.k_pages + (ok ? from : 0), held), at);
+            into(vt + u * 512, rsrc_of(a.v_pages + (ok ? from : 0), held), at);
+        } else {
+            const int skip = max(p0 - cached, 0);   // new rows before this load's
+            const int rows = min(total - cached - skip, T::kLoadRows);
+            const unsigned bytes = unsigned((rows - 1) * a.kv_stride + HD) * 2;
+            const unsigned here = unsigned((p0 + row - cached - skip) * a.kv_stride + chunk * 8) * 2;
+            into(kt + u * 512, rsrc_of(k + size_t(skip) * a.kv_stride, bytes), here);
+            into(vt + u * 512, rsrc_of(v + size_t(skip) * a.kv_stride, bytes), here);
         }
-        float x = -INFINITY;
-        if (kr != nullptr) {
-            float dot = 0.0f;
-            for (int d = 0; d < HD; d += 8) {
-                const f16x8 kv8 = *reinterpret_cast<const f16x8*>(kr + d);
-                const f16x8 qv8 = *reinterpret_cast<const f16x8*>(qr + d);
-                for (int e = 0; e < 8; ++e) dot = __builtin_fmaf(float(kv8[e]), float(qv8[e]), dot);
-            }
-            x = dot * a.c;
+        return ok || p0 >= cached;
+    }
+};
+
+// One tile of KEYS keys for a wave's 32 rows: scores, running maximum and sum,
+// O^T += V^T P^T. valid: bit u for load u's pages.
+template <int HD, int KEYS>
+struct Rows {
+    static constexpr int KK = HD / 16, DB = HD / 32, HB = KEYS / 32;
+    f16x8 q[KK];
+    float m = kFloor, l = 0.0f;
+    f32x16 acc[DB] = {};
+
+    __device__ __forceinline__ void tile(const _Float16* kt, const _Float16* vt,
+                                         const Frags<HD>& fo, int kbase, unsigned valid, int cached,
+                                         int last, float c, int h) {
+        f32x16 s[HB] = {};
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) s[hb] = mfma(fo.row(kt, hb, kk), q[kk], s[hb]);
+        constexpr unsigned kAll = unsigned((1ull << (KEYS / Tile<HD>::kLoadRows)) - 1);
+        float mx = kFloor, ce = c;
+        if (kbase + KEYS > cached || valid != kAll) {
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int in = 32 * hb + result_row(r, h), p = kbase + in;
+                    const bool paged = (valid >> (in / Tile<HD>::kLoadRows)) & 1;
+                    const bool seen = p <= last && (paged || p >= cached);
+                    const float t = seen ? s[hb][r] * c : -INFINITY;
+                    s[hb][r] = t;
+                    mx = fmaxf(mx, t);
+                }
+            ce = 1.0f;
+        } else {
+            mx = -INFINITY;
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[hb][r]);
+            mx *= c;
         }
-        float mx = x;
-        for (int d = 32; d > 0; d /= 2) mx = fmaxf(mx, __shfl_xor(mx, d));
+        mx = fmaxf(mx, xor32(mx));
         const float m_new = fmaxf(m, mx);
-        const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-        const float pr = __builtin_amdgcn_exp2f(x - m_new);
-        float sum = pr;
-        for (int d = 32; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-        l = l * alpha + sum;
-        m = m_new;
-        for (int i = 0; i < HD / 64; ++i) acc[i] *= alpha;
-        for (int j = 0; j < 64; ++j) {
-            const auto row = reinterpret_cast<const _Float16*>(
-                __shfl(reinterpret_cast<unsigned long long>(vr), j));
-            if (row == nullptr) continue;
-            const float pj = __shfl(pr, j);
-            for (int i = 0; i < HD / 64; ++i)
-                acc[i] = __builtin_fmaf(pj, float(row[64 * i + lane]), acc[i]);
+        if (__any(m_new > m + kRescale)) {
+            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
+            l *= alpha;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
+            m = m_new;
+        }
+        float sum = 0.0f;
+        f16x8 p[2 * HB];
+#pragma unroll
+        for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hb][r], ce, -m));
+                p[2 * hb + (r >> 3)][r & 7] = _Float16(e);
+                sum += e;
+            }
+        l += sum + xor32(sum);
+#pragma unroll
+        for (int cs = 0; cs < 2 * HB; ++cs) {
+            TrFrag vf[DB];
+#pragma unroll
+            for (int db = 0; db < DB; ++db) vf[db] = fo.transposed(vt, cs, db);
+            wait_lds();
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] = mfma(as_f16x8(vf[db]), p[cs], acc[db]);
         }
     }
-    _Float16* orow = a.o + size_t(sq.first + place) * a.o_stride + size_t(head) * HD;
-    for (int i = 0; i < HD / 64; ++i) orow[64 * i + lane] = _Float16(acc[i] / l);
+
+    // Rows `row` of the sequence (32 from the wave's first), zeros from `rows` on.
+    __device__ __forceinline__ void load_q(const PagedArgs& a, const Item& it, int head, int row,
+                                           int rows, int h) {
+        const int place = row / a.group;
+        const _Float16* at = a.q + size_t(it.seq.first + place) * a.q_stride +
+                             size_t(head * a.group + row - place * a.group) * HD + 8 * h;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) {
+            q[kk] = row < rows ? *reinterpret_cast<const f16x8*>(at + 16 * kk) : f16x8{};
+            if (a.negative) q[kk] = -q[kk];
+        }
+    }
+};
+
+// The tiles of a block's part: the keys up to its last row's own position.
+__device__ __forceinline__ void part_of(const PagedArgs& a, const Item& it, int rows_of_block,
+                                        int keys, int* from, int* to) {
+    const int rows = it.seq.count * a.group;
+    const int place = (min((it.block + 1) * rows_of_block, rows) - 1) / a.group;
+    const int tiles = (it.seq.cached + place) / keys + 1;
+    *from = int((long long)(tiles) * it.part / it.parts);
+    *to = int((long long)(tiles) * (it.part + 1) / it.parts);
+}
+
+// The new rows of k and v that start in a block of query rows go to their
+// pages; a block's part 0 does it.
+template <int HD>
+__device__ __forceinline__ void store_new(const PagedArgs& a, const Item& it, int head,
+                                          int rows_of_block) {
+    if (it.part != 0) return;
+    const int from = (it.block * rows_of_block + a.group - 1) / a.group;
+    const int to = min(((it.block + 1) * rows_of_block + a.group - 1) / a.group, it.seq.count);
+    for (int i = threadIdx.x; i < (to - from) * (HD / 8); i += kThreads) {
+        const int place = from + i / (HD / 8), d = i % (HD / 8) * 8;
+        const int p = it.seq.cached + place, column = column_of(a, p);
+        if (column >= a.max_pages) continue;
+        const int page = a.table[size_t(it.s) * a.max_pages + column];
+        if (page < 0 || page >= a.pages) continue;
+        const size_t src = size_t(it.seq.first + place) * a.kv_stride + size_t(head) * HD + d;
+        const size_t dst =
+            ((size_t(page) * a.kv_heads + head) * a.page_size + (p - column * a.page_size)) * HD + d;
+        *reinterpret_cast<f16x8*>(a.k_pages + dst) = *reinterpret_cast<const f16x8*>(a.k + src);
+        *reinterpret_cast<f16x8*>(a.v_pages + dst) = *reinterpret_cast<const f16x8*>(a.v + src);
+    }
+}
+
+// Where the joining launch finds a sequence's parts.
+__device__ __forceinline__ void store_splits(const PagedArgs& a, const Item& it, int head) {
+    if (a.slots > 0 && head == 0 && it.block == 0 && it.part == 0 && threadIdx.x == 0)
+        a.splits[it.s] = int2{it.slot, it.parts};
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
+    using P = Plan<HD, false>;
+    constexpr int kTile = 4096;   // halves: 8 KB of K and of V
+    __shared__ __attribute__((aligned(16))) _Float16 lds[4 * 2 * 2 * kTile];   // [wave][buf][K, V]
+    __shared__ float2 wave_sums[4][32];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, h = lane >> 5;
+    const int head = int(blockIdx.x % unsigned(a.kv_heads));
+    Item it;
+    if (!find_item<HD, false>(a, int(blockIdx.x / unsigned(a.kv_heads)), lane, &it)) return;
+    store_splits(a, it, head);
+    const int rows = it.seq.count * a.group, first_row = it.block * kFewRows;
+    const Frags<HD> fo(lane);
+    Rows<HD, P::kKeys> w;
+    w.load_q(a, it, head, first_row + fr, rows, h);
+    const int last = it.seq.cached + (first_row + fr) / a.group;
+    const Reader<HD> reader(a, it, head, lane);
+    int from, to;
+    part_of(a, it, kFewRows, P::kKeys, &from, &to);
+    _Float16* mine = lds + wave * 4 * kTile;
+    auto issue = [&](int t, int buf) __attribute__((always_inline)) {
+        _Float16* kt = mine + buf * 2 * kTile;
+        unsigned valid = 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            valid |= unsigned(reader.load(kt, kt + kTile, t * P::kKeys + u * Tile<HD>::kLoadRows, u))
+                     << u;
+        return valid;
+    };
+    int t = from + wave;
+    unsigned valid = 0;
+    if (t < to) valid = issue(t, 0);
+    for (int i = 0; t < to; ++i, t += 4) {
+        unsigned next = 0;
+        // The other buffer's reads ended with the last tile's products.
+        asm volatile("" ::: "memory");
+        if (t + 4 < to) {
+            next = issue(t + 4, (i + 1) & 1);
+            wait_vmcnt<16>();   // the newer tile's 8 loads of K and 8 of V, at least
+        } else {
+            wait_vmcnt<0>();
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        const _Float16* kt = mine + (i & 1) * 2 * kTile;
+        w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
+        valid = next;
+    }
+    // Joins the waves: each leaves O^T [HD][32] in its own tiles.
+    float* own = reinterpret_cast<float*>(mine);
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) own[(32 * db + result_row(r, h)) * 32 + fr] = w.acc[db][r];
+    if (h == 0) wave_sums[wave][fr] = float2{w.m, w.l};
+    __syncthreads();
+    const int row = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * (HD / 8);
+    if (first_row + row < rows) {
+        float m = kFloor, l = 0.0f, by[4], sum[HD / 8] = {};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m = fmaxf(m, wave_sums[i][row].x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            by[i] = __builtin_amdgcn_exp2f(wave_sums[i][row].x - m);
+            l = __builtin_fmaf(wave_sums[i][row].y, by[i], l);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float* part = reinterpret_cast<const float*>(lds + i * 4 * kTile);
+#pragma unroll
+            for (int d = 0; d < HD / 8; ++d)
+                sum[d] = __builtin_fmaf(part[(d0 + d) * 32 + row], by[i], sum[d]);
+        }
+        if (it.parts == 1) {
+            const int place = (first_row + row) / a.group;
+            _Float16* o = a.o + size_t(it.seq.first + place) * a.o_stride +
+                          size_t(head * a.group + first_row + row - place * a.group) * HD + d0;
+            const float inv = 1.0f / l;
+#pragma unroll
+            for (int d = 0; d < HD / 8; d += 8) {
+                f16x8 v;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = _Float16(sum[d + e] * inv);
+                *reinterpret_cast<f16x8*>(o + d) = v;
+            }
+        } else {
+            const size_t at = (size_t(it.slot + it.part) * a.kv_heads + head) * kFewRows + row;
+            if (d0 == 0) a.sums[at] = float2{m, l};
+#pragma unroll
+            for (int d = 0; d < HD / 8; d += 4)
+                *reinterpret_cast<f32x4*>(a.parts + at * HD + d0 + d) =
+                    f32x4{sum[d], sum[d + 1], sum[d + 2], sum[d + 3]};
+        }
+    }
+    store_new<HD>(a, it, head, kFewRows);
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
+    using P = Plan<HD, true>;
+    constexpr int kTile = Tile<HD>::kHalves;
+    constexpr int kEach = Tile<HD>::kLoads / 4;   // loads of a wave, of K and of V
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    __shared__ int paged[2][16];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int fr = lane & 31, h = lane >> 5;
+    const int head = int(blockIdx.x % unsigned(a.kv_heads));
+    Item it;
+    if (!find_item<HD, true>(a, int(blockIdx.x / unsigned(a.kv_heads)), lane, &it)) return;
+    store_splits(a, it, head);
+    const int rows = it.seq.count * a.group, first_row = it.block * kManyRows + wave * 32;
+    const Frags<HD> fo(lane);
+    Rows<HD, P::kKeys> w;
+    w.load_q(a, it, head, first_row + fr, rows, h);
+    const int last = it.seq.cached + (first_row + fr) / a.group;
+    const int wave_last = it.seq.cached + (min(first_row + 32, rows) - 1) / a.group;
+    const Reader<HD> reader(a, it, head, lane);
+    int from, to;
+    part_of(a, it, kManyRows, P::kKeys, &from, &to);
+    auto issue = [&](int t) __attribute__((always_inline)) {
+        _Float16* kt = lds + (t & 1) * 2 * kTile;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const int u = wave + 4 * i;
+            const bool ok = reader.load(kt, kt + kTile, t * P::kKeys + u * Tile<HD>::kLoadRows, u);
+            if (lane == 0) paged[t & 1][u] = ok;
+        }
+    };
+    if (from < to) issue(from);
+    for (int t = from; t < to; ++t) {
+        wait_vmcnt<0>();
+        block_sync();
+        if (t + 1 < to) issue(t + 1);
+        if (first_row >= rows || t * P::kKeys > wave_last) continue;   // no row here, or none sees it
+        const unsigned valid =
+            unsigned(__ballot(lane < Tile<HD>::kLoads && paged[t & 1][lane & 15] != 0));
+        const _Float16* kt = lds + (t & 1) * 2 * kTile;
+        w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
+    }
+    wait_vmcnt<0>();
+    const int row = first_row + fr;
+    if (row < rows) {
+        if (it.parts == 1) {
+            const int place = row / a.group;
+            store_row<HD>(a.o + size_t(it.seq.first + place) * a.o_stride +
+                              size_t(head * a.group + row - place * a.group) * HD,
+                          w.acc, 1.0f / w.l, h);
+        } else {
+            const size_t at =
+                (size_t(it.slot + it.part) * a.kv_heads + head) * kManyRows + wave * 32 + fr;
+            if (h == 0) a.sums[at] = float2{w.m, w.l};
+#pragma unroll
+            for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<f32x4*>(a.parts + at * HD + 32 * db + 8 * i + 4 * h) =
+                        f32x4{w.acc[db][4 * i], w.acc[db][4 * i + 1], w.acc[db][4 * i + 2],
+                              w.acc[db][4 * i + 3]};
+        }
+    }
+    store_new<HD>(a, it, head, kManyRows);
+}
+
+// The sequence that token t belongs to, or -1: 64 offsets a step.
+__device__ __forceinline__ int sequence_at(const PagedArgs& a, int t, int lane) {
+    int low = 0, count = a.sequences;   // among low .. low + count - 1
+    while (count > 1) {
+        const int step = (count + 63) / 64;
+        const int s = low + lane * step;
+        const bool starts = lane * step < count && min(max(a.offsets[s], 0), a.tokens) <= t;
+        const int at = __popcll(__ballot(starts)) - 1;
+        if (at < 0) return -1;
+        low += at * step;
+        count = min(step, count - at * step);
+    }
+    const Sequence q = sequence_of(a, low);
+    return t >= q.first && t < q.first + q.count ? low : -1;
+}
+
+// One wave a row: the parts' results, weighted by their maxima's distance.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_block) {
+    const int lane = threadIdx.x & 63;
+    const size_t id = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    const int t = int(id / unsigned(a.heads)), head = int(id % unsigned(a.heads));
+    if (t >= a.tokens) return;
+    const int s = sequence_at(a, t, lane);
+    if (s < 0) return;
+    const Sequence q = sequence_of(a, s);
+    const int2 split = a.splits[s];
+    const int kv = head / a.group, row = (t - q.first) * a.group + head - kv * a.group;
+    const int block = row / rows_of_block, first = split.x + block * split.y;
+    // Slots outside the workspace can come from offsets that decrease only.
+    if (split.y <= 1 || first < 0 || first + split.y > a.slots) return;
+    auto slot = [&](int p) {
+        return (size_t(first + p) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
+    };
+    float m = kFloor, l = 0.0f, sum[HD / 64] = {};
+    for (int p = lane; p < split.y; p += 64) m = fmaxf(m, a.sums[slot(p)].x);
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
+    for (int p = 0; p < split.y; ++p) {
+        const float2 part = a.sums[slot(p)];
+        const float by = __builtin_amdgcn_exp2f(part.x - m);
+        l = __builtin_fmaf(part.y, by, l);
+#pragma unroll
+        for (int i = 0; i < HD / 64; ++i)
+            sum[i] = __builtin_fmaf(a.parts[slot(p) * HD + 64 * i + lane], by, sum[i]);
+    }
+    _Float16* o = a.o + size_t(t) * a.o_stride + size_t(head) * HD;
+#pragma unroll
+    for (int i = 0; i < HD / 64; ++i) o[64 * i + lane] = _Float16(sum[i] / l);
+}
+
+bool many_rows(const flint_paged_shape& s) {
+    return std::min(s.max_new, s.tokens) * (s.heads / s.kv_heads) > kFewRows;
+}
+
+// What the kernels' grids and the workspace follow from. A block of rows may
+// have as many parts as the longest sequence has runs of kLeast tiles; a
+// sequence in p > 1 parts of `each` tiles has fewer than 2 tiles / each of them,
+// so the parts of all are below 2 target.
+struct Sizes {
+    size_t target, blocks, slots, rows;
+};
+Sizes sizes_of(const flint_paged_shape& s) {
+    const bool many = many_rows(s);
+    Sizes z;
+    z.rows = many ? kManyRows : kFewRows;
+    const size_t keys = many || s.head_width == 64 ? 64 : 32;
+    const size_t least = many ? kManyTiles : kFewTiles;
+    const size_t group = s.heads / s.kv_heads, new_rows = std::min(s.max_new, s.tokens) * group;
+    z.target = std::max<size_t>(1, (many ? kManyTarget : kFewTarget) / s.kv_heads);
+    z.blocks = std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
+                        s.tokens * group / z.rows + s.sequences);
+    const size_t longest = (s.max_pages * s.page_size + s.max_new + keys - 1) / keys;
+    const size_t parts = (longest + least - 1) / least;
+    z.slots = parts > 1 ? std::min(2 * z.target, z.blocks * parts) : 0;
+    return z;
+}
+
+// The workspace: the sequences' splits, the parts' sums, the parts.
+struct Space {
+    size_t sums, parts, bytes;
+};
+Space space_of(const flint_paged_shape& s, const Sizes& z) {
+    const size_t rows = z.slots * s.kv_heads * z.rows;
+    Space w;
+    w.sums = (s.sequences * sizeof(int2) + 15) / 16 * 16;
+    w.parts = w.sums + rows * sizeof(float2);
+    w.bytes = z.slots == 0 ? 0 : w.parts + rows * s.head_width * 4;
+    return w;
 }
 
 }  // namespace
 
-size_t paged_workspace(const flint_paged_shape&) { return 0; }
+size_t paged_workspace(const flint_paged_shape& s) { return space_of(s, sizes_of(s)).bytes; }
 
 hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const void* q,
                                   const void* k, const void* v, const void* offsets,
                                   const void* cached, const void* table,
-                                  const flint_paged_shape& s, float scale, void*,
+                                  const flint_paged_shape& s, float scale, void* workspace,
                                   hipStream_t stream) {
+    const Sizes z = sizes_of(s);
+    const Space w = space_of(s, z);
+    auto* ws = static_cast<char*>(workspace);
+    // Round-up reciprocal: exact while position x page_size < 2^shift.
+    int shift = 32;
+    while ((size_t{1} << (shift - 32)) < s.page_size) ++shift;
     PagedArgs a{static_cast<_Float16*>(o), static_cast<_Float16*>(k_pages),
                 static_cast<_Float16*>(v_pages), static_cast<const _Float16*>(q),
                 static_cast<const _Float16*>(k), static_cast<const _Float16*>(v),
                 static_cast<const int*>(offsets), static_cast<const int*>(cached),
                 static_cast<const int*>(table), int(s.tokens), int(s.sequences),
-                int(s.max_new < s.tokens ? s.max_new : s.tokens), int(s.heads), int(s.kv_heads),
-                int(s.q_stride), int(s.kv_stride), int(s.o_stride), int(s.pages),
-                int(s.page_size), int(s.max_pages), scale * kLog2e};
-    const dim3 grid(unsigned((size_t(a.max_new) * s.heads + 3) / 4), unsigned(s.sequences));
-    auto* const kernel = s.head_width == 64 ? paged_rows<64> : paged_rows<128>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, a);
+                int(std::min(s.max_new, s.tokens)), int(s.heads), int(s.kv_heads),
+                int(s.heads / s.kv_heads), int(s.q_stride), int(s.kv_stride), int(s.o_stride),
+                int(s.pages), int(s.page_size), int(s.max_pages),
+                (1ull << shift) / s.page_size + 1, shift, std::fabs(scale) * kLog2e, scale < 0.0f,
+                int(z.target), int(z.slots), reinterpret_cast<int2*>(ws),
+                reinterpret_cast<float2*>(ws + w.sums), reinterpret_cast<float*>(ws + w.parts)};
+    const dim3 grid(unsigned((z.blocks + z.target) * s.kv_heads));
+    const bool many = many_rows(s), wide = s.head_width == 128;
+    auto* const kernel = many ? (wide ? paged_many<128> : paged_many<64>)
+                              : (wide ? paged_few<128> : paged_few<64>);
+    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
+    auto* const join = wide ? paged_join<128> : paged_join<64>;
+    hipLaunchKernelGGL(join, dim3(unsigned((s.tokens * s.heads + 3) / 4)), dim3(kThreads), 0, stream,
+                       a, int(z.rows));
     return hipGetLastError();
 }
 

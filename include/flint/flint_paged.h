@@ -40,8 +40,8 @@ extern "C" {
 #endif
 
 typedef struct {
-    size_t tokens;      /* rows of q, k, v and o, up to 2^20 */
-    size_t sequences;   /* up to 65,535 */
+    size_t tokens;      /* rows of q, k, v and o, up to 2^20; tokens x heads up to 2^25 */
+    size_t sequences;   /* up to 65,535; sequences x kv_heads up to 2^22 */
     size_t max_new;     /* new tokens a sequence has at most */
     size_t heads;       /* of q and o, up to 1,024 */
     size_t kv_heads;    /* of k, v and the pages; divides heads */
