@@ -145,10 +145,19 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     return false;
 }
 
+// Where the rows of a tile's loads lie in the pages: lane u has load u's offset
+// (halves) and the bytes there that hold cached positions with a page. One
+// vector load of the table serves a whole tile, and runs a tile ahead of its
+// use (taken load by load, the table's latency bound the kernel).
+struct Where {
+    unsigned low, high, held;
+};
+
 // Reads the rows of K and V of one sequence and kv head, wherever they lie.
-template <int HD>
+template <int HD, int KEYS>
 struct Reader {
     using T = Tile<HD>;
+    static constexpr int kLoads = KEYS / T::kLoadRows;   // of a tile
     const PagedArgs& a;
     const int* table;
     int kv, cached, total;
@@ -162,40 +171,55 @@ struct Reader {
           v(args.v + size_t(it.seq.first) * args.kv_stride + size_t(head) * HD),
           row(lane_ / T::kChunks), lane(lane_) {}
 
-    static __device__ __forceinline__ void into(_Float16* lds, __amdgpu_buffer_rsrc_t rs,
-                                                unsigned at) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            rs, (__attribute__((address_space(3))) void*)(lds_half*)lds, 16, at, 0, 0, 0);
-    }
-
-    // Load u of a tile of K and of V, its rows the positions p0 on: one load
-    // each at least. Rows of no position, or of no page, are zeros. Whether the
-    // cached positions among them have a page.
-    __device__ __forceinline__ bool load(_Float16* kt, _Float16* vt, int p0, int u) const {
-        const int chunk = (lane % T::kChunks) ^ T::key(u * T::kLoadRows + row);
+    __device__ __forceinline__ Where find(int t) const {
+        const int p0 = t * KEYS + (lane % kLoads) * T::kLoadRows;
         const int column = column_of(a, p0);
         const int page = p0 < cached ? table[column] : -1;   // cached ends inside the table
         const bool ok = page >= 0 && page < a.pages;
-        const unsigned held = ok ? unsigned(min(cached - p0, T::kLoadRows)) * HD * 2 : 0u;
         const size_t from =
-            ((size_t(ok ? page : 0) * a.kv_heads + kv) * a.page_size + (p0 - column * a.page_size)) *
-            HD;
+            ok ? ((size_t(page) * a.kv_heads + kv) * a.page_size + (p0 - column * a.page_size)) * HD
+               : 0;
+        return {unsigned(from), unsigned(from >> 32),
+                ok ? unsigned(min(cached - p0, T::kLoadRows)) * HD * 2 : 0u};
+    }
+
+    // Bit u: load u's cached positions, if any, have a page.
+    __device__ __forceinline__ unsigned valid(const Where& w, int t) const {
+        const int p0 = t * KEYS + (lane % kLoads) * T::kLoadRows;
+        return unsigned(__ballot(lane < kLoads && (w.held != 0 || p0 >= cached)));
+    }
+
+    static __device__ __forceinline__ void into(_Float16* lds, const _Float16* from, unsigned bytes,
+                                                unsigned at) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            rsrc_of(from, bytes), (__attribute__((address_space(3))) void*)(lds_half*)lds, 16, at, 0,
+            0, 0);
+    }
+
+    // Load u of tile t of K and of V: one load each at least. Rows of no
+    // position, or of no page, are zeros.
+    __device__ __forceinline__ void load(_Float16* kt, _Float16* vt, const Where& w, int t,
+                                         int u) const {
+        const int p0 = t * KEYS + u * T::kLoadRows;
+        const int chunk = (lane % T::kChunks) ^ T::key(u * T::kLoadRows + row);
+        const size_t from = size_t(unsigned(__builtin_amdgcn_readlane(int(w.high), u))) << 32 |
+                            unsigned(__builtin_amdgcn_readlane(int(w.low), u));
+        const unsigned held = unsigned(__builtin_amdgcn_readlane(int(w.held), u));
         const unsigned at = unsigned(row * HD + chunk * 8) * 2;
         if (p0 + T::kLoadRows <= cached || p0 >= total) {
-            into(kt + u * 512, rsrc_of(a.k_pages + (ok ? from : 0), held), at);
-            into(vt + u * 512, rsrc_of(a.v_pages + (ok ? from : 0), held), at);
+            into(kt + u * 512, a.k_pages + from, held, at);
+            into(vt + u * 512, a.v_pages + from, held, at);
         } else if (p0 + row < cached) {
-            into(kt + u * 512, rsrc_of(a.k_pages + (ok ? from : 0), held), at);
-            into(vt + u * 512, rsrc_of(a.v_pages + (ok ? from : 0), held), at);
+            into(kt + u * 512, a.k_pages + from, held, at);
+            into(vt + u * 512, a.v_pages + from, held, at);
         } else {
             const int skip = max(p0 - cached, 0);   // new rows before this load's
             const int rows = min(total - cached - skip, T::kLoadRows);
             const unsigned bytes = unsigned((rows - 1) * a.kv_stride + HD) * 2;
             const unsigned here = unsigned((p0 + row - cached - skip) * a.kv_stride + chunk * 8) * 2;
-            into(kt + u * 512, rsrc_of(k + size_t(skip) * a.kv_stride, bytes), here);
-            into(vt + u * 512, rsrc_of(v + size_t(skip) * a.kv_stride, bytes), here);
+            into(kt + u * 512, k + size_t(skip) * a.kv_stride, bytes, here);
+            into(vt + u * 512, v + size_t(skip) * a.kv_stride, bytes, here);
         }
-        return ok || p0 >= cached;
     }
 };
 
@@ -340,28 +364,31 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
     Rows<HD, P::kKeys> w;
     w.load_q(a, it, head, first_row + fr, rows, h);
     const int last = it.seq.cached + (first_row + fr) / a.group;
-    const Reader<HD> reader(a, it, head, lane);
+    const Reader<HD, P::kKeys> reader(a, it, head, lane);
     int from, to;
     part_of(a, it, kFewRows, P::kKeys, &from, &to);
     _Float16* mine = lds + wave * 4 * kTile;
-    auto issue = [&](int t, int buf) __attribute__((always_inline)) {
+    auto issue = [&](const Where& at, int t, int buf) __attribute__((always_inline)) {
         _Float16* kt = mine + buf * 2 * kTile;
-        unsigned valid = 0;
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-            valid |= unsigned(reader.load(kt, kt + kTile, t * P::kKeys + u * Tile<HD>::kLoadRows, u))
-                     << u;
-        return valid;
+        for (int u = 0; u < 8; ++u) reader.load(kt, kt + kTile, at, t, u);
     };
     int t = from + wave;
-    unsigned valid = 0;
-    if (t < to) valid = issue(t, 0);
+    Where at = reader.find(t);
+    unsigned valid = reader.valid(at, t);
+    if (t < to) {
+        issue(at, t, 0);
+        at = reader.find(t + 4);
+    }
     for (int i = 0; t < to; ++i, t += 4) {
         unsigned next = 0;
         // The other buffer's reads ended with the last tile's products.
         asm volatile("" ::: "memory");
         if (t + 4 < to) {
-            next = issue(t + 4, (i + 1) & 1);
+            next = reader.valid(at, t + 4);
+            const Where ahead = reader.find(t + 8);
+            issue(at, t + 4, (i + 1) & 1);
+            at = ahead;
             wait_vmcnt<16>();   // the newer tile's 8 loads of K and 8 of V, at least
         } else {
             wait_vmcnt<0>();
@@ -427,7 +454,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
     constexpr int kTile = Tile<HD>::kHalves;
     constexpr int kEach = Tile<HD>::kLoads / 4;   // loads of a wave, of K and of V
     __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
-    __shared__ int paged[2][16];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, h = lane >> 5;
@@ -441,26 +467,30 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
     w.load_q(a, it, head, first_row + fr, rows, h);
     const int last = it.seq.cached + (first_row + fr) / a.group;
     const int wave_last = it.seq.cached + (min(first_row + 32, rows) - 1) / a.group;
-    const Reader<HD> reader(a, it, head, lane);
+    const Reader<HD, P::kKeys> reader(a, it, head, lane);
     int from, to;
     part_of(a, it, kManyRows, P::kKeys, &from, &to);
-    auto issue = [&](int t) __attribute__((always_inline)) {
+    auto issue = [&](const Where& at, int t) __attribute__((always_inline)) {
         _Float16* kt = lds + (t & 1) * 2 * kTile;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int u = wave + 4 * i;
-            const bool ok = reader.load(kt, kt + kTile, t * P::kKeys + u * Tile<HD>::kLoadRows, u);
-            if (lane == 0) paged[t & 1][u] = ok;
-        }
+        for (int i = 0; i < kEach; ++i) reader.load(kt, kt + kTile, at, t, wave + 4 * i);
     };
-    if (from < to) issue(from);
+    Where at = reader.find(from);
+    unsigned next = reader.valid(at, from);
+    if (from < to) {
+        issue(at, from);
+        at = reader.find(from + 1);
+    }
     for (int t = from; t < to; ++t) {
+        const unsigned valid = next;
         wait_vmcnt<0>();
         block_sync();
-        if (t + 1 < to) issue(t + 1);
+        if (t + 1 < to) {
+            next = reader.valid(at, t + 1);
+            issue(at, t + 1);
+            at = reader.find(t + 2);
+        }
         if (first_row >= rows || t * P::kKeys > wave_last) continue;   // no row here, or none sees it
-        const unsigned valid =
-            unsigned(__ballot(lane < Tile<HD>::kLoads && paged[t & 1][lane & 15] != 0));
         const _Float16* kt = lds + (t & 1) * 2 * kTile;
         w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
     }
