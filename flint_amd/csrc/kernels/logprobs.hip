@@ -20,76 +20,272 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.69314718055994531f;
+// Chunks (of 8 columns) and words that may hold an alternative, as LDS keeps
+// them. Rows with more (many equal logits) find the exact border first.
+constexpr int kChunkList = 512, kWordList = 512;
 
-// The order of the alternatives as distinct whole numbers: the FP16 value's
-// place among all values (-0 with +0, NaN above +inf), then the lower column.
-__device__ __forceinline__ unsigned rank_key(_Float16 v, int column) {
+// The place of an FP16 value among all values: -0 with +0, NaN above +inf.
+__device__ __forceinline__ unsigned order_of(_Float16 v) {
     unsigned x = __builtin_bit_cast(unsigned short, v);
     if ((x & 0x7fff) == 0) x = 0;
-    x = (x & 0x7fff) > 0x7c00 ? 0xffffu : (x & 0x8000) ? 0xffffu - x : x | 0x8000u;
-    return x << 16 | (0xffffu - unsigned(column));
+    return (x & 0x7fff) > 0x7c00 ? 0xffffu : (x & 0x8000) ? 0xffffu - x : x | 0x8000u;
+}
+__device__ __forceinline__ float value_of(unsigned order) {
+    if (order == 0xffffu) return __builtin_nanf("");
+    const unsigned short x = (unsigned short)(order & 0x8000u ? order ^ 0x8000u : 0xffffu - order);
+    return float(__builtin_bit_cast(_Float16, x));
 }
 
-template <class T, class Op>
-__device__ T block_reduce(T v, T* shared, Op op) {
-    for (int d = 32; d > 0; d /= 2) v = op(v, __shfl_xor(v, d));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
-    __syncthreads();
-    v = shared[0];
-    for (int w = 1; w < kThreads / 64; ++w) v = op(v, shared[w]);
-    return v;
+__device__ __forceinline__ _Float16 max_of(const h8& v) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const h4 a = __builtin_elementwise_maximum(__builtin_shufflevector(v, v, 0, 1, 2, 3),
+                                               __builtin_shufflevector(v, v, 4, 5, 6, 7));
+    const h2 b = __builtin_elementwise_maximum(__builtin_shufflevector(a, a, 0, 1),
+                                               __builtin_shufflevector(a, a, 2, 3));
+    return __builtin_elementwise_maximum(b[0], b[1]);
 }
 
-// One workgroup a row: the maximum, the sums, then the alternatives one by one,
-// each the largest key below the last one's.
-__global__ void __launch_bounds__(kThreads)
+// An empty asm on a chunk: what one pass formed from it is formed again in the
+// next rather than kept (8 registers or more a chunk, which cost the rows in
+// flight).
+__device__ __forceinline__ void keep_packed(h8& v) { asm volatile("" : "+v"(v)); }
+
+// One workgroup of THREADS a row, which it reads once into registers (thread t
+// holds the 16-byte chunks t, t + THREADS, ...: at most CPT). Reading bounds it:
+// 7 VALU slots a word against 2 bytes.
+//
+// Alternatives: the row falls into 64 groups of threads. The top-th largest of
+// the groups' maxima is a border that at least `top` words reach, and few more
+// do (about top (1 + top / 128) of words in no order); the chunks holding them
+// go to a list in LDS, from there the words, and a word's place in the answer
+// is the number of listed words before it. The groups' maxima are a step of the
+// row's maximum anyway.
+template <int THREADS, int CPT>
+__global__ void __launch_bounds__(THREADS)
 logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
                  float* __restrict__ stats, int* __restrict__ top_ids,
-                 float* __restrict__ top_logprobs, const _Float16* __restrict__ logits,
-                 const uint16_t* __restrict__ targets, float scale, int vocab, int cols, int top) {
-    __shared__ float red[kThreads / 64];
-    __shared__ unsigned red_key[kThreads / 64];
+                 float* __restrict__ top_logprobs, const h8* __restrict__ logits,
+                 const uint16_t* __restrict__ targets, float scale, int vocab, int chunks, int top) {
+    constexpr int kWaves = THREADS / 64;
+    __shared__ unsigned group_max[64];
+    __shared__ __attribute__((aligned(16))) h8 list[kChunkList];
+    __shared__ int list_chunk[kChunkList];
+    __shared__ unsigned words[kWordList];
+    __shared__ int counts[2];
+    __shared__ float red[3][kWaves];
+    __shared__ int red_count[kWaves];
     const size_t row = blockIdx.x;
-    const _Float16* l = logits + row * cols;
-    const int tid = threadIdx.x;
-    float mx = -INFINITY;
-    for (int j = tid; j < vocab; j += kThreads) mx = __builtin_elementwise_maximum(mx, float(l[j]));
-    mx = block_reduce(mx, red, [](float a, float b) { return __builtin_elementwise_maximum(a, b); });
-    float rest = 0.0f, largest = 0.0f, weighted = 0.0f;   // the terms below 1, how many are 1
-    for (int j = tid; j < vocab; j += kThreads) {
-        const float gap = float(l[j]) - mx, g = scale * gap;
-        const float e = __builtin_amdgcn_exp2f(g * kLog2e);
-        if (gap == 0.0f) largest += 1.0f;
-        else rest += e;
-        weighted += e * fmaxf(g, -3e38f);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const h8* lr = logits + row * chunks;
+    const int held = (vocab + 7) >> 3, last = held - 1, last_count = vocab - last * 8;
+    const _Float16 lowest = -__builtin_huge_valf16();
+    const int target = targets[row];
+    float at_target = 0.0f;
+    if (tid == 0 && target < vocab) at_target = float(reinterpret_cast<const _Float16*>(lr)[target]);
+
+    h8 raw[CPT];
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+        const int c = tid + i * THREADS;
+        raw[i] = c < held ? load_stream(lr + c) : h8(lowest);
     }
-    auto add = [](float a, float b) { return a + b; };
-    rest = block_reduce(rest, red, add);
-    largest = block_reduce(largest, red, add);
-    weighted = block_reduce(weighted, red, add);
-    const float sum = largest + rest, log_sum = log1pf(largest - 1.0f + rest);
+    if (last_count < 8 && last >= tid && (last - tid) % THREADS == 0) {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i)
+            if (i == (last - tid) / THREADS) {
+#pragma unroll
+                for (int j = 1; j < 8; ++j)
+                    if (j >= last_count) raw[i][j] = lowest;
+            }
+    }
+    if (tid < 2) counts[tid] = 0;
+
+    // The groups' maxima, the row's, and the border.
+    h8 m8 = raw[0];
+#pragma unroll
+    for (int i = 1; i < CPT; ++i) m8 = __builtin_elementwise_maximum(m8, raw[i]);
+    const unsigned own = order_of(max_of(m8));
+    unsigned group = own;
+    if constexpr (THREADS == 256) {   // groups of 4 lanes
+        group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0xB1, 0xF, 0xF, false)));
+        group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x4E, 0xF, 0xF, false)));
+        if ((lane & 3) == 0) group_max[16 * wave + (lane >> 2)] = group;
+        __syncthreads();
+        group = group_max[lane];
+    } else {
+        __syncthreads();
+    }
+    unsigned border = 0;
+    const int wanted = max(top, 1);
+#pragma unroll
+    for (int bit = 15; bit >= 0; --bit) {
+        const unsigned higher = border | 1u << bit;
+        if (__popcll(__ballot(group >= higher)) >= wanted) border = higher;
+    }
+    unsigned top_order = group;
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) top_order = max(top_order, unsigned(__shfl_xor(int(top_order), d)));
+    const float mx = value_of(top_order);
+
+    unsigned limit = 0xffffu;   // the last column that an equal to the border may have
+    if (top > 0) {
+        auto collect = [&]() {
+#pragma unroll
+            for (int i = 0; i < CPT; ++i) {
+                keep_packed(raw[i]);
+                if (own >= border && order_of(max_of(raw[i])) >= border) {
+                    const int at = atomicAdd(&counts[0], 1);
+                    if (at < kChunkList) {
+                        list[at] = raw[i];
+                        list_chunk[at] = tid + i * THREADS;
+                    }
+                }
+            }
+            __syncthreads();
+            const int n = min(counts[0], kChunkList);
+            for (int e = tid; e < 8 * n; e += THREADS) {
+                const unsigned order = order_of(list[e >> 3][e & 7]);
+                const int column = list_chunk[e >> 3] * 8 + (e & 7);
+                if (column < vocab && (order > border || (order == border && unsigned(column) <= limit))) {
+                    const int at = atomicAdd(&counts[1], 1);
+                    if (at < kWordList) words[at] = order << 16 | (0xffffu - unsigned(column));
+                }
+            }
+            __syncthreads();
+        };
+        collect();
+        if (counts[0] > kChunkList || counts[1] > kWordList) {
+            // The exact border by halving: the value, then among the words of
+            // that value the column, counting over the whole row each time. (What
+            // pads the row is -inf behind its last column: after every word.)
+            auto count = [&](auto in) {
+                int n = 0;
+#pragma unroll
+                for (int i = 0; i < CPT; ++i) {
+                    keep_packed(raw[i]);
+                    unsigned first = unsigned(tid + i * THREADS) * 8;
+                    asm volatile("" : "+v"(first));
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) n += in(order_of(raw[i][j]), first + j);
+                }
+#pragma unroll
+                for (int d = 32; d > 0; d /= 2) n += __shfl_xor(n, d);
+                __syncthreads();
+                if (lane == 0) red_count[wave] = n;
+                __syncthreads();
+                n = 0;
+                for (int w = 0; w < kWaves; ++w) n += red_count[w];
+                return n;
+            };
+            border = 0;
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned higher = border | 1u << bit;
+                if (count([&](unsigned o, unsigned) { return o >= higher; }) >= top) border = higher;
+            }
+            const int more = top - count([&](unsigned o, unsigned) { return o > border; });
+            unsigned below = 0;   // fewer than `more` of them lie before this column
+            for (int bit = 15; bit >= 0; --bit) {
+                const unsigned higher = below | 1u << bit;
+                if (count([&](unsigned o, unsigned c) { return o == border && c < higher; }) < more)
+                    below = higher;
+            }
+            limit = below;
+            // Words now, without the chunks: exactly `top`.
+            if (tid < 2) counts[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < CPT; ++i) {
+                keep_packed(raw[i]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const unsigned order = order_of(raw[i][j]);
+                    const unsigned column = unsigned(tid + i * THREADS) * 8 + j;
+                    if (order > border || (order == border && column <= limit))
+                        words[atomicAdd(&counts[1], 1)] = order << 16 | (0xffffu - column);
+                }
+            }
+            __syncthreads();
+        }
+    }
+
+    // The largest words leave the sum (each is 1) and are counted.
+    float largest = 0.0f;
+    if (__any(own == top_order)) {
+#pragma unroll
+        for (int i = 0; i < CPT; ++i) {
+            keep_packed(raw[i]);
+            if (order_of(max_of(raw[i])) != top_order) continue;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (float(raw[i][j]) == mx) {
+                    raw[i][j] = lowest;
+                    largest += 1.0f;
+                }
+        }
+    }
+    // e = 2^(x - mx c), c = scale log2 e: one fma of the exact product, and the
+    // rounding of mx c (common to every word) put right in the sums below.
+    // -1e4 keeps words of probability 0 out of 0 x inf.
+    const float c = scale * kLog2e, shift = mx * c;
+    const float off = __builtin_fmaf(mx, c, -shift);
+    float rest = 0.0f, weighted = 0.0f;
+#pragma unroll
+    for (int i = 0; i < CPT; ++i) {
+        keep_packed(raw[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float g = fmaxf(__builtin_fmaf(float(raw[i][j]), c, -shift), -1e4f);
+            const float e = __builtin_amdgcn_exp2f(g);
+            rest += e;
+            weighted = __builtin_fmaf(e, g, weighted);
+        }
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) {
+        rest += __shfl_xor(rest, d);
+        weighted += __shfl_xor(weighted, d);
+        largest += __shfl_xor(largest, d);
+    }
+    if constexpr (kWaves > 1) {
+        if (lane == 0) {
+            red[0][wave] = rest;
+            red[1][wave] = weighted;
+            red[2][wave] = largest;
+        }
+        __syncthreads();
+        rest = weighted = largest = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) {
+            rest += red[0][w];
+            weighted += red[1][w];
+            largest += red[2][w];
+        }
+    }
+    // Every g is off by `off`: weighted is the sum of e (g - off), in units of 1.
+    const float unit = __builtin_amdgcn_exp2f(-off);
+    weighted = __builtin_fmaf(-off, rest, weighted) * unit;
+    rest *= unit;
+    // (A row without a finite largest logit has no distribution.)
+    float log_sum = log1pf(largest - 1.0f + rest);
+    if (!(fabsf(mx) < __builtin_huge_valf())) log_sum = __builtin_nanf("");
     if (tid == 0) {
-        const int t = targets[row];
-        logprob[row] = t < vocab ? scale * (float(l[t]) - mx) - log_sum : 0.0f;
-        entropy[row] = log_sum - weighted / sum;
+        logprob[row] = target < vocab ? scale * (at_target - mx) - log_sum : 0.0f;
+        entropy[row] = log_sum - kLn2 * (weighted / (largest + rest));
         stats[2 * row] = mx;
         stats[2 * row + 1] = log_sum;
     }
-    unsigned last = 0xffffffffu;
-    for (int i = 0; i < top; ++i) {
-        unsigned best = 0;
-        for (int j = tid; j < vocab; j += kThreads) {
-            const unsigned key = rank_key(l[j], j);
-            // The first pass takes every key (a NaN in column 0 has the largest).
-            if ((i == 0 || key < last) && key > best) best = key;
-        }
-        best = block_reduce(best, red_key, [](unsigned a, unsigned b) { return max(a, b); });
-        last = best;
-        if (tid == 0) {
-            const int j = int(0xffffu - (best & 0xffffu));
-            top_ids[row * top + i] = j;
-            top_logprobs[row * top + i] = scale * (float(l[j]) - mx) - log_sum;
+    if (top > 0) {
+        const int n = counts[1];
+        for (int i = tid; i < n; i += THREADS) {
+            const unsigned word = words[i];
+            int place = 0;
+            for (int k = 0; k < n; ++k) place += words[k] > word;
+            if (place < top) {
+                top_ids[row * top + place] = int(0xffffu - (word & 0xffffu));
+                top_logprobs[row * top + place] = scale * (value_of(word >> 16) - mx) - log_sum;
+            }
         }
     }
 }
@@ -127,16 +323,31 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
                                    void* top_logprobs, const void* logits, const void* targets,
                                    float scale, size_t rows, size_t vocab, size_t cols, size_t top,
                                    hipStream_t stream) {
+    // A wave a row while it holds at most 4 chunks a lane, else 256 threads.
+    const size_t held = (vocab + 7) / 8;
     for (size_t done = 0; done < rows;) {
         const size_t n = std::min<size_t>(rows - done, size_t{1} << 22);
-        hipLaunchKernelGGL(logprobs_forward, dim3(unsigned(n)), dim3(kThreads), 0, stream,
-                           static_cast<float*>(logprob) + done, static_cast<float*>(entropy) + done,
-                           static_cast<float*>(stats) + 2 * done,
-                           static_cast<int*>(top_ids) + done * top,
-                           static_cast<float*>(top_logprobs) + done * top,
-                           static_cast<const _Float16*>(logits) + done * cols,
-                           static_cast<const uint16_t*>(targets) + done, scale, int(vocab),
-                           int(cols), int(top));
+#define FLINT_LP(THREADS, CPT)                                                                  \
+    if (held <= size_t{THREADS} * CPT)                                                          \
+        hipLaunchKernelGGL((logprobs_forward<THREADS, CPT>), dim3(unsigned(n)), dim3(THREADS),  \
+                           0, stream, static_cast<float*>(logprob) + done,                      \
+                           static_cast<float*>(entropy) + done,                                 \
+                           static_cast<float*>(stats) + 2 * done,                               \
+                           static_cast<int*>(top_ids) + done * top,                             \
+                           static_cast<float*>(top_logprobs) + done * top,                      \
+                           static_cast<const h8*>(logits) + done * (cols / 8),                  \
+                           static_cast<const uint16_t*>(targets) + done, scale, int(vocab),     \
+                           int(cols / 8), int(top))
+        FLINT_LP(64, 1);
+        else FLINT_LP(64, 2);
+        else FLINT_LP(64, 4);
+        else FLINT_LP(256, 2);
+        else FLINT_LP(256, 4);
+        else FLINT_LP(256, 8);
+        else FLINT_LP(256, 16);
+        else FLINT_LP(256, 25);
+        else FLINT_LP(256, 32);
+#undef FLINT_LP
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         done += n;
     }
