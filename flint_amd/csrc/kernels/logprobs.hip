@@ -108,10 +108,15 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
     for (int i = 1; i < CPT; ++i) m8 = __builtin_elementwise_maximum(m8, raw[i]);
     const unsigned own = order_of(max_of(m8));
     unsigned group = own;
-    if constexpr (THREADS == 256) {   // groups of 4 lanes
+    if constexpr (THREADS > 64) {   // groups of THREADS / 64 neighbouring lanes
+        constexpr int kGroup = THREADS / 64;
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0xB1, 0xF, 0xF, false)));
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x4E, 0xF, 0xF, false)));
-        if ((lane & 3) == 0) group_max[16 * wave + (lane >> 2)] = group;
+        if constexpr (kGroup == 16) {
+            group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x141, 0xF, 0xF, false)));
+            group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x140, 0xF, 0xF, false)));
+        }
+        if (lane % kGroup == 0) group_max[tid / kGroup] = group;
         __syncthreads();
         group = group_max[lane];
     } else {
@@ -323,12 +328,14 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
                                    void* top_logprobs, const void* logits, const void* targets,
                                    float scale, size_t rows, size_t vocab, size_t cols, size_t top,
                                    hipStream_t stream) {
-    // A wave a row while it holds at most 4 chunks a lane, else 256 threads.
+    // A wave a row while it holds at most 4 chunks a lane, else 256 threads, or
+    // 1,024 where the rows leave CUs idle and a row is long enough.
     const size_t held = (vocab + 7) / 8;
+    const bool few = rows <= 256 && held > 1024;
     for (size_t done = 0; done < rows;) {
         const size_t n = std::min<size_t>(rows - done, size_t{1} << 22);
-#define FLINT_LP(THREADS, CPT)                                                                  \
-    if (held <= size_t{THREADS} * CPT)                                                          \
+#define FLINT_LP(TAKE, THREADS, CPT)                                                            \
+    if (TAKE && held <= size_t{THREADS} * CPT)                                                  \
         hipLaunchKernelGGL((logprobs_forward<THREADS, CPT>), dim3(unsigned(n)), dim3(THREADS),  \
                            0, stream, static_cast<float*>(logprob) + done,                      \
                            static_cast<float*>(entropy) + done,                                 \
@@ -338,15 +345,19 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
                            static_cast<const h8*>(logits) + done * (cols / 8),                  \
                            static_cast<const uint16_t*>(targets) + done, scale, int(vocab),     \
                            int(cols / 8), int(top))
-        FLINT_LP(64, 1);
-        else FLINT_LP(64, 2);
-        else FLINT_LP(64, 4);
-        else FLINT_LP(256, 2);
-        else FLINT_LP(256, 4);
-        else FLINT_LP(256, 8);
-        else FLINT_LP(256, 16);
-        else FLINT_LP(256, 25);
-        else FLINT_LP(256, 32);
+        FLINT_LP(true, 64, 1);
+        else FLINT_LP(true, 64, 2);
+        else FLINT_LP(true, 64, 4);
+        else FLINT_LP(few, 1024, 2);
+        else FLINT_LP(few, 1024, 4);
+        else FLINT_LP(few, 1024, 7);
+        else FLINT_LP(few, 1024, 8);
+        else FLINT_LP(true, 256, 2);
+        else FLINT_LP(true, 256, 4);
+        else FLINT_LP(true, 256, 8);
+        else FLINT_LP(true, 256, 16);
+        else FLINT_LP(true, 256, 25);
+        else FLINT_LP(true, 256, 32);
 #undef FLINT_LP
         if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
         done += n;

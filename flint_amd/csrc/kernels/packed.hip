@@ -356,21 +356,28 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
 // ---------------------------------------------------------------- backward: dK, dV
 
 // 128 keys (32 a wave) of one head of k and v; walks the 64-query tiles at or
-// after its first key, of each query head of the group in turn. A lane holds
-// one key and 16 queries per 32-query half, whose lse and D come from LDS.
+// after its first key, of the group's query heads in turn. A lane holds one key
+// and 16 queries per 32-query half, whose lse and D come from LDS.
+//
+// With parts > 1 a workgroup takes `share` of the group's heads and leaves FP32
+// sums ([part][token][kv head][HD], dK then dV) for packed_backward_join: heads
+// of k and v are few where groups are large, and so are workgroups then.
 template <int HD>
 __global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1)
 packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                      const _Float16* __restrict__ v, const _Float16* __restrict__ dout,
                      const float* __restrict__ lse, const float* __restrict__ dsum,
-                     const int4* __restrict__ plan, int tokens, int kv_heads, int group, Strides st,
-                     float c, float scale) {
+                     const int4* __restrict__ plan, float* __restrict__ sums, int tokens,
+                     int kv_heads, int group, int share, Strides st, float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
     __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][Q, dO]
     __shared__ __attribute__((aligned(16))) float rowstat[2][2][64];       // [buf][lse, D]
     Work w;
-    if (!work_of(plan, int(blockIdx.x), kv_heads, tokens, &w)) return;
+    const int parts = group / share;
+    if (!work_of(plan, int(blockIdx.x), kv_heads * parts, tokens, &w)) return;
+    const int part = w.head % parts;
+    w.head /= parts;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, h = lane >> 5;
@@ -389,10 +396,10 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
     f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
     const int first = block * kPackedBlock / 64;
     const int per_head = (length + 63) / 64 - first;
-    const int steps = per_head * group;
+    const int steps = per_head * share;
     auto stage = [&](int i) {
         const int buf = i & 1, g = i / per_head, tile = first + i - g * per_head;
-        const int head = w.head * group + g;
+        const int head = w.head * group + part * share + g;
         _Float16* t = lds + buf * 2 * kTile;
         const int qq = 64 * tile + lane;
         float lv = 0.0f, dv0 = 0.0f;
@@ -472,12 +479,74 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             }
         }
     }
-    if (ki < length) {
+    if (ki >= length) return;
+    if (parts == 1) {
         const size_t at = kv_at + size_t(ki) * st.kv;
         store_row<HD>(dk + at, dka, scale, h);
         store_row<HD>(dv + at, dva, 1.0f, h);
+        return;
+    }
+    float* to = sums + ((size_t(part) * tokens + w.begin + ki) * kv_heads + w.head) * HD;
+    const size_t dv_at = size_t(parts) * tokens * kv_heads * HD;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int a = 0; a < 4; ++a) {
+            const int d = 32 * db + 8 * a + 4 * h;
+            *reinterpret_cast<f32x4*>(to + d) = f32x4{dka[db][4 * a], dka[db][4 * a + 1],
+                                                      dka[db][4 * a + 2], dka[db][4 * a + 3]};
+            *reinterpret_cast<f32x4*>(to + dv_at + d) =
+                f32x4{dva[db][4 * a], dva[db][4 * a + 1], dva[db][4 * a + 2], dva[db][4 * a + 3]};
+        }
+}
+
+// The parts' sums in order, of a block's 128 rows and one head: 8 values a
+// thread and step.
+template <int HD>
+__global__ void __launch_bounds__(kThreads)
+packed_backward_join(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
+                     const float* __restrict__ sums, const int4* __restrict__ plan, int tokens,
+                     int kv_heads, int parts, int stride, float scale) {
+    Work w;
+    if (!work_of(plan, int(blockIdx.x), kv_heads, tokens, &w)) return;
+    const int row0 = w.block * kPackedBlock, rows = min(w.length - row0, kPackedBlock);
+    const size_t step = size_t(tokens) * kv_heads * HD, dv_at = step * parts;
+    for (int i = threadIdx.x; i < rows * (HD / 8); i += kThreads) {
+        const size_t token = size_t(w.begin) + row0 + i / (HD / 8);
+        const int d = i % (HD / 8) * 8;
+        const float* from = sums + (token * kv_heads + w.head) * HD + d;
+        const size_t to = token * stride + size_t(w.head) * HD + d;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            f32x4 low = {}, high = {};
+            for (int p = 0; p < parts; ++p) {
+                const float* at = from + which * dv_at + p * step;
+                low += *reinterpret_cast<const f32x4*>(at);
+                high += *reinterpret_cast<const f32x4*>(at + 4);
+            }
+            const float by = which == 0 ? scale : 1.0f;
+            f16x8 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                v[e] = _Float16(low[e] * by);
+                v[4 + e] = _Float16(high[e] * by);
+            }
+            *reinterpret_cast<f16x8*>((which == 0 ? dk : dv) + to) = v;
+        }
     }
 }
+
+// How many parts the heads of a group go into for dK and dV: the fewest equal
+// ones that give the GPU two workgroups a CU (256 CUs).
+size_t group_parts(const flint_packed_shape& s) {
+    const size_t group = s.heads / s.kv_heads, blocks = packed_items(s) * s.kv_heads;
+    size_t parts = 1;
+    while (parts < group && (blocks * parts < 512 || group % parts != 0)) ++parts;
+    return parts;
+}
+
+// D, one FP32 value a query and head (padded to 16 bytes).
+size_t dsum_values(const flint_packed_shape& s) { return (s.heads * s.tokens + 3) / 4 * 4; }
 
 template <int HD>
 hipError_t forward(void* o, void* lse, const void* q, const void* k, const void* v,
@@ -509,20 +578,30 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
                        static_cast<const int4*>(plan), int(s.tokens), int(s.heads), group, st,
                        scale * kLog2e, scale);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(packed_items(s) * s.kv_heads)),
-                       dim3(kThreads), 0, stream, static_cast<_Float16*>(dk),
-                       static_cast<_Float16*>(dv), static_cast<const _Float16*>(q),
-                       static_cast<const _Float16*>(k), static_cast<const _Float16*>(v),
-                       static_cast<const _Float16*>(dout), static_cast<const float*>(lse),
-                       static_cast<const float*>(dsum), static_cast<const int4*>(plan),
-                       int(s.tokens), int(s.kv_heads), group, st, scale * kLog2e, scale);
+    const size_t parts = group_parts(s), blocks = packed_items(s) * s.kv_heads;
+    float* sums = dsum + dsum_values(s);
+    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(blocks * parts)), dim3(kThreads), 0,
+                       stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
+                       static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
+                       static_cast<const _Float16*>(v), static_cast<const _Float16*>(dout),
+                       static_cast<const float*>(lse), static_cast<const float*>(dsum),
+                       static_cast<const int4*>(plan), sums, int(s.tokens), int(s.kv_heads), group,
+                       group / int(parts), st, scale * kLog2e, scale);
+    if (hipError_t e = hipGetLastError(); e != hipSuccess || parts == 1) return e;
+    hipLaunchKernelGGL(packed_backward_join<HD>, dim3(unsigned(blocks)), dim3(kThreads), 0, stream,
+                       static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
+                       static_cast<const float*>(sums), static_cast<const int4*>(plan),
+                       int(s.tokens), int(s.kv_heads), int(parts), int(s.kv_stride), scale);
     return hipGetLastError();
 }
 
 }  // namespace
 
-// D, one FP32 value a query and head.
-size_t packed_backward_workspace(const flint_packed_shape& s) { return s.heads * s.tokens * 4; }
+size_t packed_backward_workspace(const flint_packed_shape& s) {
+    const size_t parts = group_parts(s);
+    const size_t sums = parts == 1 ? 0 : 2 * parts * s.tokens * s.kv_heads * s.head_width;
+    return (dsum_values(s) + sums) * 4;
+}
 
 hipError_t launch_packed_plan(void* plan, const void* offsets, const flint_packed_shape& s,
                               hipStream_t stream) {

@@ -148,6 +148,18 @@ def test_many_rows(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,top", [(3000, 64), (9000, 5), (30000, 33), (50257, 64), (65536, 1)])
+def test_many_rows_of_long_ones(flint, cuda, vocab, top):
+    """More rows than the GPU has compute units: other workgroup sizes."""
+    r = Rows(cuda, 300, vocab, (vocab + 7) // 8 * 8, top, seed=vocab)
+    r.logits[7] = 0.25          # equal logits: the lowest columns
+    r.logits[8, 40:] = float("-inf")
+    r.logits[9] = (r.logits[9] * 0.3).round()
+    r.targets[8] = 39
+    check(r.run(flint), r.reference())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vocab", [900, 20000])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "lowest", "masked", "ramp", "ends"])
 def test_ties_and_masks(flint, cuda, kind, vocab):

@@ -323,7 +323,10 @@ def test_buffers_refused(flint):
     fails(flint, "flint_attention_packed_plan", A, A, s, None, message="plan and offsets overlap")
     fn = "flint_attention_packed_backward"
     good = [(i + 1) * A for i in range(10)]
-    fails(flint, fn, *good, s, f, 11 * A, 100, None, message="needs 1024 bytes of workspace, given 100")
+    need = ctypes.c_size_t(0)
+    assert flint.lib.flint_attention_packed_backward_workspace(s, need) == 0 and need.value >= 1024
+    fails(flint, fn, *good, s, f, 11 * A, 100, None,
+          message=f"needs {need.value} bytes of workspace, given 100")
     fails(flint, fn, A, A + 64, *good[2:], s, f, 11 * A, 1 << 20, None, message="dq and dk overlap")
 
 
