@@ -149,6 +149,66 @@ __device__ __forceinline__ constexpr int result_row(int r, int h) {
     return 8 * (r >> 2) + 4 * h + (r & 3);
 }
 
+// A running maximum below every score: exp2(-inf - kFloor) is 0, and the first
+// key that a query sees moves it.
+constexpr float kFloor = -3e38f;
+// What a lane's probabilities of a tile may add up to before the running
+// maximum is moved: none of them is above it then, and FP16 holds 2^16.
+constexpr float kSumLimit = 32768.0f;
+
+// P = 2^(ce s - m) as FP16, and the FP32 sum of this lane's (its half of the
+// keys).
+template <int HB>
+__device__ __forceinline__ float exponentials(f16x8 (&p)[2 * HB], const f32x16 (&s)[HB], float ce,
+                                              float m) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hb][r], ce, -m));
+            p[2 * hb + (r >> 3)][r & 7] = _Float16(e);
+            sum += e;
+        }
+    return sum;
+}
+
+// A tile's probabilities and their sum. m, a query's reference in log2 units,
+// need not be its maximum: O and l share it, and it only has to keep P inside
+// FP16. So past the wave's first tile (started) the tile's maximum is not taken
+// unless the sum passes kSumLimit, or overflows, for some query; then m moves
+// to the maximum, rescale(2^(m_old - m_new)) is called and the tile is taken
+// again (scores() gives s and ce once more, so that no register holds s
+// meanwhile).
+// (scores uses an offset of 0 that the compiler cannot see through: otherwise it
+// moves the products and the masks out of the loop and keeps them after all.)
+template <int HB, class Scores, class Rescale>
+__device__ __forceinline__ float probabilities(f16x8 (&p)[2 * HB], const Scores& scores, float* m,
+                                               bool* started, const Rescale& rescale) {
+    for (;;) {
+        f32x16 s[HB];
+        unsigned zero = 0;
+        asm volatile("" : "+s"(zero));
+        const float ce = scores(s, zero);
+        const bool move = !*started;
+        if (move) {
+            *started = true;
+            float mx = s[0][0];
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[hb][r]);
+            mx *= ce;
+            const float m_new = fmaxf(*m, fmaxf(mx, xor32(mx)));
+            rescale(__builtin_amdgcn_exp2f(*m - m_new));
+            *m = m_new;
+        }
+        const float sum = exponentials<HB>(p, s, ce, *m);
+        if (move || !__any(sum > kSumLimit)) return sum;
+        *started = false;
+    }
+}
+
 // A lane's part of a result transposed to rows (one query or key of the lane,
 // HD values scaled by `by`) written to `row` as FP16.
 template <int HD>

@@ -26,9 +26,7 @@ namespace flint {
 namespace {
 
 constexpr int kThreads = 256;   // 4 waves of 32 queries (keys)
-// How far (log2 units) a query's scores may rise above the running maximum
-// before O and l are rescaled: P <= 2^8 until then, far inside FP16.
-constexpr float kRescale = 8.0f;
+constexpr int kGroups = 2;      // of 4 waves, which take the tiles in turn
 
 // ---------------------------------------------------------------- plan
 
@@ -138,20 +136,45 @@ struct Strides {
     int q, kv, o;
 };
 
+// The groups' sums of one result added in LDS (4 waves' [HD][32] floats), into
+// the first group's; false in the others.
+template <int HD>
+__device__ __forceinline__ bool join_groups(float* lds, f32x16* acc, int wave, int part, int lane) {
+    if constexpr (kGroups == 1) return true;
+    const int fr = lane & 31, h = lane >> 5;
+    float* theirs = lds + wave * HD * 32;
+    __syncthreads();
+    if (part != 0) {
+#pragma unroll
+        for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) theirs[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
+    }
+    __syncthreads();
+    if (part != 0) return false;
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[db][r] += theirs[(32 * db + result_row(r, h)) * 32 + fr];
+    return true;
+}
+
 // ---------------------------------------------------------------- forward
 
-template <int HD, bool NEG>
-__global__ void __launch_bounds__(kThreads, HD == 64 ? 3 : 2)
+template <int HD>
+__global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2)
 packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float16* __restrict__ q,
                const _Float16* __restrict__ k, const _Float16* __restrict__ v,
                const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
-               float c) {
+               float c, bool negative) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kGroups * 2 * kTile];   // [buf][group][K, V]
+    __shared__ float2 sums[4][32];
     Work w;
     if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
@@ -163,73 +186,55 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
 
     f16x8 qf[KK];
     load_frags<HD>(qf, qb, qi, length, st.q, h);
-    float m = -INFINITY, l = 0.0f;
+    if (negative)   // c is positive: the scale's sign goes into q
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = -qf[kk];
+    float m = kFloor, l = 0.0f;
+    bool started = false;
     f32x16 acc[DB] = {};
     const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
-    const int tiles = q_last / 64 + 1;
-    auto load = [&](int j) {
-        _Float16* t = lds + (j & 1) * 2 * kTile;
+    const int tiles = q_last / 64 + 1, steps = (tiles + kGroups - 1) / kGroups;
+    auto load = [&](int i) {
+        const int j = kGroups * i + part;
+        if (j >= tiles) return;
+        _Float16* t = lds + ((i & 1) * kGroups + part) * 2 * kTile;
         const size_t at = size_t(64 * j) * st.kv;
         load_tile<HD, 4>(t, kb + at, length - 64 * j, st.kv, wave, lane);
         load_tile<HD, 4>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
     };
     load(0);
-    for (int j = 0; j < tiles; ++j) {
+    for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
-        const _Float16* kt = lds + (j & 1) * 2 * kTile;
+        const _Float16* kt = lds + ((i & 1) * kGroups + part) * 2 * kTile;
         const _Float16* vt = kt + kTile;
-        if (j + 1 < tiles) load(j + 1);
-        const int kbase = 64 * j;
+        if (i + 1 < steps) load(i + 1);
+        const int kbase = 64 * (kGroups * i + part);
         if (kbase > q0 + 31) continue;          // every key after every query of the wave
-        f32x16 s[2] = {};
+        // Scores are scaled by c inside the exponent's FMA; where the tile holds
+        // keys after a query (a uniform branch), before it, and masked.
+        auto scores = [&](f32x16 (&s)[2], unsigned zero) __attribute__((always_inline)) {
+            s[0] = s[1] = f32x16{};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
+            for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-            for (int hb = 0; hb < 2; ++hb) s[hb] = mfma(fo.row(kt, hb, kk), qf[kk], s[hb]);
-        // The tile's largest scaled score. Tiles that hold keys after a query
-        // scale first and mask (a uniform branch); the others take c max(s), or
-        // c min(s) for c < 0, and scale inside the exponent's FMA below.
-        float mx = -INFINITY, ce = c;
-        if (kbase + 63 > q0) {
+                for (int hb = 0; hb < 2; ++hb) s[hb] = mfma(fo.row(kt + zero, hb, kk), qf[kk], s[hb]);
+            if (kbase + 63 <= q0) return c;
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    float t = s[hb][r] * c;
-                    if (kbase + 32 * hb + result_row(r, h) > qi) t = -INFINITY;
-                    s[hb][r] = t;
-                    mx = fmaxf(mx, t);
+                    const bool seen = kbase + int(zero) + 32 * hb + result_row(r, h) <= qi;
+                    s[hb][r] = seen ? s[hb][r] * c : -INFINITY;
                 }
-            ce = 1.0f;
-        } else {
-#pragma unroll
-            for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, NEG ? -s[hb][r] : s[hb][r]);
-            mx *= NEG ? -c : c;
-        }
-        mx = fmaxf(mx, xor32(mx));
-        // m moves only when some query passes it by more than kRescale.
-        const float m_new = fmaxf(m, mx);
-        if (__any(m_new > m + kRescale)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-            l *= alpha;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
-            m = m_new;
-        }
-        float sum = 0.0f;
+            return 1.0f;
+        };
         f16x8 pf[4];
+        l += probabilities<2>(pf, scores, &m, &started, [&](float by) __attribute__((always_inline)) {
+            l *= by;
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hb][r], ce, -m));
-                pf[2 * hb + (r >> 3)][r & 7] = _Float16(p);
-                sum += p;
-            }
-        l += sum + xor32(sum);
+            for (int db = 0; db < DB; ++db) acc[db] *= by;
+        });
         // O^T += V^T P^T, a 16-key slice at a time (two for 64-wide heads).
         constexpr int kSlices = HD == 64 ? 2 : 1;
 #pragma unroll
@@ -247,6 +252,34 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
                     acc[db] = mfma(as_f16x8(vf[i][db]), pf[cs + i], acc[db]);
         }
     }
+    l += xor32(l);
+    if constexpr (kGroups > 1) {
+        // The groups' sums join in LDS: the second leaves its O^T [HD][32] a wave.
+        __syncthreads();
+        float* theirs = reinterpret_cast<float*>(lds) + wave * HD * 32;
+        if (part != 0) {
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    theirs[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
+            if (h == 0) sums[wave][fr] = float2{m, l};
+        }
+        __syncthreads();
+        if (part != 0) return;
+        const float2 other = sums[wave][fr];
+        const float most = fmaxf(m, other.x);
+        const float by = __builtin_amdgcn_exp2f(m - most);
+        const float other_by = __builtin_amdgcn_exp2f(other.x - most);
+        m = most;
+        l = __builtin_fmaf(other.y, other_by, l * by);
+#pragma unroll
+        for (int db = 0; db < DB; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                acc[db][r] = __builtin_fmaf(theirs[(32 * db + result_row(r, h)) * 32 + fr], other_by,
+                                            acc[db][r] * by);
+    }
     if (qi < length) {
         store_row<HD>(out + size_t(w.begin + qi) * st.o + size_t(w.head) * HD, acc, 1.0f / l, h);
         if (h == 0)
@@ -257,7 +290,7 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
 // ---------------------------------------------------------------- backward: dQ (and D)
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, HD == 64 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads * kGroups, 2)
 packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                    const _Float16* __restrict__ v, const _Float16* __restrict__ o,
@@ -265,11 +298,12 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
                    float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kGroups * 2 * kTile];   // [buf][group][K, V]
     Work w;
     if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
@@ -295,25 +329,27 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
     dd += xor32(dd);
     const size_t row_at = size_t(w.head) * tokens + w.begin + qi;
     const float lse2 = qi < length ? lse[row_at] * kLog2e : 0.0f;
-    if (qi < length && h == 0) dsum[row_at] = dd;
+    if (qi < length && h == 0 && part == 0) dsum[row_at] = dd;
 
     f32x16 acc[DB] = {};   // dQ^T[d][q]
     const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
-    const int tiles = q_last / 64 + 1;
-    auto load = [&](int j) {
-        _Float16* t = lds + (j & 1) * 2 * kTile;
+    const int tiles = q_last / 64 + 1, steps = (tiles + kGroups - 1) / kGroups;
+    auto load = [&](int i) {
+        const int j = kGroups * i + part;
+        if (j >= tiles) return;
+        _Float16* t = lds + ((i & 1) * kGroups + part) * 2 * kTile;
         const size_t at = kv_at + size_t(64 * j) * st.kv;
         load_tile<HD, 4>(t, k + at, length - 64 * j, st.kv, wave, lane);
         load_tile<HD, 4>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
     };
     load(0);
-    for (int j = 0; j < tiles; ++j) {
+    for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
-        const _Float16* kt = lds + (j & 1) * 2 * kTile;
+        const _Float16* kt = lds + ((i & 1) * kGroups + part) * 2 * kTile;
         const _Float16* vt = kt + kTile;
-        if (j + 1 < tiles) load(j + 1);
-        const int kbase = 64 * j;
+        if (i + 1 < steps) load(i + 1);
+        const int kbase = 64 * (kGroups * i + part);
         if (kbase > q0 + 31) continue;
         const bool masked = kbase + 63 > q0;
         // Two halves of 32 keys, each through all of its products before the
@@ -350,6 +386,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
             }
         }
     }
+    if (!join_groups<HD>(reinterpret_cast<float*>(lds), acc, wave, part, lane)) return;
     if (qi < length) store_row<HD>(dq + q_at + size_t(qi) * st.q, acc, scale, h);
 }
 
@@ -555,14 +592,13 @@ template <int HD>
 hipError_t forward(void* o, void* lse, const void* q, const void* k, const void* v,
                    const void* plan, const flint_packed_shape& s, float scale,
                    hipStream_t stream) {
-    auto* const kernel = scale < 0.0f ? packed_forward<HD, true> : packed_forward<HD, false>;
-    hipLaunchKernelGGL(kernel, dim3(unsigned(packed_items(s) * s.heads)), dim3(kThreads), 0, stream,
-                       static_cast<_Float16*>(o), static_cast<float*>(lse),
+    hipLaunchKernelGGL(packed_forward<HD>, dim3(unsigned(packed_items(s) * s.heads)), dim3(kThreads * kGroups),
+                       0, stream, static_cast<_Float16*>(o), static_cast<float*>(lse),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const int4*>(plan),
                        int(s.tokens), int(s.heads), int(s.heads / s.kv_heads),
                        Strides{int(s.q_stride), int(s.kv_stride), int(s.o_stride)},
-                       scale * kLog2e);
+                       std::fabs(scale) * kLog2e, scale < 0.0f);
     return hipGetLastError();
 }
 
@@ -574,7 +610,7 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     auto* dsum = static_cast<float*>(workspace);
     const int group = int(s.heads / s.kv_heads);
     hipLaunchKernelGGL(packed_backward_dq<HD>, dim3(unsigned(packed_items(s) * s.heads)),
-                       dim3(kThreads), 0, stream, static_cast<_Float16*>(dq), dsum,
+                       dim3(kThreads * kGroups), 0, stream, static_cast<_Float16*>(dq), dsum,
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(o),
                        static_cast<const _Float16*>(dout), static_cast<const float*>(lse),

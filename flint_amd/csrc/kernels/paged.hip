@@ -26,10 +26,6 @@ namespace flint {
 namespace {
 
 constexpr int kThreads = 256;   // 4 waves
-constexpr float kRescale = 8.0f;
-// A running maximum below every score: a tile may hold no visible key, and
-// exp2(-inf - kFloor) is 0.
-constexpr float kFloor = -3e38f;
 constexpr int kFewRows = 32, kManyRows = 128;
 // Workgroups aimed at, and the fewest tiles that a part of a sequence takes.
 constexpr int kFewTarget = 512, kManyTarget = 512;
@@ -223,66 +219,45 @@ struct Reader {
     }
 };
 
-// One tile of KEYS keys for a wave's 32 rows: scores, running maximum and sum,
+// One tile of KEYS keys for a wave's 32 rows: scores, probabilities and sum,
 // O^T += V^T P^T. valid: bit u for load u's pages.
 template <int HD, int KEYS>
 struct Rows {
     static constexpr int KK = HD / 16, DB = HD / 32, HB = KEYS / 32;
     f16x8 q[KK];
     float m = kFloor, l = 0.0f;
+    bool started = false;
     f32x16 acc[DB] = {};
 
     __device__ __forceinline__ void tile(const _Float16* kt, const _Float16* vt,
                                          const Frags<HD>& fo, int kbase, unsigned valid, int cached,
                                          int last, float c, int h) {
-        f32x16 s[HB] = {};
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-            for (int hb = 0; hb < HB; ++hb) s[hb] = mfma(fo.row(kt, hb, kk), q[kk], s[hb]);
         constexpr unsigned kAll = unsigned((1ull << (KEYS / Tile<HD>::kLoadRows)) - 1);
-        float mx = kFloor, ce = c;
-        if (kbase + KEYS > cached || valid != kAll) {
+        auto scores = [&](f32x16 (&s)[HB], unsigned zero) __attribute__((always_inline)) {
+#pragma unroll
+            for (int hb = 0; hb < HB; ++hb) s[hb] = f32x16{};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int hb = 0; hb < HB; ++hb) s[hb] = mfma(fo.row(kt + zero, hb, kk), q[kk], s[hb]);
+            if (kbase + KEYS <= cached && valid == kAll) return c;
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int in = 32 * hb + result_row(r, h), p = kbase + in;
-                    const bool paged = (valid >> (in / Tile<HD>::kLoadRows)) & 1;
+                    const int in = 32 * hb + result_row(r, h), p = kbase + int(zero) + in;
+                    const bool paged = ((valid + zero) >> (in / Tile<HD>::kLoadRows)) & 1;
                     const bool seen = p <= last && (paged || p >= cached);
-                    const float t = seen ? s[hb][r] * c : -INFINITY;
-                    s[hb][r] = t;
-                    mx = fmaxf(mx, t);
+                    s[hb][r] = seen ? s[hb][r] * c : -INFINITY;
                 }
-            ce = 1.0f;
-        } else {
-            mx = -INFINITY;
-#pragma unroll
-            for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[hb][r]);
-            mx *= c;
-        }
-        mx = fmaxf(mx, xor32(mx));
-        const float m_new = fmaxf(m, mx);
-        if (__any(m_new > m + kRescale)) {
-            const float alpha = __builtin_amdgcn_exp2f(m - m_new);
-            l *= alpha;
-#pragma unroll
-            for (int db = 0; db < DB; ++db) acc[db] *= alpha;
-            m = m_new;
-        }
-        float sum = 0.0f;
+            return 1.0f;
+        };
         f16x8 p[2 * HB];
+        l += probabilities<HB>(p, scores, &m, &started, [&](float by) __attribute__((always_inline)) {
+            l *= by;
 #pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[hb][r], ce, -m));
-                p[2 * hb + (r >> 3)][r & 7] = _Float16(e);
-                sum += e;
-            }
-        l += sum + xor32(sum);
+            for (int db = 0; db < DB; ++db) acc[db] *= by;
+        });
 #pragma unroll
         for (int cs = 0; cs < 2 * HB; ++cs) {
             TrFrag vf[DB];
@@ -293,6 +268,9 @@ struct Rows {
             for (int db = 0; db < DB; ++db) acc[db] = mfma(as_f16x8(vf[db]), p[cs], acc[db]);
         }
     }
+
+    // The keys' halves of a row, in lanes l and l ^ 32, become one.
+    __device__ __forceinline__ void finish() { l += xor32(l); }
 
     // Rows `row` of the sequence (32 from the wave's first), zeros from `rows` on.
     __device__ __forceinline__ void load_q(const PagedArgs& a, const Item& it, int head, int row,
@@ -399,6 +377,7 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
         w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
         valid = next;
     }
+    w.finish();
     // Joins the waves: each leaves O^T [HD][32] in its own tiles.
     float* own = reinterpret_cast<float*>(mine);
 #pragma unroll
@@ -495,6 +474,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
         w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
     }
     wait_vmcnt<0>();
+    w.finish();
     const int row = first_row + fr;
     if (row < rows) {
         if (it.parts == 1) {
