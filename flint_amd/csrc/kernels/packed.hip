@@ -27,6 +27,9 @@ namespace {
 
 constexpr int kThreads = 256;   // 4 waves of 32 queries (keys)
 constexpr int kGroups = 2;      // of 4 waves, which take the tiles in turn
+// The same for dK and dV, whose sums take all the registers at 128-wide heads.
+template <int HD>
+constexpr int kKeyGroups = HD == 64 ? 2 : 1;
 
 // ---------------------------------------------------------------- plan
 
@@ -138,9 +141,9 @@ struct Strides {
 
 // The groups' sums of one result added in LDS (4 waves' [HD][32] floats), into
 // the first group's; false in the others.
-template <int HD>
+template <int HD, int G>
 __device__ __forceinline__ bool join_groups(float* lds, f32x16* acc, int wave, int part, int lane) {
-    if constexpr (kGroups == 1) return true;
+    if constexpr (G == 1) return true;
     const int fr = lane & 31, h = lane >> 5;
     float* theirs = lds + wave * HD * 32;
     __syncthreads();
@@ -386,7 +389,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
             }
         }
     }
-    if (!join_groups<HD>(reinterpret_cast<float*>(lds), acc, wave, part, lane)) return;
+    if (!join_groups<HD, kGroups>(reinterpret_cast<float*>(lds), acc, wave, part, lane)) return;
     if (qi < length) store_row<HD>(dq + q_at + size_t(qi) * st.q, acc, scale, h);
 }
 
@@ -400,7 +403,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
 // sums ([part][token][kv head][HD], dK then dV) for packed_backward_join: heads
 // of k and v are few where groups are large, and so are workgroups then.
 template <int HD>
-__global__ void __launch_bounds__(kThreads, HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kThreads * kKeyGroups<HD>, HD == 64 ? 2 : 1)
 packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                      const _Float16* __restrict__ v, const _Float16* __restrict__ dout,
@@ -408,15 +411,17 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const int4* __restrict__ plan, float* __restrict__ sums, int tokens,
                      int kv_heads, int group, int share, Strides st, float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][Q, dO]
-    __shared__ __attribute__((aligned(16))) float rowstat[2][2][64];       // [buf][lse, D]
+    constexpr int G = kKeyGroups<HD>;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][Q, dO]
+    __shared__ __attribute__((aligned(16))) float rowstat[2][G][2][64];        // [buf][group][lse, D]
     Work w;
     const int parts = group / share;
     if (!work_of(plan, int(blockIdx.x), kv_heads * parts, tokens, &w)) return;
     const int part = w.head % parts;
     w.head /= parts;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
@@ -433,9 +438,12 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
     f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
     const int first = block * kPackedBlock / 64;
     const int per_head = (length + 63) / 64 - first;
-    const int steps = per_head * share;
+    const int tiles = per_head * share, steps = (tiles + G - 1) / G;
     auto stage = [&](int i) {
-        const int buf = i & 1, g = i / per_head, tile = first + i - g * per_head;
+        const int at_tile = G * i + turn;
+        if (at_tile >= tiles) return;
+        const int buf = (i & 1) * G + turn, g = at_tile / per_head;
+        const int tile = first + at_tile - g * per_head;
         const int head = w.head * group + part * share + g;
         _Float16* t = lds + buf * 2 * kTile;
         const int qq = 64 * tile + lane;
@@ -450,23 +458,25 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
         load_tile<HD, 4>(t + kTile, dout + row * st.o + size_t(head) * HD, length - 64 * tile, st.o,
                          wave, lane);
         if (wave == 0) {
-            rowstat[buf][0][lane] = lv * kLog2e;
-            rowstat[buf][1][lane] = dv0;
+            (&rowstat[0][0])[buf][0][lane] = lv * kLog2e;
+            (&rowstat[0][0])[buf][1][lane] = dv0;
         }
     };
     stage(0);
-    int tile = first;
+    int tile = first + turn % per_head;
     for (int i = 0; i < steps; ++i) {
-        const int buf = i & 1;
+        const int buf = (i & 1) * G + turn;
         wait_vmcnt<0>();
         __syncthreads();
         const _Float16* qt = lds + buf * 2 * kTile;
         const _Float16* gt = qt + kTile;
-        const float* l2 = rowstat[buf][0];
-        const float* dd = rowstat[buf][1];
+        const float* l2 = (&rowstat[0][0])[buf][0];
+        const float* dd = (&rowstat[0][0])[buf][1];
         if (i + 1 < steps) stage(i + 1);
         const int qbase = 64 * tile;
-        tile = tile + 1 == first + per_head ? first : tile + 1;
+        tile += G;
+        while (tile >= first + per_head) tile -= per_head;
+        if (G * i + turn >= tiles) break;
         if (qbase + 63 < k0) continue;        // every query before every key of the wave
         const bool masked = qbase < k0 + 31 || qbase + 63 >= length;
 #pragma unroll
@@ -516,7 +526,9 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             }
         }
     }
-    if (ki >= length) return;
+    join_groups<HD, G>(reinterpret_cast<float*>(lds), dka, wave, turn, lane);
+    if (!join_groups<HD, G>(reinterpret_cast<float*>(lds), dva, wave, turn, lane) || ki >= length)
+        return;
     if (parts == 1) {
         const size_t at = kv_at + size_t(ki) * st.kv;
         store_row<HD>(dk + at, dka, scale, h);
@@ -619,8 +631,8 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const size_t parts = group_parts(s), blocks = packed_items(s) * s.kv_heads;
     float* sums = dsum + dsum_values(s);
-    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(blocks * parts)), dim3(kThreads), 0,
-                       stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
+    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(blocks * parts)),
+                       dim3(kThreads * kKeyGroups<HD>), 0, stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(dout),
                        static_cast<const float*>(lse), static_cast<const float*>(dsum),
