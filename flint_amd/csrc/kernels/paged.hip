@@ -45,8 +45,9 @@ struct PagedArgs {
     int tokens, sequences, max_new, heads, kv_heads, group;
     int q_stride, kv_stride, o_stride;
     int pages, page_size, max_pages;
-    unsigned long long magic;   // column of position p: (p magic) >> shift
+    unsigned magic;   // column of position p: p / 8 times magic, high word >> shift
     int shift;
+    int page_rows;    // kv_heads x page_size
     float c;       // |scale| log2 e
     int negative;  // scale < 0: q enters negated
     int target;    // items a kv head aimed at
@@ -68,10 +69,13 @@ __device__ __forceinline__ Sequence sequence_of(const PagedArgs& a, int s) {
     return q;
 }
 
-// The table column of a position: an exact division by page_size, as a product
-// (positions stay below 2^31).
+// The table column of a position: an exact division of p / 8 (below 2^28) by
+// page_size / 8 = d, as the high word of a product. With 2^shift < d <=
+// 2^(shift + 1) and magic = floor(2^(32 + shift) / d) + 1, magic d - 2^(32 +
+// shift) is at most d, and 2^28 d at most 2^(29 + shift). d = 1 has magic 0.
 __device__ __forceinline__ int column_of(const PagedArgs& a, int p) {
-    return int((unsigned long long)(unsigned(p)) * a.magic >> a.shift);
+    const unsigned n = unsigned(p) >> 3;
+    return int(a.magic == 0 ? n : __umulhi(n, a.magic) >> a.shift);
 }
 
 template <class T>
@@ -173,7 +177,8 @@ struct Reader {
         const int page = p0 < cached ? table[column] : -1;   // cached ends inside the table
         const bool ok = page >= 0 && page < a.pages;
         const size_t from =
-            ok ? ((size_t(page) * a.kv_heads + kv) * a.page_size + (p0 - column * a.page_size)) * HD
+            ok ? (size_t(unsigned(page)) * unsigned(a.page_rows) +
+                  unsigned(kv * a.page_size + p0 - column * a.page_size)) * HD
                : 0;
         return {unsigned(from), unsigned(from >> 32),
                 ok ? unsigned(min(cached - p0, T::kLoadRows)) * HD * 2 : 0u};
@@ -514,10 +519,13 @@ __device__ __forceinline__ int sequence_at(const PagedArgs& a, int t, int lane) 
     return t >= q.first && t < q.first + q.count ? low : -1;
 }
 
-// One wave a row: the parts' results, weighted by their maxima's distance.
+// One wave a row: the parts' results, weighted by their maxima's distance. HD /
+// 4 lanes take 4 columns each, the wave's 4 or 2 sets of them the parts in
+// turn, and then add up.
 template <int HD>
 __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_block) {
-    const int lane = threadIdx.x & 63;
+    constexpr int kLanes = HD / 4, kSets = 64 / kLanes;
+    const int lane = threadIdx.x & 63, set = lane / kLanes, d = lane % kLanes * 4;
     const size_t id = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
     const int t = int(id / unsigned(a.heads)), head = int(id % unsigned(a.heads));
     if (t >= a.tokens) return;
@@ -529,24 +537,33 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_
     const int block = row / rows_of_block, first = split.x + block * split.y;
     // Slots outside the workspace can come from offsets that decrease only.
     if (split.y <= 1 || first < 0 || first + split.y > a.slots) return;
-    auto slot = [&](int p) {
-        return (size_t(first + p) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
-    };
-    float m = kFloor, l = 0.0f, sum[HD / 64] = {};
-    for (int p = lane; p < split.y; p += 64) m = fmaxf(m, a.sums[slot(p)].x);
+    const size_t step = size_t(a.kv_heads) * rows_of_block;
+    const size_t at = (size_t(first) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
+    float m = kFloor;
+    for (int p = lane; p < split.y; p += 64) m = fmaxf(m, a.sums[at + p * step].x);
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) m = fmaxf(m, __shfl_xor(m, d));
-    for (int p = 0; p < split.y; ++p) {
-        const float2 part = a.sums[slot(p)];
+    for (int i = 32; i > 0; i /= 2) m = fmaxf(m, __shfl_xor(m, i));
+    float l = 0.0f;
+    f32x4 sum = {};
+#pragma unroll 4
+    for (int p = set; p < split.y; p += kSets) {
+        const float2 part = a.sums[at + p * step];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.parts + (at + p * step) * HD + d);
         const float by = __builtin_amdgcn_exp2f(part.x - m);
         l = __builtin_fmaf(part.y, by, l);
-#pragma unroll
-        for (int i = 0; i < HD / 64; ++i)
-            sum[i] = __builtin_fmaf(a.parts[slot(p) * HD + 64 * i + lane], by, sum[i]);
+        sum += v * by;
     }
-    _Float16* o = a.o + size_t(t) * a.o_stride + size_t(head) * HD;
 #pragma unroll
-    for (int i = 0; i < HD / 64; ++i) o[64 * i + lane] = _Float16(sum[i] / l);
+    for (int i = kLanes; i < 64; i *= 2) {
+        l += __shfl_xor(l, i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], i);
+    }
+    if (set != 0) return;
+    const float inv = 1.0f / l;
+    const f16x4 v = {_Float16(sum[0] * inv), _Float16(sum[1] * inv), _Float16(sum[2] * inv),
+                     _Float16(sum[3] * inv)};
+    *reinterpret_cast<f16x4*>(a.o + size_t(t) * a.o_stride + size_t(head) * HD + d) = v;
 }
 
 bool many_rows(const flint_paged_shape& s) {
@@ -601,9 +618,10 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
     const Sizes z = sizes_of(s);
     const Space w = space_of(s, z);
     auto* ws = static_cast<char*>(workspace);
-    // Round-up reciprocal: exact while position x page_size < 2^shift.
-    int shift = 32;
-    while ((size_t{1} << (shift - 32)) < s.page_size) ++shift;
+    const size_t eighths = s.page_size / 8;
+    int shift = 0;
+    while ((size_t{2} << shift) < eighths) ++shift;
+    const unsigned magic = eighths == 1 ? 0u : unsigned((size_t{1} << (32 + shift)) / eighths + 1);
     PagedArgs a{static_cast<_Float16*>(o), static_cast<_Float16*>(k_pages),
                 static_cast<_Float16*>(v_pages), static_cast<const _Float16*>(q),
                 static_cast<const _Float16*>(k), static_cast<const _Float16*>(v),
@@ -612,7 +630,7 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                 int(std::min(s.max_new, s.tokens)), int(s.heads), int(s.kv_heads),
                 int(s.heads / s.kv_heads), int(s.q_stride), int(s.kv_stride), int(s.o_stride),
                 int(s.pages), int(s.page_size), int(s.max_pages),
-                (1ull << shift) / s.page_size + 1, shift, std::fabs(scale) * kLog2e, scale < 0.0f,
+                magic, shift, int(s.kv_heads * s.page_size), std::fabs(scale) * kLog2e, scale < 0.0f,
                 int(z.target), int(z.slots), reinterpret_cast<int2*>(ws),
                 reinterpret_cast<float2*>(ws + w.sums), reinterpret_cast<float*>(ws + w.parts)};
     const dim3 grid(unsigned((z.blocks + z.target) * s.kv_heads));
