@@ -223,13 +223,12 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
 #pragma unroll
                 for (int hb = 0; hb < 2; ++hb) s[hb] = mfma(fo.row(kt + zero, hb, kk), qf[kk], s[hb]);
             if (kbase + 63 <= q0) return c;
+            const int seen = qi - kbase - 4 * h + int(zero);   // a register's key: a constant + 4h
 #pragma unroll
             for (int hb = 0; hb < 2; ++hb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const bool seen = kbase + int(zero) + 32 * hb + result_row(r, h) <= qi;
-                    s[hb][r] = seen ? s[hb][r] * c : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)
+                    s[hb][r] = 32 * hb + result_row(r, 0) <= seen ? s[hb][r] * c : -INFINITY;
             return 1.0f;
         };
         f16x8 pf[4];

@@ -28,8 +28,8 @@ namespace {
 constexpr int kThreads = 256;   // 4 waves
 constexpr int kFewRows = 32, kManyRows = 128;
 // Workgroups aimed at, and the fewest tiles that a part of a sequence takes.
-constexpr int kFewTarget = 512, kManyTarget = 512;
-constexpr int kFewTiles = 8, kManyTiles = 4;
+constexpr int kFewTarget = 1024, kManyTarget = 768;
+constexpr int kFewTiles = 4, kManyTiles = 4;
 
 template <int HD, bool MANY>
 struct Plan {
@@ -78,19 +78,20 @@ __device__ __forceinline__ int column_of(const PagedArgs& a, int p) {
     return int(a.magic == 0 ? n : __umulhi(n, a.magic) >> a.shift);
 }
 
-template <class T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v += __shfl_xor(v, d);
+// Inclusive prefix sum over the wave by lane exchanges within the vector unit:
+// 1, 2, 4 and 8 lanes up within 16, then the last lane of a row of 16, and of
+// the first 32, to those above.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
     return v;
 }
-__device__ __forceinline__ int wave_scan(int v, int lane) {   // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int w = __shfl_up(v, d);
-        if (lane >= d) v += w;
-    }
-    return v;
+__device__ __forceinline__ int wave_sum(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v), 63);
 }
 
 // Item `idx` of a kv head. Every item takes about the same number of tiles,
@@ -114,8 +115,13 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
         if (s0 + lane < a.sequences) q = sequence_of(a, s0 + lane);
         total += (long long)(blocks_of(q)) * tiles_of(q);
     }
-    total = wave_sum(total);
-    const int each = max(P::kLeast, int((total + a.target - 1) / a.target));
+    // In two words: the rows' blocks add up to at most 2^21, tiles are at most
+    // 2^26.
+    total = ((long long)(wave_sum(int(total >> 20))) << 20) + wave_sum(int(total & 0xfffff));
+    int each = max(P::kLeast, int((total + a.target - 1) / a.target));
+    // Few rows: a workgroup on each CU first (a quarter of the target), then
+    // parts of 16 tiles, and only then more of them.
+    if constexpr (!MANY) each = max(each, int(min(16ll, (4 * total + a.target - 1) / a.target)));
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
         if (a.sequences > 64) {
@@ -124,8 +130,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
         }
         const int parts = (tiles_of(q) + each - 1) / each;
         const int items = blocks_of(q) * parts;
-        const int upto = wave_scan(items, lane);
-        const int held = wave_scan(parts > 1 ? items : 0, lane);
+        const int upto = wave_scan(items);
+        const int held = wave_scan(parts > 1 ? items : 0);
         const unsigned long long past = __ballot(before + upto > idx);
         if (past != 0) {
             const int at = __ffsll(past) - 1;
@@ -246,15 +252,25 @@ struct Rows {
 #pragma unroll
                 for (int hb = 0; hb < HB; ++hb) s[hb] = mfma(fo.row(kt + zero, hb, kk), q[kk], s[hb]);
             if (kbase + KEYS <= cached && valid == kAll) return c;
+            // Keys after the query: the register's key is a constant plus 4h.
+            const int seen = last - kbase - 4 * h + int(zero);
 #pragma unroll
             for (int hb = 0; hb < HB; ++hb)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int in = 32 * hb + result_row(r, h), p = kbase + int(zero) + in;
-                    const bool paged = ((valid + zero) >> (in / Tile<HD>::kLoadRows)) & 1;
-                    const bool seen = p <= last && (paged || p >= cached);
-                    s[hb][r] = seen ? s[hb][r] * c : -INFINITY;
-                }
+                for (int r = 0; r < 16; ++r)
+                    s[hb][r] = 32 * hb + result_row(r, 0) <= seen ? s[hb][r] * c : -INFINITY;
+            if (valid != kAll) {
+                const int fresh = cached - kbase - 4 * h;
+                const unsigned paged = HD == 64 ? valid : valid >> h;
+#pragma unroll
+                for (int hb = 0; hb < HB; ++hb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        constexpr int kRows = Tile<HD>::kLoadRows;
+                        const int in = 32 * hb + result_row(r, 0);
+                        if (!(paged >> (in / kRows) & 1) && in < fresh) s[hb][r] = -INFINITY;
+                    }
+            }
             return 1.0f;
         };
         f16x8 p[2 * HB];
@@ -363,6 +379,7 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
         issue(at, t, 0);
         at = reader.find(t + 4);
     }
+    store_new<HD>(a, it, head, kFewRows);   // waits for no more than the tile does
     for (int i = 0; t < to; ++i, t += 4) {
         unsigned next = 0;
         // The other buffer's reads ended with the last tile's products.
@@ -429,7 +446,6 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
                     f32x4{sum[d], sum[d + 1], sum[d + 2], sum[d + 3]};
         }
     }
-    store_new<HD>(a, it, head, kFewRows);
 }
 
 template <int HD>
@@ -465,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
         issue(at, from);
         at = reader.find(from + 1);
     }
+    store_new<HD>(a, it, head, kManyRows);
     for (int t = from; t < to; ++t) {
         const unsigned valid = next;
         wait_vmcnt<0>();
@@ -500,7 +517,6 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
                               w.acc[db][4 * i + 3]};
         }
     }
-    store_new<HD>(a, it, head, kManyRows);
 }
 
 // The sequence that token t belongs to, or -1: 64 offsets a step.
@@ -519,14 +535,19 @@ __device__ __forceinline__ int sequence_at(const PagedArgs& a, int t, int lane) 
     return t >= q.first && t < q.first + q.count ? low : -1;
 }
 
-// One wave a row: the parts' results, weighted by their maxima's distance. HD /
-// 4 lanes take 4 columns each, the wave's 4 or 2 sets of them the parts in
-// turn, and then add up.
-template <int HD>
+// WAVES waves a row: the parts' results, weighted by their maxima's distance.
+// HD / 4 lanes take 4 columns each, the waves' sets of such lanes the parts in
+// turn, and then add up. One wave where rows are many; four where they are few
+// and a sequence may have a thousand parts.
+template <int HD, int WAVES>
 __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_block) {
     constexpr int kLanes = HD / 4, kSets = 64 / kLanes;
-    const int lane = threadIdx.x & 63, set = lane / kLanes, d = lane % kLanes * 4;
-    const size_t id = size_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    __shared__ __attribute__((aligned(16))) f32x4 wave_parts[WAVES][kLanes];
+    __shared__ float wave_sums[WAVES];
+    const int lane = threadIdx.x & 63, d = lane % kLanes * 4;
+    const int wave = WAVES == 1 ? 0 : int(threadIdx.x >> 6);
+    const int set = wave * kSets + lane / kLanes;
+    const size_t id = WAVES == 1 ? size_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : blockIdx.x;
     const int t = int(id / unsigned(a.heads)), head = int(id % unsigned(a.heads));
     if (t >= a.tokens) return;
     const int s = sequence_at(a, t, lane);
@@ -546,7 +567,7 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_
     float l = 0.0f;
     f32x4 sum = {};
 #pragma unroll 4
-    for (int p = set; p < split.y; p += kSets) {
+    for (int p = set; p < split.y; p += kSets * WAVES) {
         const float2 part = a.sums[at + p * step];
         const f32x4 v = *reinterpret_cast<const f32x4*>(a.parts + (at + p * step) * HD + d);
         const float by = __builtin_amdgcn_exp2f(part.x - m);
@@ -558,6 +579,18 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_
         l += __shfl_xor(l, i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], i);
+    }
+    if constexpr (WAVES > 1) {
+        if (lane < kLanes) wave_parts[wave][lane] = sum;
+        if (lane == 0) wave_sums[wave] = l;
+        __syncthreads();
+        l = 0.0f;
+        sum = f32x4{};
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+            l += wave_sums[w];
+            sum += wave_parts[w][lane % kLanes];
+        }
     }
     if (set != 0) return;
     const float inv = 1.0f / l;
@@ -639,9 +672,11 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                               : (wide ? paged_few<128> : paged_few<64>);
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
-    auto* const join = wide ? paged_join<128> : paged_join<64>;
-    hipLaunchKernelGGL(join, dim3(unsigned((s.tokens * s.heads + 3) / 4)), dim3(kThreads), 0, stream,
-                       a, int(z.rows));
+    auto* const join = many ? (wide ? paged_join<128, 1> : paged_join<64, 1>)
+                            : (wide ? paged_join<128, 4> : paged_join<64, 4>);
+    const size_t joined = s.tokens * s.heads;
+    hipLaunchKernelGGL(join, dim3(unsigned(many ? (joined + 3) / 4 : joined)), dim3(kThreads), 0,
+                       stream, a, int(z.rows));
     return hipGetLastError();
 }
 
