@@ -535,41 +535,54 @@ __device__ __forceinline__ int sequence_at(const PagedArgs& a, int t, int lane) 
     return t >= q.first && t < q.first + q.count ? low : -1;
 }
 
-// WAVES waves a row: the parts' results, weighted by their maxima's distance.
-// HD / 4 lanes take 4 columns each, the waves' sets of such lanes the parts in
-// turn, and then add up. One wave where rows are many; four where they are few
-// and a sequence may have a thousand parts.
-template <int HD, int WAVES>
-__global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_block) {
-    constexpr int kLanes = HD / 4, kSets = 64 / kLanes;
-    __shared__ __attribute__((aligned(16))) f32x4 wave_parts[WAVES][kLanes];
-    __shared__ float wave_sums[WAVES];
-    const int lane = threadIdx.x & 63, d = lane % kLanes * 4;
-    const int wave = WAVES == 1 ? 0 : int(threadIdx.x >> 6);
-    const int set = wave * kSets + lane / kLanes;
-    const size_t id = WAVES == 1 ? size_t(blockIdx.x) * 4 + (threadIdx.x >> 6) : blockIdx.x;
-    const int t = int(id / unsigned(a.heads)), head = int(id % unsigned(a.heads));
-    if (t >= a.tokens) return;
-    const int s = sequence_at(a, t, lane);
-    if (s < 0) return;
-    const Sequence q = sequence_of(a, s);
-    const int2 split = a.splits[s];
+__device__ __forceinline__ void store_joined(_Float16* o, const f32x4& sum, float by) {
+    *reinterpret_cast<f16x4*>(o) = f16x4{_Float16(sum[0] * by), _Float16(sum[1] * by),
+                                         _Float16(sum[2] * by), _Float16(sum[3] * by)};
+}
+
+// A row's parts in the workspace: false where it has none to join.
+struct Parts {
+    size_t at, step;   // of the first part's row, in rows
+    int count;
+};
+__device__ __forceinline__ bool parts_of_row(const PagedArgs& a, const Sequence& q, int2 split,
+                                             int t, int head, int rows_of_block, Parts* p) {
     const int kv = head / a.group, row = (t - q.first) * a.group + head - kv * a.group;
     const int block = row / rows_of_block, first = split.x + block * split.y;
+    p->step = size_t(a.kv_heads) * rows_of_block;
+    p->at = (size_t(first) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
+    p->count = split.y;
     // Slots outside the workspace can come from offsets that decrease only.
-    if (split.y <= 1 || first < 0 || first + split.y > a.slots) return;
-    const size_t step = size_t(a.kv_heads) * rows_of_block;
-    const size_t at = (size_t(first) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
+    return split.y > 1 && first >= 0 && first + split.y <= a.slots;
+}
+
+// The parts' results, weighted by their maxima's distance; HD / 4 lanes (a set)
+// take 4 columns of a row each.
+//
+// Few rows: four waves a row, whose sets take the parts in turn (a sequence may
+// have a thousand) and then add up.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a, int rows_of_block) {
+    constexpr int kLanes = HD / 4, kSets = 64 / kLanes, kWaves = kThreads / 64;
+    __shared__ __attribute__((aligned(16))) f32x4 wave_parts[kWaves][kLanes];
+    __shared__ float wave_sums[kWaves];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane % kLanes * 4;
+    const int set = wave * kSets + lane / kLanes;
+    const int t = int(blockIdx.x / unsigned(a.heads)), head = int(blockIdx.x % unsigned(a.heads));
+    const int s = sequence_at(a, t, lane);
+    if (s < 0) return;
+    Parts p;
+    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, rows_of_block, &p)) return;
     float m = kFloor;
-    for (int p = lane; p < split.y; p += 64) m = fmaxf(m, a.sums[at + p * step].x);
+    for (int i = lane; i < p.count; i += 64) m = fmaxf(m, a.sums[p.at + i * p.step].x);
 #pragma unroll
     for (int i = 32; i > 0; i /= 2) m = fmaxf(m, __shfl_xor(m, i));
     float l = 0.0f;
     f32x4 sum = {};
 #pragma unroll 4
-    for (int p = set; p < split.y; p += kSets * WAVES) {
-        const float2 part = a.sums[at + p * step];
-        const f32x4 v = *reinterpret_cast<const f32x4*>(a.parts + (at + p * step) * HD + d);
+    for (int i = set; i < p.count; i += kSets * kWaves) {
+        const float2 part = a.sums[p.at + i * p.step];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.parts + (p.at + i * p.step) * HD + d);
         const float by = __builtin_amdgcn_exp2f(part.x - m);
         l = __builtin_fmaf(part.y, by, l);
         sum += v * by;
@@ -580,23 +593,48 @@ __global__ void __launch_bounds__(kThreads) paged_join(PagedArgs a, int rows_of_
 #pragma unroll
         for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], i);
     }
-    if constexpr (WAVES > 1) {
-        if (lane < kLanes) wave_parts[wave][lane] = sum;
-        if (lane == 0) wave_sums[wave] = l;
-        __syncthreads();
-        l = 0.0f;
-        sum = f32x4{};
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-            l += wave_sums[w];
-            sum += wave_parts[w][lane % kLanes];
-        }
-    }
+    if (lane < kLanes) wave_parts[wave][lane] = sum;
+    if (lane == 0) wave_sums[wave] = l;
+    __syncthreads();
     if (set != 0) return;
-    const float inv = 1.0f / l;
-    const f16x4 v = {_Float16(sum[0] * inv), _Float16(sum[1] * inv), _Float16(sum[2] * inv),
-                     _Float16(sum[3] * inv)};
-    *reinterpret_cast<f16x4*>(a.o + size_t(t) * a.o_stride + size_t(head) * HD + d) = v;
+    l = 0.0f;
+    sum = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+        l += wave_sums[w];
+        sum += wave_parts[w][lane];
+    }
+    store_joined(a.o + size_t(t) * a.o_stride + size_t(head) * HD + d, sum, 1.0f / l);
+}
+
+// Many rows, of few parts each: a set a row, a wave on heads of one token, since
+// finding the token's sequence is a chain of loads.
+template <int HD>
+__global__ void __launch_bounds__(kThreads) paged_join_many(PagedArgs a, int rows_of_block) {
+    constexpr int kLanes = HD / 4, kSets = 64 / kLanes;
+    const int lane = threadIdx.x & 63, d = lane % kLanes * 4;
+    const unsigned id = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+    const unsigned runs = unsigned(a.heads + kSets - 1) / kSets;   // of kSets heads
+    const int t = int(id / runs), head = int(id % runs) * kSets + lane / kLanes;
+    if (t >= a.tokens) return;
+    const int s = sequence_at(a, t, lane);
+    if (s < 0 || head >= a.heads) return;
+    Parts p;
+    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, rows_of_block, &p)) return;
+    float m = kFloor;
+#pragma unroll 4
+    for (int i = 0; i < p.count; ++i) m = fmaxf(m, a.sums[p.at + i * p.step].x);
+    float l = 0.0f;
+    f32x4 sum = {};
+#pragma unroll 4
+    for (int i = 0; i < p.count; ++i) {
+        const float2 part = a.sums[p.at + i * p.step];
+        const f32x4 v = *reinterpret_cast<const f32x4*>(a.parts + (p.at + i * p.step) * HD + d);
+        const float by = __builtin_amdgcn_exp2f(part.x - m);
+        l = __builtin_fmaf(part.y, by, l);
+        sum += v * by;
+    }
+    store_joined(a.o + size_t(t) * a.o_stride + size_t(head) * HD + d, sum, 1.0f / l);
 }
 
 bool many_rows(const flint_paged_shape& s) {
@@ -672,11 +710,17 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                               : (wide ? paged_few<128> : paged_few<64>);
     hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
-    auto* const join = many ? (wide ? paged_join<128, 1> : paged_join<64, 1>)
-                            : (wide ? paged_join<128, 4> : paged_join<64, 4>);
-    const size_t joined = s.tokens * s.heads;
-    hipLaunchKernelGGL(join, dim3(unsigned(many ? (joined + 3) / 4 : joined)), dim3(kThreads), 0,
-                       stream, a, int(z.rows));
+    // Waves enough for the GPU without sharing a row out.
+    const size_t rows = s.tokens * s.heads, sets = 256 / s.head_width;
+    if (rows <= 4096) {
+        auto* const join = wide ? paged_join_few<128> : paged_join_few<64>;
+        hipLaunchKernelGGL(join, dim3(unsigned(rows)), dim3(kThreads), 0, stream, a, int(z.rows));
+    } else {
+        auto* const join = wide ? paged_join_many<128> : paged_join_many<64>;
+        const size_t waves = s.tokens * ((s.heads + sets - 1) / sets);
+        hipLaunchKernelGGL(join, dim3(unsigned((waves + 3) / 4)), dim3(kThreads), 0, stream, a,
+                           int(z.rows));
+    }
     return hipGetLastError();
 }
 
