@@ -26,9 +26,11 @@ namespace flint {
 namespace {
 
 constexpr int kThreads = 256;   // 4 waves
+constexpr int kGroups = 2;      // of 4 waves, where rows are many
 constexpr int kFewRows = 32, kManyRows = 128;
-// Workgroups aimed at, and the fewest tiles that a part of a sequence takes.
-constexpr int kFewTarget = 1024, kManyTarget = 768;
+// Workgroups aimed at (many rows: what the GPU holds at once, two a CU at width
+// 64 and one at 128), and the fewest tiles that a part of a sequence takes.
+constexpr int kFewTarget = 1024, kManyTarget = 512;
 constexpr int kFewTiles = 4, kManyTiles = 4;
 
 template <int HD, bool MANY>
@@ -94,6 +96,12 @@ __device__ __forceinline__ int wave_sum(int v) {
     return __builtin_amdgcn_readlane(wave_scan(v), 63);
 }
 
+__device__ __forceinline__ int wave_max(int v) {
+#pragma unroll
+    for (int d = 32; d > 0; d /= 2) v = max(v, __shfl_xor(v, d));
+    return v;
+}
+
 // Item `idx` of a kv head. Every item takes about the same number of tiles,
 // total / target: the sequences' lengths are known only here, so each wave adds
 // them up (64 sequences a step) and finds its item by a prefix sum.
@@ -122,6 +130,15 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     // Few rows: a workgroup on each CU first (a quarter of the target), then
     // parts of 16 tiles, and only then more of them.
     if constexpr (!MANY) each = max(each, int(min(16ll, (4 * total + a.target - 1) / a.target)));
+    // Many rows: the target is what the GPU holds at once, and parts that round
+    // up past it would run behind the others. (One step of sequences only; the
+    // parts of more are many anyway.)
+    if constexpr (MANY)
+        for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
+            const int parts = (tiles_of(q) + each - 1) / each;
+            if (wave_sum(blocks_of(q) * parts) <= a.target || wave_max(parts) <= 1) break;
+            each += (each + 7) / 8;
+        }
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
         if (a.sequences > 64) {
@@ -319,13 +336,13 @@ __device__ __forceinline__ void part_of(const PagedArgs& a, const Item& it, int 
 
 // The new rows of k and v that start in a block of query rows go to their
 // pages; a block's part 0 does it.
-template <int HD>
+template <int HD, int THREADS>
 __device__ __forceinline__ void store_new(const PagedArgs& a, const Item& it, int head,
                                           int rows_of_block) {
     if (it.part != 0) return;
     const int from = (it.block * rows_of_block + a.group - 1) / a.group;
     const int to = min(((it.block + 1) * rows_of_block + a.group - 1) / a.group, it.seq.count);
-    for (int i = threadIdx.x; i < (to - from) * (HD / 8); i += kThreads) {
+    for (int i = threadIdx.x; i < (to - from) * (HD / 8); i += THREADS) {
         const int place = from + i / (HD / 8), d = i % (HD / 8) * 8;
         const int p = it.seq.cached + place, column = column_of(a, p);
         if (column >= a.max_pages) continue;
@@ -379,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
         issue(at, t, 0);
         at = reader.find(t + 4);
     }
-    store_new<HD>(a, it, head, kFewRows);   // waits for no more than the tile does
+    store_new<HD, kThreads>(a, it, head, kFewRows);   // waits for no more than the tile does
     for (int i = 0; t < to; ++i, t += 4) {
         unsigned next = 0;
         // The other buffer's reads ended with the last tile's products.
@@ -449,13 +466,15 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
+__global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2) paged_many(PagedArgs a) {
     using P = Plan<HD, true>;
     constexpr int kTile = Tile<HD>::kHalves;
     constexpr int kEach = Tile<HD>::kLoads / 4;   // loads of a wave, of K and of V
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * 2 * kTile];   // [buf][K, V]
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kGroups * 2 * kTile];   // [buf][group][K, V]
+    __shared__ float2 sums[4][32];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int fr = lane & 31, h = lane >> 5;
     const int head = int(blockIdx.x % unsigned(a.kv_heads));
     Item it;
@@ -470,53 +489,78 @@ __global__ void __launch_bounds__(kThreads, 2) paged_many(PagedArgs a) {
     const Reader<HD, P::kKeys> reader(a, it, head, lane);
     int from, to;
     part_of(a, it, kManyRows, P::kKeys, &from, &to);
-    auto issue = [&](const Where& at, int t) __attribute__((always_inline)) {
-        _Float16* kt = lds + (t & 1) * 2 * kTile;
+    auto issue = [&](const Where& at, int t, int buf) __attribute__((always_inline)) {
+        _Float16* kt = lds + (buf * kGroups + turn) * 2 * kTile;
 #pragma unroll
         for (int i = 0; i < kEach; ++i) reader.load(kt, kt + kTile, at, t, wave + 4 * i);
     };
-    Where at = reader.find(from);
-    unsigned next = reader.valid(at, from);
-    if (from < to) {
-        issue(at, from);
-        at = reader.find(from + 1);
+    int t = from + turn;
+    Where at = reader.find(t);
+    unsigned next = reader.valid(at, t);
+    if (t < to) {
+        issue(at, t, 0);
+        at = reader.find(t + kGroups);
     }
-    store_new<HD>(a, it, head, kManyRows);
-    for (int t = from; t < to; ++t) {
+    store_new<HD, kThreads * kGroups>(a, it, head, kManyRows);
+    const int steps = (to - from + kGroups - 1) / kGroups;
+    for (int i = 0; i < steps; ++i, t += kGroups) {
         const unsigned valid = next;
         wait_vmcnt<0>();
         block_sync();
-        if (t + 1 < to) {
-            next = reader.valid(at, t + 1);
-            issue(at, t + 1);
-            at = reader.find(t + 2);
+        if (t + kGroups < to) {
+            next = reader.valid(at, t + kGroups);
+            issue(at, t + kGroups, (i + 1) & 1);
+            at = reader.find(t + 2 * kGroups);
         }
-        if (first_row >= rows || t * P::kKeys > wave_last) continue;   // no row here, or none sees it
-        const _Float16* kt = lds + (t & 1) * 2 * kTile;
+        // No tile for this group, no row of this wave, or none that sees it.
+        if (t >= to || first_row >= rows || t * P::kKeys > wave_last) continue;
+        const _Float16* kt = lds + ((i & 1) * kGroups + turn) * 2 * kTile;
         w.tile(kt, kt + kTile, fo, t * P::kKeys, valid, it.seq.cached, last, a.c, h);
     }
     wait_vmcnt<0>();
     w.finish();
-    const int row = first_row + fr;
-    if (row < rows) {
-        if (it.parts == 1) {
-            const int place = row / a.group;
-            store_row<HD>(a.o + size_t(it.seq.first + place) * a.o_stride +
-                              size_t(head * a.group + row - place * a.group) * HD,
-                          w.acc, 1.0f / w.l, h);
-        } else {
-            const size_t at =
-                (size_t(it.slot + it.part) * a.kv_heads + head) * kManyRows + wave * 32 + fr;
-            if (h == 0) a.sums[at] = float2{w.m, w.l};
+    // The second group's sums join the first's in LDS, as in packed.hip.
+    float* theirs = reinterpret_cast<float*>(lds) + wave * HD * 32;
+    __syncthreads();
+    if (turn != 0) {
 #pragma unroll
-            for (int db = 0; db < HD / 32; ++db)
+        for (int db = 0; db < HD / 32; ++db)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<f32x4*>(a.parts + at * HD + 32 * db + 8 * i + 4 * h) =
-                        f32x4{w.acc[db][4 * i], w.acc[db][4 * i + 1], w.acc[db][4 * i + 2],
-                              w.acc[db][4 * i + 3]};
-        }
+            for (int r = 0; r < 16; ++r)
+                theirs[(32 * db + result_row(r, h)) * 32 + fr] = w.acc[db][r];
+        if (h == 0) sums[wave][fr] = float2{w.m, w.l};
     }
+    __syncthreads();
+    const int row = first_row + fr;
+    if (turn != 0 || row >= rows) return;
+    const float2 other = sums[wave][fr];
+    const float most = fmaxf(w.m, other.x);
+    const float by = __builtin_amdgcn_exp2f(w.m - most);
+    const float other_by = __builtin_amdgcn_exp2f(other.x - most);
+    w.l = __builtin_fmaf(other.y, other_by, w.l * by);
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            w.acc[db][r] = __builtin_fmaf(theirs[(32 * db + result_row(r, h)) * 32 + fr], other_by,
+                                          w.acc[db][r] * by);
+    if (it.parts == 1) {
+        const int place = row / a.group;
+        store_row<HD>(a.o + size_t(it.seq.first + place) * a.o_stride +
+                          size_t(head * a.group + row - place * a.group) * HD,
+                      w.acc, 1.0f / w.l, h);
+        return;
+    }
+    const size_t slot =
+        (size_t(it.slot + it.part) * a.kv_heads + head) * kManyRows + wave * 32 + fr;
+    if (h == 0) a.sums[slot] = float2{most, w.l};
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(a.parts + slot * HD + 32 * db + 8 * i + 4 * h) =
+                f32x4{w.acc[db][4 * i], w.acc[db][4 * i + 1], w.acc[db][4 * i + 2],
+                      w.acc[db][4 * i + 3]};
 }
 
 // The sequence that token t belongs to, or -1: 64 offsets a step.
@@ -655,7 +699,8 @@ Sizes sizes_of(const flint_paged_shape& s) {
     const size_t keys = many || s.head_width == 64 ? 64 : 32;
     const size_t least = many ? kManyTiles : kFewTiles;
     const size_t group = s.heads / s.kv_heads, new_rows = std::min(s.max_new, s.tokens) * group;
-    z.target = std::max<size_t>(1, (many ? kManyTarget : kFewTarget) / s.kv_heads);
+    const size_t target = many ? kManyTarget * 64 / s.head_width : kFewTarget;
+    z.target = std::max<size_t>(1, target / s.kv_heads);
     z.blocks = std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
                         s.tokens * group / z.rows + s.sequences);
     const size_t longest = (s.max_pages * s.page_size + s.max_new + keys - 1) / keys;
@@ -708,7 +753,7 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
     const bool many = many_rows(s), wide = s.head_width == 128;
     auto* const kernel = many ? (wide ? paged_many<128> : paged_many<64>)
                               : (wide ? paged_few<128> : paged_few<64>);
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
     // Waves enough for the GPU without sharing a row out.
     const size_t rows = s.tokens * s.heads, sets = 256 / s.head_width;
