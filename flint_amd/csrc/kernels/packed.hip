@@ -25,11 +25,26 @@
 namespace flint {
 namespace {
 
-constexpr int kThreads = 256;   // 4 waves of 32 queries (keys)
-constexpr int kGroups = 2;      // of 4 waves, which take the tiles in turn
-// The same for dK and dV, whose sums take all the registers at 128-wide heads.
+constexpr int kThreads = 256;   // of the joining launch
+
+// A workgroup's waves: `rows` of them over its 32 x rows queries (keys), times
+// `turns` groups that take the 64-row tiles in turn and join their sums in LDS
+// at the end. Two turns halve the longest block's time, which bounds batches of
+// different lengths (one head of one 3,913-token sequence: forward 53 -> 41 us,
+// backward 163 -> 110; the forward of 12 heads and 24 sequences up to that
+// length 59 -> 53), and cost batches of equal short ones some of their second
+// round of workgroups (8 x 1,024 tokens, 12 heads: forward 24 -> 29). Two rows
+// and four turns shorten that block more (25 us), but read each tile for half
+// the rows (one 8,192-token sequence 127 -> 182). dK and dV at 128-wide heads
+// take a wave's 512 registers: one turn (two rows and two turns: 616 -> 634).
+struct Waves {
+    int rows, turns;
+    constexpr int threads() const { return 64 * rows * turns; }
+    constexpr int parts() const { return kPackedBlock / (32 * rows); }   // workgroups of a block
+};
+constexpr Waves kForward{4, 2}, kQuery{4, 2};
 template <int HD>
-constexpr int kKeyGroups = HD == 64 ? 2 : 1;
+constexpr Waves kKey = HD == 64 ? Waves{4, 2} : Waves{4, 1};
 
 // ---------------------------------------------------------------- plan
 
@@ -139,52 +154,59 @@ struct Strides {
     int q, kv, o;
 };
 
-// The groups' sums of one result added in LDS (4 waves' [HD][32] floats), into
-// the first group's; false in the others.
-template <int HD, int G>
-__device__ __forceinline__ bool join_groups(float* lds, f32x16* acc, int wave, int part, int lane) {
+// The turns' sums of one result added in LDS, in order, into the first's; false
+// in the others.
+template <int HD, int W, int G>
+__device__ __forceinline__ bool join_turns(float* lds, f32x16* acc, int wave, int turn, int lane) {
     if constexpr (G == 1) return true;
     const int fr = lane & 31, h = lane >> 5;
-    float* theirs = lds + wave * HD * 32;
+    auto theirs = [&](int g) { return lds + ((g - 1) * W + wave) * HD * 32; };
     __syncthreads();
-    if (part != 0) {
+    if (turn != 0) {
 #pragma unroll
         for (int db = 0; db < HD / 32; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) theirs[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
+            for (int r = 0; r < 16; ++r)
+                theirs(turn)[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
     }
     __syncthreads();
-    if (part != 0) return false;
+    if (turn != 0) return false;
 #pragma unroll
-    for (int db = 0; db < HD / 32; ++db)
+    for (int g = 1; g < G; ++g)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) acc[db][r] += theirs[(32 * db + result_row(r, h)) * 32 + fr];
+        for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                acc[db][r] += theirs(g)[(32 * db + result_row(r, h)) * 32 + fr];
     return true;
 }
 
 // ---------------------------------------------------------------- forward
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2)
+__global__ void __launch_bounds__(kForward.threads(), HD == 64 ? 4 : 2)
 packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float16* __restrict__ q,
                const _Float16* __restrict__ k, const _Float16* __restrict__ v,
                const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
                float c, bool negative) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kGroups * 2 * kTile];   // [buf][group][K, V]
-    __shared__ float2 sums[4][32];
+    constexpr int W = kForward.rows, G = kForward.turns, kParts = kForward.parts();
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][K, V]
+    __shared__ float2 sums[G][W][32];
     Work w;
-    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    if (!work_of(plan, int(blockIdx.x) / kParts, heads, tokens, &w)) return;
+    const int row0 = w.block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
+    if (row0 >= w.length) return;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
     const _Float16* qb = q + size_t(w.begin) * st.q + size_t(w.head) * HD;
     const _Float16* kb = k + size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
     const _Float16* vb = v + size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
-    const int q0 = w.block * kPackedBlock + wave * 32;
+    const int q0 = row0 + wave * 32;
     const int qi = q0 + fr;
 
     f16x8 qf[KK];
@@ -195,24 +217,24 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
     float m = kFloor, l = 0.0f;
     bool started = false;
     f32x16 acc[DB] = {};
-    const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
-    const int tiles = q_last / 64 + 1, steps = (tiles + kGroups - 1) / kGroups;
+    const int q_last = min(row0 + 32 * W, length) - 1;
+    const int tiles = q_last / 64 + 1, steps = (tiles + G - 1) / G;
     auto load = [&](int i) {
-        const int j = kGroups * i + part;
+        const int j = G * i + turn;
         if (j >= tiles) return;
-        _Float16* t = lds + ((i & 1) * kGroups + part) * 2 * kTile;
+        _Float16* t = lds + ((i & 1) * G + turn) * 2 * kTile;
         const size_t at = size_t(64 * j) * st.kv;
-        load_tile<HD, 4>(t, kb + at, length - 64 * j, st.kv, wave, lane);
-        load_tile<HD, 4>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, W>(t, kb + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, W>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
     };
     load(0);
     for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
-        const _Float16* kt = lds + ((i & 1) * kGroups + part) * 2 * kTile;
+        const _Float16* kt = lds + ((i & 1) * G + turn) * 2 * kTile;
         const _Float16* vt = kt + kTile;
         if (i + 1 < steps) load(i + 1);
-        const int kbase = 64 * (kGroups * i + part);
+        const int kbase = 64 * (G * i + turn);
         if (kbase > q0 + 31) continue;          // every key after every query of the wave
         // Scores are scaled by c inside the exponent's FMA; where the tile holds
         // keys after a query (a uniform branch), before it, and masked.
@@ -255,21 +277,23 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         }
     }
     l += xor32(l);
-    if constexpr (kGroups > 1) {
-        // The groups' sums join in LDS: the second leaves its O^T [HD][32] a wave.
-        __syncthreads();
-        float* theirs = reinterpret_cast<float*>(lds) + wave * HD * 32;
-        if (part != 0) {
+    // The turns' sums join in LDS: each but the first leaves its O^T [HD][32] a
+    // wave.
+    __syncthreads();
+    auto theirs = [&](int g) { return reinterpret_cast<float*>(lds) + ((g - 1) * W + wave) * HD * 32; };
+    if (turn != 0) {
 #pragma unroll
-            for (int db = 0; db < DB; ++db)
+        for (int db = 0; db < DB; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    theirs[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
-            if (h == 0) sums[wave][fr] = float2{m, l};
-        }
-        __syncthreads();
-        if (part != 0) return;
-        const float2 other = sums[wave][fr];
+            for (int r = 0; r < 16; ++r)
+                theirs(turn)[(32 * db + result_row(r, h)) * 32 + fr] = acc[db][r];
+        if (h == 0) sums[turn][wave][fr] = float2{m, l};
+    }
+    __syncthreads();
+    if (turn != 0) return;
+#pragma unroll
+    for (int g = 1; g < G; ++g) {
+        const float2 other = sums[g][wave][fr];
         const float most = fmaxf(m, other.x);
         const float by = __builtin_amdgcn_exp2f(m - most);
         const float other_by = __builtin_amdgcn_exp2f(other.x - most);
@@ -279,8 +303,8 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         for (int db = 0; db < DB; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                acc[db][r] = __builtin_fmaf(theirs[(32 * db + result_row(r, h)) * 32 + fr], other_by,
-                                            acc[db][r] * by);
+                acc[db][r] = __builtin_fmaf(theirs(g)[(32 * db + result_row(r, h)) * 32 + fr],
+                                            other_by, acc[db][r] * by);
     }
     if (qi < length) {
         store_row<HD>(out + size_t(w.begin + qi) * st.o + size_t(w.head) * HD, acc, 1.0f / l, h);
@@ -292,7 +316,7 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
 // ---------------------------------------------------------------- backward: dQ (and D)
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads * kGroups, 2)
+__global__ void __launch_bounds__(kQuery.threads(), 2)
 packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                    const _Float16* __restrict__ v, const _Float16* __restrict__ o,
@@ -300,19 +324,22 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
                    float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * kGroups * 2 * kTile];   // [buf][group][K, V]
+    constexpr int W = kQuery.rows, G = kQuery.turns, kParts = kQuery.parts();
+    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][K, V]
     Work w;
-    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    if (!work_of(plan, int(blockIdx.x) / kParts, heads, tokens, &w)) return;
+    const int row0 = w.block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
+    if (row0 >= w.length) return;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-    const int part = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
     const size_t o_at = size_t(w.begin) * st.o + size_t(w.head) * HD;
     const size_t kv_at = size_t(w.begin) * st.kv + size_t(w.head / group) * HD;
     const size_t q_at = size_t(w.begin) * st.q + size_t(w.head) * HD;
-    const int q0 = w.block * kPackedBlock + wave * 32;
+    const int q0 = row0 + wave * 32;
     const int qi = q0 + fr;
 
     f16x8 qf[KK], df[KK];
@@ -331,27 +358,27 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
     dd += xor32(dd);
     const size_t row_at = size_t(w.head) * tokens + w.begin + qi;
     const float lse2 = qi < length ? lse[row_at] * kLog2e : 0.0f;
-    if (qi < length && h == 0 && part == 0) dsum[row_at] = dd;
+    if (qi < length && h == 0 && turn == 0) dsum[row_at] = dd;
 
     f32x16 acc[DB] = {};   // dQ^T[d][q]
-    const int q_last = min(w.block * kPackedBlock + kPackedBlock, length) - 1;
-    const int tiles = q_last / 64 + 1, steps = (tiles + kGroups - 1) / kGroups;
+    const int q_last = min(row0 + 32 * W, length) - 1;
+    const int tiles = q_last / 64 + 1, steps = (tiles + G - 1) / G;
     auto load = [&](int i) {
-        const int j = kGroups * i + part;
+        const int j = G * i + turn;
         if (j >= tiles) return;
-        _Float16* t = lds + ((i & 1) * kGroups + part) * 2 * kTile;
+        _Float16* t = lds + ((i & 1) * G + turn) * 2 * kTile;
         const size_t at = kv_at + size_t(64 * j) * st.kv;
-        load_tile<HD, 4>(t, k + at, length - 64 * j, st.kv, wave, lane);
-        load_tile<HD, 4>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, W>(t, k + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, W>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
     };
     load(0);
     for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
-        const _Float16* kt = lds + ((i & 1) * kGroups + part) * 2 * kTile;
+        const _Float16* kt = lds + ((i & 1) * G + turn) * 2 * kTile;
         const _Float16* vt = kt + kTile;
         if (i + 1 < steps) load(i + 1);
-        const int kbase = 64 * (kGroups * i + part);
+        const int kbase = 64 * (G * i + turn);
         if (kbase > q0 + 31) continue;
         const bool masked = kbase + 63 > q0;
         // Two halves of 32 keys, each through all of its products before the
@@ -388,7 +415,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
             }
         }
     }
-    if (!join_groups<HD, kGroups>(reinterpret_cast<float*>(lds), acc, wave, part, lane)) return;
+    if (!join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane)) return;
     if (qi < length) store_row<HD>(dq + q_at + size_t(qi) * st.q, acc, scale, h);
 }
 
@@ -402,7 +429,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
 // sums ([part][token][kv head][HD], dK then dV) for packed_backward_join: heads
 // of k and v are few where groups are large, and so are workgroups then.
 template <int HD>
-__global__ void __launch_bounds__(kThreads * kKeyGroups<HD>, HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(kKey<HD>.threads(), HD == 64 ? 2 : 1)
 packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                      const _Float16* __restrict__ v, const _Float16* __restrict__ dout,
@@ -410,32 +437,34 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const int4* __restrict__ plan, float* __restrict__ sums, int tokens,
                      int kv_heads, int group, int share, Strides st, float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    constexpr int G = kKeyGroups<HD>;
+    constexpr int W = kKey<HD>.rows, G = kKey<HD>.turns, kParts = kKey<HD>.parts();
     __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][Q, dO]
     __shared__ __attribute__((aligned(16))) float rowstat[2][G][2][64];        // [buf][group][lse, D]
     Work w;
     const int parts = group / share;
-    if (!work_of(plan, int(blockIdx.x), kv_heads * parts, tokens, &w)) return;
+    if (!work_of(plan, int(blockIdx.x) / kParts, kv_heads * parts, tokens, &w)) return;
     const int part = w.head % parts;
     w.head /= parts;
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
-    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
+    const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
     const int fr = lane & 31, h = lane >> 5;
     const Frags<HD> fo(lane);
     const int length = w.length;
     // The list's long blocks are the last of their sequences; as keys the first
     // ones have the most queries.
     const int block = (length + kPackedBlock - 1) / kPackedBlock - 1 - w.block;
+    const int row0 = block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
+    if (row0 >= length) return;
     const size_t kv_at = size_t(w.begin) * st.kv + size_t(w.head) * HD;
-    const int k0 = block * kPackedBlock + wave * 32;
+    const int k0 = row0 + wave * 32;
     const int ki = k0 + fr;
 
     f16x8 kf[KK], vf[KK];
     load_frags<HD>(kf, k + kv_at, ki, length, st.kv, h);
     load_frags<HD>(vf, v + kv_at, ki, length, st.kv, h);
     f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
-    const int first = block * kPackedBlock / 64;
+    const int first = row0 / 64;
     const int per_head = (length + 63) / 64 - first;
     const int tiles = per_head * share, steps = (tiles + G - 1) / G;
     auto stage = [&](int i) {
@@ -453,8 +482,8 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             dv0 = dsum[at];
         }
         const size_t row = size_t(w.begin) + 64 * tile;
-        load_tile<HD, 4>(t, q + row * st.q + size_t(head) * HD, length - 64 * tile, st.q, wave, lane);
-        load_tile<HD, 4>(t + kTile, dout + row * st.o + size_t(head) * HD, length - 64 * tile, st.o,
+        load_tile<HD, W>(t, q + row * st.q + size_t(head) * HD, length - 64 * tile, st.q, wave, lane);
+        load_tile<HD, W>(t + kTile, dout + row * st.o + size_t(head) * HD, length - 64 * tile, st.o,
                          wave, lane);
         if (wave == 0) {
             (&rowstat[0][0])[buf][0][lane] = lv * kLog2e;
@@ -525,8 +554,8 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             }
         }
     }
-    join_groups<HD, G>(reinterpret_cast<float*>(lds), dka, wave, turn, lane);
-    if (!join_groups<HD, G>(reinterpret_cast<float*>(lds), dva, wave, turn, lane) || ki >= length)
+    join_turns<HD, W, G>(reinterpret_cast<float*>(lds), dka, wave, turn, lane);
+    if (!join_turns<HD, W, G>(reinterpret_cast<float*>(lds), dva, wave, turn, lane) || ki >= length)
         return;
     if (parts == 1) {
         const size_t at = kv_at + size_t(ki) * st.kv;
@@ -603,8 +632,9 @@ template <int HD>
 hipError_t forward(void* o, void* lse, const void* q, const void* k, const void* v,
                    const void* plan, const flint_packed_shape& s, float scale,
                    hipStream_t stream) {
-    hipLaunchKernelGGL(packed_forward<HD>, dim3(unsigned(packed_items(s) * s.heads)), dim3(kThreads * kGroups),
-                       0, stream, static_cast<_Float16*>(o), static_cast<float*>(lse),
+    hipLaunchKernelGGL(packed_forward<HD>,
+                       dim3(unsigned(packed_items(s) * s.heads * kForward.parts())),
+                       dim3(kForward.threads()), 0, stream, static_cast<_Float16*>(o), static_cast<float*>(lse),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const int4*>(plan),
                        int(s.tokens), int(s.heads), int(s.heads / s.kv_heads),
@@ -620,8 +650,9 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     const Strides st{int(s.q_stride), int(s.kv_stride), int(s.o_stride)};
     auto* dsum = static_cast<float*>(workspace);
     const int group = int(s.heads / s.kv_heads);
-    hipLaunchKernelGGL(packed_backward_dq<HD>, dim3(unsigned(packed_items(s) * s.heads)),
-                       dim3(kThreads * kGroups), 0, stream, static_cast<_Float16*>(dq), dsum,
+    hipLaunchKernelGGL(packed_backward_dq<HD>,
+                       dim3(unsigned(packed_items(s) * s.heads * kQuery.parts())),
+                       dim3(kQuery.threads()), 0, stream, static_cast<_Float16*>(dq), dsum,
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(o),
                        static_cast<const _Float16*>(dout), static_cast<const float*>(lse),
@@ -630,8 +661,8 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const size_t parts = group_parts(s), blocks = packed_items(s) * s.kv_heads;
     float* sums = dsum + dsum_values(s);
-    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(blocks * parts)),
-                       dim3(kThreads * kKeyGroups<HD>), 0, stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
+    hipLaunchKernelGGL(packed_backward_dkdv<HD>, 
+                       dim3(unsigned(blocks * parts * kKey<HD>.parts())), dim3(kKey<HD>.threads()), 0, stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(dout),
                        static_cast<const float*>(lse), static_cast<const float*>(dsum),
