@@ -162,6 +162,28 @@ def test_chunks(flint, cuda, cached, new, heads, kv_heads, width):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 128])
+def test_many_rows_in_several_parts(flint, cuda, width):
+    """More than 4,096 rows of o whose sequences are cut into parts."""
+    check(Run(flint, cuda, Cache([900, 1300], [290, 230], 8, 2, width, 32, seed=21)).run())
+    check(Run(flint, cuda, Cache([2000], [600], 7, 1, width, 16, seed=22)).run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 9])
+def test_more_sequences_than_a_wave_has_lanes(flint, cuda, new):
+    cached = [(i * 37) % 400 for i in range(150)]
+    chunk = [(i * 5) % (new + 1) if new > 1 else 1 for i in range(150)]
+    check(Run(flint, cuda, Cache(cached, chunk, 4, 1, 64, 16, seed=23)).run())
+
+
+@pytest.mark.gpu
+def test_one_long_sequence_in_many_parts(flint, cuda):
+    check(Run(flint, cuda, Cache([60000], [1], 2, 1, 64, 64, seed=24)).run())
+    check(Run(flint, cuda, Cache([30000], [40], 1, 1, 128, 128, seed=25)).run())
+
+
+@pytest.mark.gpu
 def test_a_long_cache_and_an_empty_one(flint, cuda):
     check(Run(flint, cuda, Cache([9000, 0, 4097], [1, 1, 1], 4, 2, 64, 32, seed=4)).run())
     check(Run(flint, cuda, Cache([5000, 3], [7, 2], 4, 4, 128, 64, seed=5)).run())
