@@ -34,6 +34,22 @@ __device__ __forceinline__ void wait_lds() {
 // The value of lane ^ 32 (the other half of the wave holds the same query).
 __device__ __forceinline__ float xor32(float v) { return __shfl_xor(v, 32); }
 
+// Inclusive prefix sum over the wave by lane exchanges within the vector unit:
+// 1, 2, 4 and 8 lanes up within 16, then the last lane of a row of 16, and of
+// the first 32, to those above.
+__device__ __forceinline__ int wave_scan(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+    return v;
+}
+__device__ __forceinline__ int wave_sum(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v), 63);
+}
+
 // A tile holds rows of HD halves back to back, 16-byte chunk c of row r at
 // chunk position c ^ key(r). Two reads have to spread over the banks: the 16
 // lanes of a row fragment take one chunk of 16 consecutive rows, those of a

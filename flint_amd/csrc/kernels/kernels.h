@@ -166,7 +166,7 @@ constexpr size_t kPackedMaxTokens = size_t{1} << 26;
 constexpr size_t kPackedMaxSequences = size_t{1} << 20;
 constexpr size_t kHeadsMax = 1024;
 constexpr size_t kStrideMax = size_t{1} << 23;
-constexpr size_t kPackedMaxBlocks = size_t{1} << 23;   // workgroups: below 2^32 threads
+constexpr size_t kPackedMaxBlocks = size_t{1} << 22;   // workgroups of 512: below 2^32 threads
 constexpr int kPackedBlock = 128;
 struct PackedItem {
     int begin, end;   // the sequence's rows

@@ -295,30 +295,52 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
     }
 }
 
+// A streaming pass (log p of a word of probability 0 is -1e4: no 0 x inf, however
+// large dH is): kAhead chunks of a thread are read before the first of
+// them is written (dlogits may be logits, so the compiler keeps that order).
 __global__ void __launch_bounds__(kThreads)
-logprobs_backward(h8* __restrict__ dlogits, const float* __restrict__ dlogprob,
-                  const float* __restrict__ dentropy, const h8* __restrict__ logits,
+logprobs_backward(h8* dlogits, const float* __restrict__ dlogprob,
+                  const float* __restrict__ dentropy, const h8* logits,
                   const uint16_t* __restrict__ targets, const float* __restrict__ entropy,
                   const float* __restrict__ stats, float scale, int vocab, int chunks) {
+    constexpr int kAhead = 5;
     const size_t row = blockIdx.x;
     const int t = targets[row];
     const float mx = stats[2 * row], log_sum = stats[2 * row + 1];
     const float dlp = t < vocab ? dlogprob[row] : 0.0f;
     const float dh = dentropy != nullptr ? dentropy[row] : 0.0f;
     const float ent = dentropy != nullptr ? entropy[row] : 0.0f;
-    for (int c = threadIdx.x; c < chunks; c += kThreads) {
-        const h8 l = logits[row * chunks + c];
-        h8 d;
+    const h8* from = logits + row * chunks;
+    h8* to = dlogits + row * chunks;
+    for (int c0 = threadIdx.x; c0 < chunks; c0 += kThreads * kAhead) {
+        h8 l[kAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int j = 8 * c + i;
-            const float lp = scale * (float(l[i]) - mx) - log_sum;
-            const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
-            float g = -p * (dlp + dh * (fmaxf(lp, -3e38f) + ent));
-            if (j == t) g += dlp;
-            d[i] = j < vocab ? _Float16(scale * g) : _Float16(0.0f);
+        for (int k = 0; k < kAhead; ++k)
+            if (c0 + k * kThreads < chunks) l[k] = from[c0 + k * kThreads];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int c = c0 + k * kThreads;
+            if (c >= chunks) break;
+            float d[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float lp = __builtin_fmaf(scale, float(l[k][i]) - mx, -log_sum);
+                const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+                d[i] = -scale * p * __builtin_fmaf(dh, fmaxf(lp, -1e4f) + ent, dlp);
+            }
+            if (c == t >> 3 || c == (vocab - 1) >> 3 || c > (vocab - 1) >> 3) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int j = 8 * c + i;
+                    if (j == t) d[i] += scale * dlp;
+                    if (j >= vocab) d[i] = 0.0f;
+                }
+            }
+            h8 out;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) out[i] = _Float16(d[i]);
+            store_stream(to + c, out);
         }
-        dlogits[row * chunks + c] = d;
     }
 }
 

@@ -80,28 +80,6 @@ __device__ __forceinline__ int column_of(const PagedArgs& a, int p) {
     return int(a.magic == 0 ? n : __umulhi(n, a.magic) >> a.shift);
 }
 
-// Inclusive prefix sum over the wave by lane exchanges within the vector unit:
-// 1, 2, 4 and 8 lanes up within 16, then the last lane of a row of 16, and of
-// the first 32, to those above.
-__device__ __forceinline__ int wave_scan(int v) {
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
-    return v;
-}
-__device__ __forceinline__ int wave_sum(int v) {
-    return __builtin_amdgcn_readlane(wave_scan(v), 63);
-}
-
-__device__ __forceinline__ int wave_max(int v) {
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) v = max(v, __shfl_xor(v, d));
-    return v;
-}
-
 // Item `idx` of a kv head. Every item takes about the same number of tiles,
 // total / target: the sequences' lengths are known only here, so each wave adds
 // them up (64 sequences a step) and finds its item by a prefix sum.
@@ -126,7 +104,8 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     // In two words: the rows' blocks add up to at most 2^21, tiles are at most
     // 2^26.
     total = ((long long)(wave_sum(int(total >> 20))) << 20) + wave_sum(int(total & 0xfffff));
-    int each = max(P::kLeast, int((total + a.target - 1) / a.target));
+    constexpr long long kMost = 1 << 30;   // more tiles than any sequence has
+    int each = max(P::kLeast, int(min(kMost, (total + a.target - 1) / a.target)));
     // Few rows: a workgroup on each CU first (a quarter of the target), then
     // parts of 16 tiles, and only then more of them.
     if constexpr (!MANY) each = max(each, int(min(16ll, (4 * total + a.target - 1) / a.target)));
@@ -136,7 +115,7 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     if constexpr (MANY)
         for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
             const int parts = (tiles_of(q) + each - 1) / each;
-            if (wave_sum(blocks_of(q) * parts) <= a.target || wave_max(parts) <= 1) break;
+            if (wave_sum(blocks_of(q) * parts) <= a.target || __ballot(parts > 1) == 0) break;
             each += (each + 7) / 8;
         }
     int before = 0, slots = 0;

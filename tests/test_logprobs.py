@@ -178,6 +178,7 @@ def test_ties_and_masks(flint, cuda, kind, vocab):
         r.logits[:, 10:] = -65504.0
     elif kind == "masked":
         r.logits[:, 10:] = float("-inf")
+        r.dh[:] = torch.tensor([3.0, -40.0, 1e4, 0.0])
         r.targets[0] = 20          # a target of probability 0
     elif kind == "ramp":
         r.logits[:] = (column.float() / r.cols * 10).half()
