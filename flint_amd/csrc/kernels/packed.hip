@@ -121,8 +121,11 @@ packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequen
 // go longest first, heads side by side: workgroup id runs on XCD id % 8, so with
 // 8 heads an XCD's L2 holds one head's rows. (Every other run of 256 workgroups
 // backwards, to put short blocks beside long ones, breaks that: 8 heads of 128
-// over 8,192 tokens 158 -> 197 us, and the ragged batch gained nothing.) A plan
-// of other sequences gives wrong rows, but none outside the tokens.
+// over 8,192 tokens 158 -> 197 us, and the ragged batch gained nothing. Nor did
+// cutting the longest blocks into parts of their tiles, joined by another
+// launch: blocks that start together read the same tiles of K and V at the same
+// time, out of L2, which parts do not; 8 heads of 128 over 8,192 tokens 165 ->
+// 191.) A plan of other sequences gives wrong rows, but none outside the tokens.
 struct Work {
     int begin, length, block, head;
 };

@@ -152,6 +152,19 @@ def test_many_short_sequences(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lengths", [[1] * 200, [3, 1] * 60 + [65], [900, 1, 2, 30]])
+def test_large_groups_of_heads(flint, cuda, lengths):
+    """The heads of a group go into parts for dK and dV, and join."""
+    check(Run(flint, cuda, Batch(lengths, 32, 1, 64, seed=28)).run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,width", [(1, 1, 64), (2, 1, 128), (3, 3, 64)])
+def test_one_sequence_much_longer(flint, cuda, heads, kv_heads, width):
+    check(Run(flint, cuda, Batch([5, 2300, 64, 130], heads, kv_heads, width, seed=29)).run())
+
+
+@pytest.mark.gpu
 def test_a_sequence_keeps_its_non_finite_values(flint, cuda):
     b = Batch([100, 90, 130], 2, 2, 64, seed=12)
     clean = Run(flint, cuda, b).run().outputs()
