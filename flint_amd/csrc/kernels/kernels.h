@@ -160,8 +160,8 @@ hipError_t launch_attention_backward(void* dq, void* dk, void* dv, const void* d
                                      void* dsum, size_t batches, size_t length, float scale,
                                      hipStream_t stream, AttnLayout layout = {});
 // Causal attention over packed sequences (packed.hip): blocks of kPackedBlock
-// queries of one sequence, listed longest first by the plan (PackedItem, at
-// most packed_items of them, behind one 16-byte header holding their count).
+// queries of one sequence, listed longest first by the plan (packed_items
+// entries; those past the last block are empty).
 constexpr size_t kPackedMaxTokens = size_t{1} << 26;
 constexpr size_t kPackedMaxSequences = size_t{1} << 20;
 constexpr size_t kHeadsMax = 1024;
@@ -177,7 +177,7 @@ inline size_t packed_items(const flint_packed_shape& s) {
     return s.tokens / kPackedBlock + s.sequences;
 }
 inline size_t packed_plan_bytes(const flint_packed_shape& s) {
-    return (packed_items(s) + 1) * sizeof(PackedItem);
+    return packed_items(s) * sizeof(PackedItem);
 }
 size_t packed_backward_workspace(const flint_packed_shape& s);
 hipError_t launch_packed_plan(void* plan, const void* offsets, const flint_packed_shape& s,

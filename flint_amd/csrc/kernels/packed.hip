@@ -60,7 +60,7 @@ constexpr int kBuckets = 1024;
 __global__ void __launch_bounds__(kPlanThreads)
 packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequences, int tokens,
             int capacity, int shift) {
-    __shared__ int full[kBuckets], part[kBuckets], next[kBuckets];
+    __shared__ int full[kBuckets], part[kBuckets], next[kBuckets], filled;
     const int tid = threadIdx.x;
     full[tid] = part[tid] = 0;
     __syncthreads();
@@ -95,8 +95,10 @@ packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequen
     const int items = part[bucket] + (before(full[bucket]) << shift);
     const int first = before(items);
     next[bucket] = first;
-    if (bucket == 0) plan[0] = int4{min(first + items, capacity), 0, 0, 0};
+    // Entries past the last block are empty: a workgroup reads its own alone.
+    if (bucket == 0) filled = first + items;
     __syncthreads();
+    for (int i = filled + tid; i < capacity; i += kPlanThreads) plan[i] = int4{0, 0, 0, 0};
     // A sequence of many blocks is written by its whole wave.
     for (int base = 0; base < sequences; base += kPlanThreads) {
         const int s = base + tid;
@@ -105,7 +107,7 @@ packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequen
         const int n = (end - begin + kPackedBlock - 1) / kPackedBlock;
         auto put = [&](int b0, int e0, int block) {
             const int at = atomicAdd(&next[min(block >> shift, kBuckets - 1)], 1);
-            if (at < capacity) plan[1 + at] = int4{b0, e0, block, 0};
+            if (at < capacity) plan[at] = int4{b0, e0, block, 0};
         };
         if (n <= 16)
             for (int b = 0; b < n; ++b) put(begin, end, b);
@@ -132,8 +134,7 @@ struct Work {
 __device__ __forceinline__ bool work_of(const int4* plan, int id, int heads, int tokens,
                                         Work* w) {
     const int item = id / heads;
-    if (item >= plan[0].x) return false;
-    const int4 it = plan[1 + item];
+    const int4 it = plan[item];
     w->begin = min(max(it.x, 0), tokens);
     w->length = min(max(it.y, w->begin), tokens) - w->begin;
     w->block = it.z;
@@ -211,11 +212,6 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
     const int q0 = row0 + wave * 32;
     const int qi = q0 + fr;
 
-    f16x8 qf[KK];
-    load_frags<HD>(qf, qb, qi, length, st.q, h);
-    if (negative)   // c is positive: the scale's sign goes into q
-#pragma unroll
-        for (int kk = 0; kk < KK; ++kk) qf[kk] = -qf[kk];
     float m = kFloor, l = 0.0f;
     bool started = false;
     f32x16 acc[DB] = {};
@@ -230,6 +226,11 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         load_tile<HD, W>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
     };
     load(0);
+    f16x8 qf[KK];
+    load_frags<HD>(qf, qb, qi, length, st.q, h);
+    if (negative)   // c is positive: the scale's sign goes into q
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) qf[kk] = -qf[kk];
     for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
