@@ -142,8 +142,28 @@ __device__ __forceinline__ bool work_of(const int4* plan, int id, int heads, int
     return it.z >= 0 && it.z <= (w->length - 1) / kPackedBlock && w->length > 0;
 }
 
-// Fragments of rows `row0 + l % 32` of a head's matrix (zeros from `left` on):
-// 16-byte chunks 2 kk + l / 32.
+// A block's 128 rows of one head into two tiles, shared out over WAVES waves.
+// Read by the lanes straight into their fragments, 16 bytes of 32 rows at a time
+// and by both turns, they come slower: over 8 x 1,024 tokens of 8 heads of 128
+// the forward pass takes 34.9 us so and 33.3 through LDS, dQ 47.8 and 43.0.
+template <int HD, int WAVES>
+__device__ __forceinline__ void load_block(_Float16* tiles, const _Float16* from, int left,
+                                           int stride, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        load_tile<HD, WAVES>(tiles + i * Tile<HD>::kHalves, from + size_t(64 * i) * stride,
+                             left - 64 * i, stride, wave, lane);
+}
+// The fragments of wave `wave`'s 32 of them.
+template <int HD>
+__device__ __forceinline__ void block_frags(f16x8 (&f)[HD / 16], const _Float16* tiles,
+                                            const Frags<HD>& fo, int wave) {
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+        f[kk] = fo.row(tiles + (wave >> 1) * Tile<HD>::kHalves, wave & 1, kk);
+}
+
+// Fragments of row `row` of a head's matrix from memory (zeros from `left` on).
 template <int HD>
 __device__ __forceinline__ void load_frags(f16x8 (&f)[HD / 16], const _Float16* base, int row,
                                            int left, int stride, int h) {
@@ -161,10 +181,10 @@ struct Strides {
 // in the others.
 template <int HD, int W, int G>
 __device__ __forceinline__ bool join_turns(float* lds, f32x16* acc, int wave, int turn, int lane) {
+    __syncthreads();
     if constexpr (G == 1) return true;
     const int fr = lane & 31, h = lane >> 5;
     auto theirs = [&](int g) { return lds + ((g - 1) * W + wave) * HD * 32; };
-    __syncthreads();
     if (turn != 0) {
 #pragma unroll
         for (int db = 0; db < HD / 32; ++db)
@@ -225,9 +245,15 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         load_tile<HD, W>(t, kb + at, length - 64 * j, st.kv, wave, lane);
         load_tile<HD, W>(t + kTile, vb + at, length - 64 * j, st.kv, wave, lane);
     };
+    // The queries go through the buffers of the second step.
+    _Float16* block = lds + 2 * G * kTile;
+    load_block<HD, W * G>(block, qb + size_t(row0) * st.q, length - row0, st.q,
+                          wave + W * turn, lane);
     load(0);
+    wait_vmcnt<0>();
+    block_sync();
     f16x8 qf[KK];
-    load_frags<HD>(qf, qb, qi, length, st.q, h);
+    block_frags<HD>(qf, block, fo, wave);
     if (negative)   // c is positive: the scale's sign goes into q
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk) qf[kk] = -qf[kk];
@@ -293,27 +319,31 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         if (h == 0) sums[turn][wave][fr] = float2{m, l};
     }
     __syncthreads();
-    if (turn != 0) return;
+    _Float16* rows = lds + (G - 1) * W * HD * 32 * 2;   // behind theirs
+    if (turn == 0) {
 #pragma unroll
-    for (int g = 1; g < G; ++g) {
-        const float2 other = sums[g][wave][fr];
-        const float most = fmaxf(m, other.x);
-        const float by = __builtin_amdgcn_exp2f(m - most);
-        const float other_by = __builtin_amdgcn_exp2f(other.x - most);
-        m = most;
-        l = __builtin_fmaf(other.y, other_by, l * by);
+        for (int g = 1; g < G; ++g) {
+            const float2 other = sums[g][wave][fr];
+            const float most = fmaxf(m, other.x);
+            const float by = __builtin_amdgcn_exp2f(m - most);
+            const float other_by = __builtin_amdgcn_exp2f(other.x - most);
+            m = most;
+            l = __builtin_fmaf(other.y, other_by, l * by);
 #pragma unroll
-        for (int db = 0; db < DB; ++db)
+            for (int db = 0; db < DB; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                acc[db][r] = __builtin_fmaf(theirs(g)[(32 * db + result_row(r, h)) * 32 + fr],
-                                            other_by, acc[db][r] * by);
-    }
-    if (qi < length) {
-        store_row<HD>(out + size_t(w.begin + qi) * st.o + size_t(w.head) * HD, acc, 1.0f / l, h);
-        if (h == 0)
+                for (int r = 0; r < 16; ++r)
+                    acc[db][r] = __builtin_fmaf(theirs(g)[(32 * db + result_row(r, h)) * 32 + fr],
+                                                other_by, acc[db][r] * by);
+        }
+        write_rows<HD>(rows, acc, 1.0f / l, wave * 32 + fr, h);
+        if (qi < length && h == 0)
             lse[size_t(w.head) * tokens + w.begin + qi] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
+    __syncthreads();
+    copy_rows<HD, kForward.threads()>(rows, length - row0, [&](int row) {
+        return out + size_t(w.begin + row0 + row) * st.o + size_t(w.head) * HD;
+    });
 }
 
 // ---------------------------------------------------------------- backward: dQ (and D)
@@ -345,13 +375,32 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
     const int q0 = row0 + wave * 32;
     const int qi = q0 + fr;
 
+    const int q_last = min(row0 + 32 * W, length) - 1;
+    const int tiles = q_last / 64 + 1, steps = (tiles + G - 1) / G;
+    auto load = [&](int i) {
+        const int j = G * i + turn;
+        if (j >= tiles) return;
+        _Float16* t = lds + ((i & 1) * G + turn) * 2 * kTile;
+        const size_t at = kv_at + size_t(64 * j) * st.kv;
+        load_tile<HD, W>(t, k + at, length - 64 * j, st.kv, wave, lane);
+        load_tile<HD, W>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
+    };
+    // Q and dO go through the buffers of the second step.
+    _Float16* block = lds + 2 * G * kTile;
+    load_block<HD, W * G>(block, q + q_at + size_t(row0) * st.q, length - row0, st.q,
+                          wave + W * turn, lane);
+    load_block<HD, W * G>(block + 2 * kTile, dout + o_at + size_t(row0) * st.o, length - row0,
+                          st.o, wave + W * turn, lane);
+    load(0);
+    f16x8 of[KK];
+    load_frags<HD>(of, o + o_at, qi, length, st.o, h);
+    wait_vmcnt<0>();
+    block_sync();
     f16x8 qf[KK], df[KK];
-    load_frags<HD>(qf, q + q_at, qi, length, st.q, h);
-    load_frags<HD>(df, dout + o_at, qi, length, st.o, h);
+    block_frags<HD>(qf, block, fo, wave);
+    block_frags<HD>(df, block + 2 * kTile, fo, wave);
     float dd = 0.0f;
     {
-        f16x8 of[KK];
-        load_frags<HD>(of, o + o_at, qi, length, st.o, h);
 #pragma unroll
         for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
@@ -364,17 +413,6 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
     if (qi < length && h == 0 && turn == 0) dsum[row_at] = dd;
 
     f32x16 acc[DB] = {};   // dQ^T[d][q]
-    const int q_last = min(row0 + 32 * W, length) - 1;
-    const int tiles = q_last / 64 + 1, steps = (tiles + G - 1) / G;
-    auto load = [&](int i) {
-        const int j = G * i + turn;
-        if (j >= tiles) return;
-        _Float16* t = lds + ((i & 1) * G + turn) * 2 * kTile;
-        const size_t at = kv_at + size_t(64 * j) * st.kv;
-        load_tile<HD, W>(t, k + at, length - 64 * j, st.kv, wave, lane);
-        load_tile<HD, W>(t + kTile, v + at, length - 64 * j, st.kv, wave, lane);
-    };
-    load(0);
     for (int i = 0; i < steps; ++i) {
         wait_vmcnt<0>();
         block_sync();
@@ -418,8 +456,13 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
             }
         }
     }
-    if (!join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane)) return;
-    if (qi < length) store_row<HD>(dq + q_at + size_t(qi) * st.q, acc, scale, h);
+    _Float16* rows = lds + (G - 1) * W * HD * 32 * 2;   // behind the turns' sums
+    if (join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane))
+        write_rows<HD>(rows, acc, scale, wave * 32 + fr, h);
+    __syncthreads();
+    copy_rows<HD, kQuery.threads()>(rows, length - row0, [&](int row) {
+        return dq + q_at + size_t(row0 + row) * st.q;
+    });
 }
 
 // ---------------------------------------------------------------- backward: dK, dV
@@ -463,9 +506,6 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
     const int k0 = row0 + wave * 32;
     const int ki = k0 + fr;
 
-    f16x8 kf[KK], vf[KK];
-    load_frags<HD>(kf, k + kv_at, ki, length, st.kv, h);
-    load_frags<HD>(vf, v + kv_at, ki, length, st.kv, h);
     f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
     const int first = row0 / 64;
     const int per_head = (length + 63) / 64 - first;
@@ -493,7 +533,24 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             (&rowstat[0][0])[buf][1][lane] = dv0;
         }
     };
-    stage(0);
+    // K and V go through the buffers: the second step's, and the first's for
+    // want of room with one turn.
+    _Float16* keys = lds + 2 * G * kTile;
+    _Float16* values = G == 1 ? lds : keys + 2 * kTile;
+    load_block<HD, W * G>(keys, k + kv_at + size_t(row0) * st.kv, length - row0, st.kv,
+                          wave + W * turn, lane);
+    load_block<HD, W * G>(values, v + kv_at + size_t(row0) * st.kv, length - row0, st.kv,
+                          wave + W * turn, lane);
+    if constexpr (G > 1) stage(0);
+    wait_vmcnt<0>();
+    block_sync();
+    f16x8 kf[KK], vf[KK];
+    block_frags<HD>(kf, keys, fo, wave);
+    block_frags<HD>(vf, values, fo, wave);
+    if constexpr (G == 1) {
+        block_sync();
+        stage(0);
+    }
     int tile = first + turn % per_head;
     for (int i = 0; i < steps; ++i) {
         const int buf = (i & 1) * G + turn;
@@ -557,15 +614,21 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
             }
         }
     }
-    join_turns<HD, W, G>(reinterpret_cast<float*>(lds), dka, wave, turn, lane);
-    if (!join_turns<HD, W, G>(reinterpret_cast<float*>(lds), dva, wave, turn, lane) || ki >= length)
-        return;
-    if (parts == 1) {
-        const size_t at = kv_at + size_t(ki) * st.kv;
-        store_row<HD>(dk + at, dka, scale, h);
-        store_row<HD>(dv + at, dva, 1.0f, h);
-        return;
+    const size_t at = kv_at + size_t(row0) * st.kv;
+    _Float16* rows = lds + (G - 1) * W * HD * 32 * 2;   // behind the turns' sums
+    bool mine = false;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        f32x16* acc = which == 0 ? dka : dva;
+        mine = join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane);
+        if (parts > 1) continue;
+        if (mine) write_rows<HD>(rows, acc, which == 0 ? scale : 1.0f, wave * 32 + fr, h);
+        __syncthreads();
+        copy_rows<HD, kKey<HD>.threads()>(rows, length - row0, [&](int row) {
+            return (which == 0 ? dk : dv) + at + size_t(row) * st.kv;
+        });
     }
+    if (parts == 1 || !mine || ki >= length) return;
     float* to = sums + ((size_t(part) * tokens + w.begin + ki) * kv_heads + w.head) * HD;
     const size_t dv_at = size_t(parts) * tokens * kv_heads * HD;
 #pragma unroll

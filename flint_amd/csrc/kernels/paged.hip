@@ -510,29 +510,36 @@ __global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2) paged_ma
         if (h == 0) sums[wave][fr] = float2{w.m, w.l};
     }
     __syncthreads();
-    const int row = first_row + fr;
-    if (turn != 0 || row >= rows) return;
-    const float2 other = sums[wave][fr];
-    const float most = fmaxf(w.m, other.x);
-    const float by = __builtin_amdgcn_exp2f(w.m - most);
-    const float other_by = __builtin_amdgcn_exp2f(other.x - most);
-    w.l = __builtin_fmaf(other.y, other_by, w.l * by);
+    if (turn == 0) {
+        const float2 other = sums[wave][fr];
+        const float most = fmaxf(w.m, other.x);
+        const float by = __builtin_amdgcn_exp2f(w.m - most);
+        const float other_by = __builtin_amdgcn_exp2f(other.x - most);
+        w.m = most;
+        w.l = __builtin_fmaf(other.y, other_by, w.l * by);
 #pragma unroll
-    for (int db = 0; db < HD / 32; ++db)
+        for (int db = 0; db < HD / 32; ++db)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            w.acc[db][r] = __builtin_fmaf(theirs[(32 * db + result_row(r, h)) * 32 + fr], other_by,
-                                          w.acc[db][r] * by);
+            for (int r = 0; r < 16; ++r)
+                w.acc[db][r] = __builtin_fmaf(theirs[(32 * db + result_row(r, h)) * 32 + fr],
+                                              other_by, w.acc[db][r] * by);
+    }
     if (it.parts == 1) {
-        const int place = row / a.group;
-        store_row<HD>(a.o + size_t(it.seq.first + place) * a.o_stride +
-                          size_t(head * a.group + row - place * a.group) * HD,
-                      w.acc, 1.0f / w.l, h);
+        _Float16* block = lds + 4 * HD * 32 * 2;   // behind theirs
+        if (turn == 0) write_rows<HD>(block, w.acc, 1.0f / w.l, wave * 32 + fr, h);
+        __syncthreads();
+        const int row0 = it.block * kManyRows;
+        copy_rows<HD, kThreads * kGroups>(block, rows - row0, [&](int i) {
+            const int place = (row0 + i) / a.group;
+            return a.o + size_t(it.seq.first + place) * a.o_stride +
+                   size_t(head * a.group + row0 + i - place * a.group) * HD;
+        });
         return;
     }
+    if (turn != 0 || first_row + fr >= rows) return;
     const size_t slot =
         (size_t(it.slot + it.part) * a.kv_heads + head) * kManyRows + wave * 32 + fr;
-    if (h == 0) a.sums[slot] = float2{most, w.l};
+    if (h == 0) a.sums[slot] = float2{w.m, w.l};
 #pragma unroll
     for (int db = 0; db < HD / 32; ++db)
 #pragma unroll
