@@ -497,6 +497,88 @@ def run(f, torch, dev, path, only=None):
         del ts, ws
         torch.cuda.empty_cache()
 
+    def section_packed():
+        # Attention over packed sequences at GPT-2 124M's width: 8,192 tokens of
+        # 12 documents, ragged, 12 heads of 64 as column slices of one qkv
+        # matrix. Work counted as the visible pairs: forward 2 products, backward
+        # 5; the plan is made once for both, as a step's layers do.
+        lengths = [3001, 1999, 1024, 777, 501, 333, 255, 128, 100, 63, 10, 1]
+        qkv = uniform((M, 3 * C), 110).to(dev)
+        dqkv = torch.empty_like(qkv)
+        g = normal((M, C), 111, 1.0, torch.float16).to(dev)
+        o = torch.empty((M, C), dtype=torch.float16, device=dev)
+        lse = torch.empty((H, M), device=dev)
+        edges = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+        offsets = torch.tensor(edges, dtype=torch.int32, device=dev)
+        shape = f.packed_shape(M, len(lengths), H, H, C // H, 3 * C, 3 * C, C)
+        plan = torch.empty(f.attention_packed_plan_bytes(shape), dtype=torch.uint8, device=dev)
+        ws = torch.empty(max(16, f.attention_packed_backward_workspace(shape)), dtype=torch.uint8,
+                         device=dev)
+        q, k, v = (qkv[:, i * C:(i + 1) * C] for i in range(3))
+        dq, dk, dv = (dqkv[:, i * C:(i + 1) * C] for i in range(3))
+        product = 2 * C * sum(n * (n + 1) // 2 for n in lengths)
+        f.attention_packed_plan(plan, offsets, shape)
+        ms = _time_gpu(torch, lambda _: f.attention_packed_forward(o, lse, q, k, v, plan, shape,
+                                                                   0.125), [0], per_round=8)
+        if want("flint_attention_packed_forward"):
+            record("flint_attention_packed_forward 8192 tokens of 12 documents, 12x64", "gemm",
+                   2 * product, ms, note="visible pairs of S = QK^T and O = PV; lengths 1 to 3001")
+        if want("flint_attention_packed_backward"):
+            ms = _time_gpu(torch, lambda _: f.attention_packed_backward(
+                dq, dk, dv, g, q, k, v, o, lse, plan, shape, 0.125, workspace=ws), [0], per_round=8)
+            record("flint_attention_packed_backward 8192 tokens of 12 documents, 12x64", "gemm",
+                   5 * product, ms, note="visible pairs of S (recomputed), dP, dV, dK, dQ")
+
+    def section_paged():
+        # One step of generation: 64 sequences, one new token each, over caches
+        # of 33 to 1,023 positions in pages of 16, 12 heads of 64.
+        S, P, W = 64, 16, T // 16
+        lengths = [33 + 990 * i // (S - 1) for i in range(S)]
+        shape = f.paged_shape(S, S, 1, H, H, C // H, 3 * C, 3 * C, C, S * W, P, W)
+        ws = torch.empty(max(16, f.attention_paged_workspace(shape)), dtype=torch.uint8, device=dev)
+        order = torch.randperm(S * W, generator=torch.Generator().manual_seed(120))
+        table = order.to(torch.int32).reshape(S, W).to(dev)
+        cached = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        offsets = torch.arange(S + 1, dtype=torch.int32, device=dev)
+        o = torch.empty((S, C), dtype=torch.float16, device=dev)
+        per = 2 * sum(lengths) * C * 2
+        sets = []
+        for r in range(_nsets(per)):
+            qkv = uniform((S, 3 * C), 121 + r).to(dev)
+            pages = [torch.randn(S * W, H, P, C // H, device=dev).half() for _ in range(2)]
+            sets.append((qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], *pages))
+        ms = _time_gpu(torch, lambda st: f.attention_paged(
+            o, st[3], st[4], st[0], st[1], st[2], offsets, cached, table, shape, 0.125,
+            workspace=ws), sets, per_round=16)
+        record("flint_attention_paged 64 sequences, 1 new token, 33-1023 cached, 12x64", "red",
+               per + 5 * S * C * 2 + S * C * 2, ms, note="K and V of the cached positions read once")
+        del sets
+        torch.cuda.empty_cache()
+
+    def section_logprobs():
+        # Log probabilities and entropy 8192 x 50304 (vocab 50257), and the
+        # gradient of the logits.
+        lg = normal((M, VP), 130, 2.0, torch.float16).to(dev)
+        _, t16 = targets(M, V, 131)
+        t16 = t16.to(dev)
+        lp, ent, dlp, dent = (torch.empty(M, device=dev) for _ in range(4))
+        dlp.fill_(1.0 / M)
+        dent.fill_(0.01 / M)
+        stats = torch.empty((M, 2), device=dev)
+        ms = _time_gpu(torch, lambda _: f.logprobs_forward(lp, ent, stats, None, None, lg, t16, 1.0,
+                                                           M, V, VP, 0), [0], per_round=8)
+        if want("flint_logprobs_forward"):
+            record("flint_logprobs_forward 8192x50304", "red", M * V * 2 + M * 18, ms,
+                   note="log probability and entropy; one set (824 MB logits) exceeds the cache")
+        if want("flint_logprobs_backward"):
+            dl = torch.empty_like(lg)
+            ms = _time_gpu(torch, lambda _: f.logprobs_backward(dl, dlp, dent, lg, t16, ent, stats,
+                                                                1.0, M, V, VP), [0], per_round=8)
+            record("flint_logprobs_backward 8192x50304", "red", M * (V + VP) * 2 + M * 22, ms)
+            del dl
+        del lg
+        torch.cuda.empty_cache()
+
     if any(want(x) for x in ("flint_gemm_nt_batched", "flint_gemm_nn_batched",
                              "flint_gemm_tn_batched")):
         section_batched()
@@ -509,6 +591,12 @@ def run(f, torch, dev, path, only=None):
         section_ce()
     if want("flint_attention_forward") or want("flint_attention_backward"):
         section_attention()
+    if want("flint_attention_packed_forward") or want("flint_attention_packed_backward"):
+        section_packed()
+    if want("flint_attention_paged"):
+        section_paged()
+    if want("flint_logprobs_forward") or want("flint_logprobs_backward"):
+        section_logprobs()
     if want("gpt2_124m_train_step stored") or want("gpt2_124m_train_step fused"):
         section_gpt2()
     if any(want(x) for x in ("flint_copy", "flint_fp32_to_fp16", "flint_heads_split",

@@ -8,9 +8,13 @@
 // item is a block of such rows and a part of the sequence's 64- or 32-key tiles;
 // the parts are joined by a second, small launch. Two kernels:
 //  * few rows (up to 32: generation). Reading the cache bounds it: 2 values of
-//    K and V a key and column against 4 FLOPs a row. Each of the four waves
-//    streams tiles of its own through LDS, two in flight, with no barrier until
-//    the waves' results are joined at the end.
+//    K and V a key and column against 4 FLOPs a row. Each wave streams tiles of
+//    its own through LDS, two in flight, with no barrier until the results of the
+//    workgroup's two waves are joined at the end. Until its first tile is there a
+//    workgroup takes some 6 us (its item, the pages, the rows), so four small ones
+//    share a CU (two at width 128): 64 sequences of 512 positions, 12 heads of 64,
+//    take 29 us so, and 50 with one workgroup of four waves and tiles of 64 keys
+//    (16 sequences of 4,096: 46 and 66).
 //  * many rows (chunks of prompts). Each wave takes 32 of 128 rows, and the four
 //    share the tiles, as in packed.hip.
 #include <hip/hip_runtime.h>
@@ -26,17 +30,25 @@ namespace flint {
 namespace {
 
 constexpr int kThreads = 256;   // 4 waves
+constexpr int kFewWaves = 2, kFewThreads = 64 * kFewWaves;
 constexpr int kGroups = 2;      // of 4 waves, where rows are many
 constexpr int kFewRows = 32, kManyRows = 128;
-// Workgroups aimed at (many rows: what the GPU holds at once, two a CU at width
-// 64 and one at 128), and the fewest tiles that a part of a sequence takes.
+// Workgroups aimed at: what the GPU holds at once at width 64 (few rows: four a
+// CU, many: two), half of it at 128; and the fewest tiles that a part of a
+// sequence takes.
 constexpr int kFewTarget = 1024, kManyTarget = 512;
 constexpr int kFewTiles = 4, kManyTiles = 4;
+// From this many tiles a workgroup on, few rows are cut for two rounds of
+// workgroups, the second of which evens out what the first did not. 64 ragged
+// sequences, 309,000 positions with 8 heads of K and V of 128 (150 tiles each),
+// take 258 us in two rounds and 309 in one; 32 of 3,000 positions, 12 heads of 64
+// (35 tiles), 65 and 62.
+constexpr int kTwoRounds = 64;
 
 template <int HD, bool MANY>
 struct Plan {
     static constexpr int kRows = MANY ? kManyRows : kFewRows;
-    static constexpr int kKeys = MANY || HD == 64 ? 64 : 32;   // of a tile
+    static constexpr int kKeys = MANY ? 64 : 32;   // of a tile
     static constexpr int kLeast = MANY ? kManyTiles : kFewTiles;
 };
 
@@ -54,6 +66,7 @@ struct PagedArgs {
     int negative;  // scale < 0: q enters negated
     int target;    // items a kv head aimed at
     int slots;     // parts that the workspace holds, a kv head
+    int rows;      // of a part there
     int2* splits;  // [sequences]: first slot, parts
     float2* sums;  // [slots][kv_heads][rows]: maximum (log2 units), sum
     float* parts;  // [slots][kv_heads][rows][HD]
@@ -105,19 +118,17 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     // 2^26.
     total = ((long long)(wave_sum(int(total >> 20))) << 20) + wave_sum(int(total & 0xfffff));
     constexpr long long kMost = 1 << 30;   // more tiles than any sequence has
-    int each = max(P::kLeast, int(min(kMost, (total + a.target - 1) / a.target)));
-    // Few rows: a workgroup on each CU first (a quarter of the target), then
-    // parts of 16 tiles, and only then more of them.
-    if constexpr (!MANY) each = max(each, int(min(16ll, (4 * total + a.target - 1) / a.target)));
-    // Many rows: the target is what the GPU holds at once, and parts that round
-    // up past it would run behind the others. (One step of sequences only; the
-    // parts of more are many anyway.)
-    if constexpr (MANY)
-        for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
-            const int parts = (tiles_of(q) + each - 1) / each;
-            if (wave_sum(blocks_of(q) * parts) <= a.target || __ballot(parts > 1) == 0) break;
-            each += (each + 7) / 8;
-        }
+    const bool twice = !MANY && total >= (long long)(kTwoRounds) * a.target;
+    const int target = twice ? 2 * a.target : a.target;
+    int each = max(P::kLeast, int(min(kMost, (total + target - 1) / target)));
+    // The target is what the GPU holds at once: parts that round up past it would
+    // run behind the others. (One step of sequences only; the parts of more are
+    // many anyway.)
+    for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
+        const int parts = (tiles_of(q) + each - 1) / each;
+        if (wave_sum(blocks_of(q) * parts) <= target || __ballot(parts > 1) == 0) break;
+        each += (each + 7) / 8;
+    }
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
         if (a.sequences > 64) {
@@ -342,11 +353,13 @@ __device__ __forceinline__ void store_splits(const PagedArgs& a, const Item& it,
 }
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
+__global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged_few(PagedArgs a) {
     using P = Plan<HD, false>;
-    constexpr int kTile = 4096;   // halves: 8 KB of K and of V
-    __shared__ __attribute__((aligned(16))) _Float16 lds[4 * 2 * 2 * kTile];   // [wave][buf][K, V]
-    __shared__ float2 wave_sums[4][32];
+    using R = Reader<HD, P::kKeys>;
+    constexpr int kTile = P::kKeys * HD, kW = kFewWaves;
+    constexpr int kOut = HD * kFewRows / kFewThreads;   // values of a thread at the end
+    __shared__ __attribute__((aligned(16))) _Float16 lds[kW * 2 * 2 * kTile];   // [wave][buf][K, V]
+    __shared__ float2 wave_sums[kW][32];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int fr = lane & 31, h = lane >> 5;
@@ -359,33 +372,33 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
     Rows<HD, P::kKeys> w;
     w.load_q(a, it, head, first_row + fr, rows, h);
     const int last = it.seq.cached + (first_row + fr) / a.group;
-    const Reader<HD, P::kKeys> reader(a, it, head, lane);
+    const R reader(a, it, head, lane);
     int from, to;
     part_of(a, it, kFewRows, P::kKeys, &from, &to);
     _Float16* mine = lds + wave * 4 * kTile;
     auto issue = [&](const Where& at, int t, int buf) __attribute__((always_inline)) {
         _Float16* kt = mine + buf * 2 * kTile;
 #pragma unroll
-        for (int u = 0; u < 8; ++u) reader.load(kt, kt + kTile, at, t, u);
+        for (int u = 0; u < R::kLoads; ++u) reader.load(kt, kt + kTile, at, t, u);
     };
     int t = from + wave;
     Where at = reader.find(t);
     unsigned valid = reader.valid(at, t);
     if (t < to) {
         issue(at, t, 0);
-        at = reader.find(t + 4);
+        at = reader.find(t + kW);
     }
-    store_new<HD, kThreads>(a, it, head, kFewRows);   // waits for no more than the tile does
-    for (int i = 0; t < to; ++i, t += 4) {
+    store_new<HD, kFewThreads>(a, it, head, kFewRows);   // waits for no more than the tile does
+    for (int i = 0; t < to; ++i, t += kW) {
         unsigned next = 0;
         // The other buffer's reads ended with the last tile's products.
         asm volatile("" ::: "memory");
-        if (t + 4 < to) {
-            next = reader.valid(at, t + 4);
-            const Where ahead = reader.find(t + 8);
-            issue(at, t + 4, (i + 1) & 1);
+        if (t + kW < to) {
+            next = reader.valid(at, t + kW);
+            const Where ahead = reader.find(t + 2 * kW);
+            issue(at, t + kW, (i + 1) & 1);
             at = ahead;
-            wait_vmcnt<16>();   // the newer tile's 8 loads of K and 8 of V, at least
+            wait_vmcnt<2 * R::kLoads>();   // the newer tile's loads of K and V, at least
         } else {
             wait_vmcnt<0>();
         }
@@ -404,21 +417,21 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
         for (int r = 0; r < 16; ++r) own[(32 * db + result_row(r, h)) * 32 + fr] = w.acc[db][r];
     if (h == 0) wave_sums[wave][fr] = float2{w.m, w.l};
     __syncthreads();
-    const int row = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * (HD / 8);
+    const int row = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * kOut;
     if (first_row + row < rows) {
-        float m = kFloor, l = 0.0f, by[4], sum[HD / 8] = {};
+        float m = kFloor, l = 0.0f, by[kW], sum[kOut] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m = fmaxf(m, wave_sums[i][row].x);
+        for (int i = 0; i < kW; ++i) m = fmaxf(m, wave_sums[i][row].x);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kW; ++i) {
             by[i] = __builtin_amdgcn_exp2f(wave_sums[i][row].x - m);
             l = __builtin_fmaf(wave_sums[i][row].y, by[i], l);
         }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kW; ++i) {
             const float* part = reinterpret_cast<const float*>(lds + i * 4 * kTile);
 #pragma unroll
-            for (int d = 0; d < HD / 8; ++d)
+            for (int d = 0; d < kOut; ++d)
                 sum[d] = __builtin_fmaf(part[(d0 + d) * 32 + row], by[i], sum[d]);
         }
         if (it.parts == 1) {
@@ -427,17 +440,17 @@ __global__ void __launch_bounds__(kThreads) paged_few(PagedArgs a) {
                           size_t(head * a.group + first_row + row - place * a.group) * HD + d0;
             const float inv = 1.0f / l;
 #pragma unroll
-            for (int d = 0; d < HD / 8; d += 8) {
+            for (int d = 0; d < kOut; d += 8) {
                 f16x8 v;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = _Float16(sum[d + e] * inv);
                 *reinterpret_cast<f16x8*>(o + d) = v;
             }
         } else {
-            const size_t at = (size_t(it.slot + it.part) * a.kv_heads + head) * kFewRows + row;
+            const size_t at = (size_t(it.slot + it.part) * a.kv_heads + head) * a.rows + row;
             if (d0 == 0) a.sums[at] = float2{m, l};
 #pragma unroll
-            for (int d = 0; d < HD / 8; d += 4)
+            for (int d = 0; d < kOut; d += 4)
                 *reinterpret_cast<f32x4*>(a.parts + at * HD + d0 + d) =
                     f32x4{sum[d], sum[d + 1], sum[d + 2], sum[d + 3]};
         }
@@ -538,7 +551,7 @@ __global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2) paged_ma
     }
     if (turn != 0 || first_row + fr >= rows) return;
     const size_t slot =
-        (size_t(it.slot + it.part) * a.kv_heads + head) * kManyRows + wave * 32 + fr;
+        (size_t(it.slot + it.part) * a.kv_heads + head) * a.rows + wave * 32 + fr;
     if (h == 0) a.sums[slot] = float2{w.m, w.l};
 #pragma unroll
     for (int db = 0; db < HD / 32; ++db)
@@ -576,11 +589,11 @@ struct Parts {
     int count;
 };
 __device__ __forceinline__ bool parts_of_row(const PagedArgs& a, const Sequence& q, int2 split,
-                                             int t, int head, int rows_of_block, Parts* p) {
+                                             int t, int head, Parts* p) {
     const int kv = head / a.group, row = (t - q.first) * a.group + head - kv * a.group;
-    const int block = row / rows_of_block, first = split.x + block * split.y;
-    p->step = size_t(a.kv_heads) * rows_of_block;
-    p->at = (size_t(first) * a.kv_heads + kv) * rows_of_block + (row - block * rows_of_block);
+    const int block = row / a.rows, first = split.x + block * split.y;
+    p->step = size_t(a.kv_heads) * a.rows;
+    p->at = (size_t(first) * a.kv_heads + kv) * a.rows + (row - block * a.rows);
     p->count = split.y;
     // Slots outside the workspace can come from offsets that decrease only.
     return split.y > 1 && first >= 0 && first + split.y <= a.slots;
@@ -592,7 +605,7 @@ __device__ __forceinline__ bool parts_of_row(const PagedArgs& a, const Sequence&
 // Few rows: four waves a row, whose sets take the parts in turn (a sequence may
 // have a thousand) and then add up.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a, int rows_of_block) {
+__global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a) {
     constexpr int kLanes = HD / 4, kSets = 64 / kLanes, kWaves = kThreads / 64;
     __shared__ __attribute__((aligned(16))) f32x4 wave_parts[kWaves][kLanes];
     __shared__ float wave_sums[kWaves];
@@ -602,7 +615,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a, int rows
     const int s = sequence_at(a, t, lane);
     if (s < 0) return;
     Parts p;
-    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, rows_of_block, &p)) return;
+    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, &p)) return;
     float m = kFloor;
     for (int i = lane; i < p.count; i += 64) m = fmaxf(m, a.sums[p.at + i * p.step].x);
 #pragma unroll
@@ -640,7 +653,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a, int rows
 // Many rows, of few parts each: a set a row, a wave on heads of one token, since
 // finding the token's sequence is a chain of loads.
 template <int HD>
-__global__ void __launch_bounds__(kThreads) paged_join_many(PagedArgs a, int rows_of_block) {
+__global__ void __launch_bounds__(kThreads) paged_join_many(PagedArgs a) {
     constexpr int kLanes = HD / 4, kSets = 64 / kLanes;
     const int lane = threadIdx.x & 63, d = lane % kLanes * 4;
     const unsigned id = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
@@ -650,7 +663,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_many(PagedArgs a, int row
     const int s = sequence_at(a, t, lane);
     if (s < 0 || head >= a.heads) return;
     Parts p;
-    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, rows_of_block, &p)) return;
+    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, &p)) return;
     float m = kFloor;
 #pragma unroll 4
     for (int i = 0; i < p.count; ++i) m = fmaxf(m, a.sums[p.at + i * p.step].x);
@@ -674,24 +687,26 @@ bool many_rows(const flint_paged_shape& s) {
 // What the kernels' grids and the workspace follow from. A block of rows may
 // have as many parts as the longest sequence has runs of kLeast tiles; a
 // sequence in p > 1 parts of `each` tiles has fewer than 2 tiles / each of them,
-// so the parts of all are below 2 target.
+// so the parts of all are below twice the items aimed at. Few rows are one block
+// of a sequence, and its parts hold no more rows than it can have.
 struct Sizes {
-    size_t target, blocks, slots, rows;
+    size_t target, most, blocks, slots, rows;
 };
 Sizes sizes_of(const flint_paged_shape& s) {
     const bool many = many_rows(s);
-    Sizes z;
-    z.rows = many ? kManyRows : kFewRows;
-    const size_t keys = many || s.head_width == 64 ? 64 : 32;
-    const size_t least = many ? kManyTiles : kFewTiles;
     const size_t group = s.heads / s.kv_heads, new_rows = std::min(s.max_new, s.tokens) * group;
-    const size_t target = many ? kManyTarget * 64 / s.head_width : kFewTarget;
+    Sizes z;
+    z.rows = many ? kManyRows : new_rows;
+    const size_t keys = many ? 64 : 32, least = many ? kManyTiles : kFewTiles;
+    const size_t target = (many ? kManyTarget : kFewTarget) * 64 / s.head_width;
     z.target = std::max<size_t>(1, target / s.kv_heads);
-    z.blocks = std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
-                        s.tokens * group / z.rows + s.sequences);
+    z.most = many ? z.target : 2 * z.target;
+    z.blocks = many ? std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
+                               s.tokens * group / z.rows + s.sequences)
+                    : s.sequences;
     const size_t longest = (s.max_pages * s.page_size + s.max_new + keys - 1) / keys;
     const size_t parts = (longest + least - 1) / least;
-    z.slots = parts > 1 ? std::min(2 * z.target, z.blocks * parts) : 0;
+    z.slots = parts > 1 ? std::min(2 * z.most, z.blocks * parts) : 0;
     return z;
 }
 
@@ -733,24 +748,23 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                 int(s.heads / s.kv_heads), int(s.q_stride), int(s.kv_stride), int(s.o_stride),
                 int(s.pages), int(s.page_size), int(s.max_pages),
                 magic, shift, int(s.kv_heads * s.page_size), std::fabs(scale) * kLog2e, scale < 0.0f,
-                int(z.target), int(z.slots), reinterpret_cast<int2*>(ws),
+                int(z.target), int(z.slots), int(z.rows), reinterpret_cast<int2*>(ws),
                 reinterpret_cast<float2*>(ws + w.sums), reinterpret_cast<float*>(ws + w.parts)};
-    const dim3 grid(unsigned((z.blocks + z.target) * s.kv_heads));
+    const dim3 grid(unsigned((z.blocks + z.most) * s.kv_heads));
     const bool many = many_rows(s), wide = s.head_width == 128;
     auto* const kernel = many ? (wide ? paged_many<128> : paged_many<64>)
                               : (wide ? paged_few<128> : paged_few<64>);
-    hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kThreads), 0, stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kFewThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
     // Waves enough for the GPU without sharing a row out.
     const size_t rows = s.tokens * s.heads, sets = 256 / s.head_width;
     if (rows <= 4096) {
         auto* const join = wide ? paged_join_few<128> : paged_join_few<64>;
-        hipLaunchKernelGGL(join, dim3(unsigned(rows)), dim3(kThreads), 0, stream, a, int(z.rows));
+        hipLaunchKernelGGL(join, dim3(unsigned(rows)), dim3(kThreads), 0, stream, a);
     } else {
         auto* const join = wide ? paged_join_many<128> : paged_join_many<64>;
         const size_t waves = s.tokens * ((s.heads + sets - 1) / sets);
-        hipLaunchKernelGGL(join, dim3(unsigned((waves + 3) / 4)), dim3(kThreads), 0, stream, a,
-                           int(z.rows));
+        hipLaunchKernelGGL(join, dim3(unsigned((waves + 3) / 4)), dim3(kThreads), 0, stream, a);
     }
     return hipGetLastError();
 }

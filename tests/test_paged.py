@@ -28,11 +28,11 @@ class Cache:
         self.max_new = max(new) if max_new is None else max_new
         S = len(cached)
         need = [-(-(c + n) // page_size) for c, n in zip(cached, new)]
-        self.pages = sum(need) + 2
+        self.pages = sum(need) - shared * (S - 1) + 2
         order = torch.randperm(self.pages, generator=gen(seed)).tolist()
         self.table = torch.full((S, max(max(need) + spare_columns, 1)), -1, dtype=torch.int32)
         for s, n in enumerate(need):
-            for i in range(min(n, self.table.shape[1])):
+            for i in range(shared if s else 0, min(n, self.table.shape[1])):
                 self.table[s, i] = order.pop()
             if s:   # the first pages are the first sequence's own: a shared prefix
                 self.table[s, :shared] = self.table[0, :shared]
@@ -181,6 +181,13 @@ def test_more_sequences_than_a_wave_has_lanes(flint, cuda, new):
 def test_one_long_sequence_in_many_parts(flint, cuda):
     check(Run(flint, cuda, Cache([60000], [1], 2, 1, 64, 64, seed=24)).run())
     check(Run(flint, cuda, Cache([30000], [40], 1, 1, 128, 128, seed=25)).run())
+
+
+@pytest.mark.gpu
+def test_so_many_tiles_that_the_parts_take_two_rounds(flint, cuda):
+    """64 tiles for each of the 16 items that one of 64 heads of K and V gets."""
+    c = Cache([2100 - 3 * s for s in range(16)], [1] * 16, 64, 64, 64, 64, seed=30, shared=32)
+    check(Run(flint, cuda, c).run())
 
 
 @pytest.mark.gpu
