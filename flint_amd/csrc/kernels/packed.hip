@@ -56,13 +56,16 @@ constexpr int kBuckets = 1024;
 // counting sort: full[b] counts the sequences whose last, partly filled bucket
 // is b, part[b] their places in it; the items of b are part[b] + (full[b + 1] +
 // full[b + 2] + ...) << shift. Within a bucket the order is the arrival's: it
-// changes which workgroup takes which block and no result.
+// changes which workgroup takes which block and no result. More blocks than the
+// plan holds, which takes offsets that decrease, make it empty: their number is
+// not bounded by tokens, nor the time to write them.
 __global__ void __launch_bounds__(kPlanThreads)
 packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequences, int tokens,
             int capacity, int shift) {
-    __shared__ int full[kBuckets], part[kBuckets], next[kBuckets], filled;
+    __shared__ int full[kBuckets], part[kBuckets], next[kBuckets], filled, blocks;
     const int tid = threadIdx.x;
     full[tid] = part[tid] = 0;
+    if (tid == 0) blocks = 0;
     __syncthreads();
     auto rows_of = [&](int s, int* begin) {
         const int a = min(max(offsets[s], 0), tokens), b = min(max(offsets[s + 1], a), tokens);
@@ -70,15 +73,23 @@ packed_plan(int4* __restrict__ plan, const int* __restrict__ offsets, int sequen
         return b;
     };
     const int low = (1 << shift) - 1;
+    int own = 0;   // this thread's blocks, and a wave's: at most capacity + 1
     for (int s = tid; s < sequences; s += kPlanThreads) {
         int begin;
         const int end = rows_of(s, &begin);
         const int n = (end - begin + kPackedBlock - 1) / kPackedBlock;
         if (n == 0) continue;
+        own = min(own + n, capacity + 1);
         atomicAdd(&full[n >> shift], 1);
         atomicAdd(&part[n >> shift], n & low);
     }
+    own = min(wave_sum(own), capacity + 1);
+    if (tid % 64 == 0) atomicAdd(&blocks, own);
     __syncthreads();
+    if (blocks > capacity) {
+        for (int i = tid; i < capacity; i += kPlanThreads) plan[i] = int4{0, 0, 0, 0};
+        return;
+    }
     // Sums over the buckets after this thread's, the last bucket first: a scan
     // in each wave and of the waves' totals.
     __shared__ int totals[kPlanThreads / 64];

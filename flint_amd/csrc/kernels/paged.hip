@@ -95,7 +95,10 @@ __device__ __forceinline__ int column_of(const PagedArgs& a, int p) {
 
 // Item `idx` of a kv head. Every item takes about the same number of tiles,
 // total / target: the sequences' lengths are known only here, so each wave adds
-// them up (64 sequences a step) and finds its item by a prefix sum.
+// them up (64 sequences a step) and finds its item by a prefix sum. (Four
+// sequences a lane, which saves 256 of them three chains of loads, cost as much in
+// divisions: 256 sequences of 200 positions stayed at 58 us, 64 of 512 took 32
+// instead of 29.)
 struct Item {
     Sequence seq;
     int s, block, part, parts, slot;   // slot of the block's part 0 (parts > 1)
@@ -114,9 +117,10 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
         if (s0 + lane < a.sequences) q = sequence_of(a, s0 + lane);
         total += (long long)(blocks_of(q)) * tiles_of(q);
     }
-    // In two words: the rows' blocks add up to at most 2^21, tiles are at most
-    // 2^26.
-    total = ((long long)(wave_sum(int(total >> 20))) << 20) + wave_sum(int(total & 0xfffff));
+    // In two words of 24 bits: the rows' blocks add up to at most 2^21 and tiles
+    // to 2^26, and only offsets that decrease pass that.
+    total = min(total, 1ll << 48);
+    total = ((long long)(wave_sum(int(total >> 24))) << 24) + wave_sum(int(total & 0xffffff));
     constexpr long long kMost = 1 << 30;   // more tiles than any sequence has
     const bool twice = !MANY && total >= (long long)(kTwoRounds) * a.target;
     const int target = twice ? 2 * a.target : a.target;

@@ -10,7 +10,8 @@
  * Token t of a sequence sees its sequence's tokens up to itself. Rows before
  * offsets[0] and from offsets[sequences] on belong to no sequence: they are not
  * read into any result, and their rows of every output stay as they were.
- * Offsets outside 0 .. tokens are taken as the nearer end.
+ * Offsets outside 0 .. tokens are taken as the nearer end; offsets that decrease
+ * may leave any row of the outputs as it was, and lead to none outside them.
  *
  * q and o hold heads x head_width FP16 values a token, k and v kv_heads x
  * head_width; query head h reads head h / (heads / kv_heads) of k and v. Rows

@@ -29,7 +29,9 @@
  * Rows of o outside every sequence stay as they were. Pages may be shared by
  * sequences as long as no call stores into a row that another sequence of the
  * call reads. Cache rows that hold no position (past a sequence's end, or of
- * no sequence) are not read into any result, whatever they hold. */
+ * no sequence) are not read into any result, whatever they hold. A non-finite
+ * value in a sequence's q, k or v, or in its cached positions, may reach every
+ * row of that sequence, and no other sequence. */
 #ifndef FLINT_FLINT_PAGED_H
 #define FLINT_FLINT_PAGED_H
 

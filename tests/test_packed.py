@@ -193,6 +193,16 @@ def test_offsets_outside_the_tokens_are_taken_inside(flint, cuda):
 
 
 @pytest.mark.gpu
+def test_offsets_that_decrease_make_no_more_blocks_than_the_plan_holds(flint, cuda):
+    """20 sequences of the same 512 tokens: 80 blocks, where 44 is the most."""
+    b = Batch([512] + [0] * 39, 2, 2, 64, seed=19)
+    r = Run(flint, cuda, b)
+    r.offsets = torch.tensor([0, 512] * 20 + [0], dtype=torch.int32, device=cuda)
+    for name, got in r.run().outputs().items():
+        assert torch.all(got == SENTINEL), name
+
+
+@pytest.mark.gpu
 def test_two_runs_are_bit_identical(flint, cuda):
     b = Batch([500, 33, 700], 4, 2, 128, seed=16)
     one, two = Run(flint, cuda, b).run().outputs(), Run(flint, cuda, b).run().outputs()

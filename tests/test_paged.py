@@ -281,6 +281,18 @@ def test_step_after_step_matches_one_chunk(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [1, 30])
+def test_offsets_that_decrease_stay_inside(flint, cuda, new):
+    c = Cache([500, 40, 3000, 7], [new] * 4, 4, 2, 64, 16, seed=31, after=9)
+    r = Run(flint, cuda, c)
+    n = 4 * new
+    r.offsets = torch.tensor([n, 0, n, -5, n], dtype=torch.int32, device=cuda)
+    r.run()
+    torch.cuda.synchronize()
+    assert torch.all(r.o[n:] == SENTINEL)
+
+
+@pytest.mark.gpu
 def test_two_runs_are_bit_identical(flint, cuda):
     c = Cache([3000, 100, 800], [1, 1, 1], 8, 2, 128, 16, seed=16)
     one, two = Run(flint, cuda, c).run().o, Run(flint, cuda, c).run().o
