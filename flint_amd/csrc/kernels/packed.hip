@@ -27,24 +27,27 @@ namespace {
 
 constexpr int kThreads = 256;   // of the joining launch
 
-// A workgroup's waves: `rows` of them over its 32 x rows queries (keys), times
-// `turns` groups that take the 64-row tiles in turn and join their sums in LDS
-// at the end. Two turns halve the longest block's time, which bounds batches of
-// different lengths (one head of one 3,913-token sequence: forward 53 -> 41 us,
-// backward 163 -> 110; the forward of 12 heads and 24 sequences up to that
-// length 59 -> 53), and cost batches of equal short ones some of their second
-// round of workgroups (8 x 1,024 tokens, 12 heads: forward 24 -> 29). Two rows
-// and four turns shorten that block more (25 us), but read each tile for half
-// the rows (one 8,192-token sequence 127 -> 182). dK and dV at 128-wide heads
-// take a wave's 512 registers: one turn (two rows and two turns: 616 -> 634).
-struct Waves {
-    int rows, turns;
-    constexpr int threads() const { return 64 * rows * turns; }
-    constexpr int parts() const { return kPackedBlock / (32 * rows); }   // workgroups of a block
-};
-constexpr Waves kForward{4, 2}, kQuery{4, 2};
+// A workgroup's waves: four over its 128 queries (keys), times `turns` groups
+// that take the 64-row tiles in turn and join their sums in LDS at the end. Two
+// turns halve the longest block's time, which bounds batches of different
+// lengths (one head of one 3,913-token sequence: forward 53 -> 41 us, backward
+// 163 -> 110; the forward of 12 heads and 24 sequences up to that length 59 ->
+// 53), and cost batches of equal short ones some of their second round of
+// workgroups (8 x 1,024 tokens, 12 heads: forward 24 -> 29, since then 27). Two
+// waves over 64 queries and four turns shorten that block more (25 us), but read
+// each tile for half the rows (one 8,192-token sequence 127 -> 182). dK and dV at
+// 128-wide heads take a wave's 512 registers: one turn (two waves and two turns:
+// 616 -> 634).
+constexpr int kRowWaves = kPackedBlock / 32;
+constexpr int kForwardTurns = 2, kQueryTurns = 2;
 template <int HD>
-constexpr Waves kKey = HD == 64 ? Waves{4, 2} : Waves{4, 1};
+constexpr int kKeyTurns = HD == 64 ? 2 : 1;
+constexpr int threads_of(int turns) { return 64 * kRowWaves * turns; }
+
+// The kernels that load tiles ahead keep all of a workgroup's LDS in one array:
+// with others beside it the compiler cannot tell the loads under way from what it
+// reads, and waits for them before every tile (the forward pass of 24 ragged
+// sequences, 12 heads of 64: 53 us instead of 46).
 
 // ---------------------------------------------------------------- plan
 
@@ -188,6 +191,25 @@ struct Strides {
     int q, kv, o;
 };
 
+// The backward kernels form 2^kUp P and with it 2^kUp dS, and take the factor
+// out of their sums again: over thousands of keys, or from a small dO, dS is
+// often below FP16's normal values (one head over 3,000 tokens, dO of 0.01: dQ
+// 3.2e-4 off relative to its size without the factor, 3.0e-4 with it, 2.1e-4
+// from storing it alone). A block whose sums overflow by it is done again
+// without it.
+constexpr float kUp = 8.0f;
+__device__ __forceinline__ float down_by(float up) { return up == 0.0f ? 1.0f : 0x1p-8f; }
+
+template <int DB>
+__device__ __forceinline__ bool non_finite(const f32x16 (&acc)[DB]) {
+    float zero = 0.0f;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) zero = __builtin_fmaf(acc[db][r], 0.0f, zero);
+    return !(zero == 0.0f);
+}
+
 // The turns' sums of one result added in LDS, in order, into the first's; false
 // in the others.
 template <int HD, int W, int G>
@@ -218,19 +240,20 @@ __device__ __forceinline__ bool join_turns(float* lds, f32x16* acc, int wave, in
 // ---------------------------------------------------------------- forward
 
 template <int HD>
-__global__ void __launch_bounds__(kForward.threads(), HD == 64 ? 4 : 2)
+__global__ void __launch_bounds__(threads_of(kForwardTurns), HD == 64 ? 4 : 2)
 packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float16* __restrict__ q,
                const _Float16* __restrict__ k, const _Float16* __restrict__ v,
                const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
                float c, bool negative) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    constexpr int W = kForward.rows, G = kForward.turns, kParts = kForward.parts();
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][K, V]
-    __shared__ float2 sums[G][W][32];
+    constexpr int W = kRowWaves, G = kForwardTurns;
+    // [buf][group][K, V]; behind them the turns' maxima and sums.
+    constexpr int kTiles = 2 * G * 2 * kTile;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[kTiles + G * W * 32 * 4];
+    float2(*sums)[W][32] = reinterpret_cast<float2(*)[W][32]>(lds + kTiles);
     Work w;
-    if (!work_of(plan, int(blockIdx.x) / kParts, heads, tokens, &w)) return;
-    const int row0 = w.block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
-    if (row0 >= w.length) return;
+    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    const int row0 = w.block * kPackedBlock;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
     const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
@@ -352,7 +375,7 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
             lse[size_t(w.head) * tokens + w.begin + qi] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
     __syncthreads();
-    copy_rows<HD, kForward.threads()>(rows, length - row0, [&](int row) {
+    copy_rows<HD, threads_of(kForwardTurns)>(rows, length - row0, [&](int row) {
         return out + size_t(w.begin + row0 + row) * st.o + size_t(w.head) * HD;
     });
 }
@@ -360,7 +383,7 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
 // ---------------------------------------------------------------- backward: dQ (and D)
 
 template <int HD>
-__global__ void __launch_bounds__(kQuery.threads(), 2)
+__global__ void __launch_bounds__(threads_of(kQueryTurns), 2)
 packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                    const _Float16* __restrict__ v, const _Float16* __restrict__ o,
@@ -368,12 +391,16 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
                    const int4* __restrict__ plan, int tokens, int heads, int group, Strides st,
                    float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    constexpr int W = kQuery.rows, G = kQuery.turns, kParts = kQuery.parts();
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][K, V]
+    constexpr int W = kRowWaves, G = kQueryTurns;
+    // [buf][group][K, V]; behind them the turns' rests and the overflow flag.
+    constexpr int kTiles = 2 * G * 2 * kTile;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[kTiles + (G * W * 32 + 4) * 2];
+    float(*rests)[W][32] = reinterpret_cast<float(*)[W][32]>(lds + kTiles);
+    int& overflow = *reinterpret_cast<int*>(lds + kTiles + G * W * 32 * 2);
     Work w;
-    if (!work_of(plan, int(blockIdx.x) / kParts, heads, tokens, &w)) return;
-    const int row0 = w.block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
-    if (row0 >= w.length) return;
+    if (!work_of(plan, int(blockIdx.x), heads, tokens, &w)) return;
+    if (threadIdx.x == 0) overflow = 0;
+    const int row0 = w.block * kPackedBlock;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) % W;
     const int turn = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) / W;
@@ -421,57 +448,81 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
     dd += xor32(dd);
     const size_t row_at = size_t(w.head) * tokens + w.begin + qi;
     const float lse2 = qi < length ? lse[row_at] * kLog2e : 0.0f;
-    if (qi < length && h == 0 && turn == 0) dsum[row_at] = dd;
 
-    f32x16 acc[DB] = {};   // dQ^T[d][q]
-    for (int i = 0; i < steps; ++i) {
-        wait_vmcnt<0>();
-        block_sync();
-        const _Float16* kt = lds + ((i & 1) * G + turn) * 2 * kTile;
-        const _Float16* vt = kt + kTile;
-        if (i + 1 < steps) load(i + 1);
-        const int kbase = 64 * (G * i + turn);
-        if (kbase > q0 + 31) continue;
-        const bool masked = kbase + 63 > q0;
-        // Two halves of 32 keys, each through all of its products before the
-        // next (fewer registers live at once).
+    f32x16 acc[DB];   // 2^up dQ^T[d][q]
+    float up = kUp;
+    for (;;) {
 #pragma unroll
-        for (int hb = 0; hb < 2; ++hb) {
-            f32x16 s = {}, dp = {};
+        for (int db = 0; db < DB; ++db) acc[db] = f32x16{};
+        const float l2 = lse2 - up;
+        float rest = 0.0f;   // 2^up times the sum of dS over the keys
+        for (int i = 0; i < steps; ++i) {
+            wait_vmcnt<0>();
+            block_sync();
+            const _Float16* kt = lds + ((i & 1) * G + turn) * 2 * kTile;
+            const _Float16* vt = kt + kTile;
+            if (i + 1 < steps) load(i + 1);
+            const int kbase = 64 * (G * i + turn);
+            if (kbase > q0 + 31) continue;
+            const bool masked = kbase + 63 > q0;
+            // Two halves of 32 keys, each through all of its products before the
+            // next (fewer registers live at once).
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                s = mfma(fo.row(kt, hb, kk), qf[kk], s);
-                dp = mfma(fo.row(vt, hb, kk), df[kk], dp);
-            }
-            f16x8 sf[2];
-            auto form = [&](auto mask) {
+            for (int hb = 0; hb < 2; ++hb) {
+                f32x16 s = {}, dp = {};
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    float p = __builtin_amdgcn_exp2f(s[r] * c - lse2);
-                    if constexpr (mask)
-                        if (kbase + 32 * hb + result_row(r, h) > qi) p = 0.0f;
-                    sf[r >> 3][r & 7] = _Float16(p * (dp[r] - dd));
+                for (int kk = 0; kk < KK; ++kk) {
+                    s = mfma(fo.row(kt, hb, kk), qf[kk], s);
+                    dp = mfma(fo.row(vt, hb, kk), df[kk], dp);
                 }
-            };
-            if (masked) form(std::true_type{});
-            else form(std::false_type{});
-            // dQ^T += K^T dS^T.
+                f16x8 sf[2];
+                auto form = [&](auto mask) {
 #pragma unroll
-            for (int cs = 0; cs < 2; ++cs) {
-                TrFrag kf[DB];
+                    for (int r = 0; r < 16; ++r) {
+                        float p = __builtin_amdgcn_exp2f(s[r] * c - l2);
+                        if constexpr (mask)
+                            if (kbase + 32 * hb + result_row(r, h) > qi) p = 0.0f;
+                        const float ds = p * (dp[r] - dd);
+                        rest += ds;
+                        sf[r >> 3][r & 7] = _Float16(ds);
+                    }
+                };
+                if (masked) form(std::true_type{});
+                else form(std::false_type{});
+                // dQ^T += K^T dS^T.
 #pragma unroll
-                for (int db = 0; db < DB; ++db) kf[db] = fo.transposed(kt, 2 * hb + cs, db);
-                wait_lds();
+                for (int cs = 0; cs < 2; ++cs) {
+                    TrFrag kf[DB];
 #pragma unroll
-                for (int db = 0; db < DB; ++db) acc[db] = mfma(as_f16x8(kf[db]), sf[cs], acc[db]);
+                    for (int db = 0; db < DB; ++db) kf[db] = fo.transposed(kt, 2 * hb + cs, db);
+                    wait_lds();
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[db] = mfma(as_f16x8(kf[db]), sf[cs], acc[db]);
+                }
             }
         }
+        // dS adds up to 0 over a query's keys where D is what it should be. D from
+        // an FP16 O is not quite; dK, in the next launch, gets it put right.
+        rest += xor32(rest);
+        if (h == 0) rests[turn][wave][fr] = rest;
+        if (__any(non_finite(acc)) && lane == 0) overflow = 1;
+        __syncthreads();
+        if (up == 0.0f || overflow == 0) break;
+        up = 0.0f;
+        load(0);
+    }
+    const float down = down_by(up);
+    if (qi < length && h == 0 && turn == 0) {
+        float rest = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; ++g) rest += rests[g][wave][fr];
+        dsum[row_at] = __builtin_fmaf(rest, down, dd);
     }
     _Float16* rows = lds + (G - 1) * W * HD * 32 * 2;   // behind the turns' sums
     if (join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane))
-        write_rows<HD>(rows, acc, scale, wave * 32 + fr, h);
+        write_rows<HD>(rows, acc, scale * down, wave * 32 + fr, h);
     __syncthreads();
-    copy_rows<HD, kQuery.threads()>(rows, length - row0, [&](int row) {
+    copy_rows<HD, threads_of(kQueryTurns)>(rows, length - row0, [&](int row) {
         return dq + q_at + size_t(row0 + row) * st.q;
     });
 }
@@ -486,7 +537,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
 // sums ([part][token][kv head][HD], dK then dV) for packed_backward_join: heads
 // of k and v are few where groups are large, and so are workgroups then.
 template <int HD>
-__global__ void __launch_bounds__(kKey<HD>.threads(), HD == 64 ? 2 : 1)
+__global__ void __launch_bounds__(threads_of(kKeyTurns<HD>), HD == 64 ? 2 : 1)
 packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const _Float16* __restrict__ q, const _Float16* __restrict__ k,
                      const _Float16* __restrict__ v, const _Float16* __restrict__ dout,
@@ -494,12 +545,16 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
                      const int4* __restrict__ plan, float* __restrict__ sums, int tokens,
                      int kv_heads, int group, int share, Strides st, float c, float scale) {
     constexpr int kTile = Tile<HD>::kHalves, KK = HD / 16, DB = HD / 32;
-    constexpr int W = kKey<HD>.rows, G = kKey<HD>.turns, kParts = kKey<HD>.parts();
-    __shared__ __attribute__((aligned(16))) _Float16 lds[2 * G * 2 * kTile];   // [buf][group][Q, dO]
-    __shared__ __attribute__((aligned(16))) float rowstat[2][G][2][64];        // [buf][group][lse, D]
+    constexpr int W = kRowWaves, G = kKeyTurns<HD>;
+    // [buf][group][Q, dO]; behind them [buf][group][lse, D] and the overflow flag.
+    constexpr int kTiles = 2 * G * 2 * kTile, kStats = 2 * G * 2 * 64;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[kTiles + (kStats + 4) * 2];
+    float(*rowstat)[2][64] = reinterpret_cast<float(*)[2][64]>(lds + kTiles);
+    int& overflow = *reinterpret_cast<int*>(lds + kTiles + kStats * 2);
     Work w;
     const int parts = group / share;
-    if (!work_of(plan, int(blockIdx.x) / kParts, kv_heads * parts, tokens, &w)) return;
+    if (!work_of(plan, int(blockIdx.x), kv_heads * parts, tokens, &w)) return;
+    if (threadIdx.x == 0) overflow = 0;
     const int part = w.head % parts;
     w.head /= parts;
     const int lane = threadIdx.x & 63;
@@ -511,16 +566,25 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
     // The list's long blocks are the last of their sequences; as keys the first
     // ones have the most queries.
     const int block = (length + kPackedBlock - 1) / kPackedBlock - 1 - w.block;
-    const int row0 = block * kPackedBlock + int(blockIdx.x) % kParts * 32 * W;
-    if (row0 >= length) return;
+    const int row0 = block * kPackedBlock;
     const size_t kv_at = size_t(w.begin) * st.kv + size_t(w.head) * HD;
     const int k0 = row0 + wave * 32;
     const int ki = k0 + fr;
 
-    f32x16 dka[DB] = {}, dva[DB] = {};   // dK^T, dV^T [d][key]
+    f32x16 dka[DB], dva[DB];   // 2^up dK^T, dV^T [d][key]
+    float up = kUp;
     const int first = row0 / 64;
     const int per_head = (length + 63) / 64 - first;
     const int tiles = per_head * share, steps = (tiles + G - 1) / G;
+    // A step's lse and D, of wave 0's lanes, go to LDS at the step's start, when
+    // its tiles are there as well.
+    float lv = 0.0f, dv0 = 0.0f;
+    auto note = [&](int i) {
+        if (wave != 0) return;
+        const int buf = (i & 1) * G + turn;
+        rowstat[buf][0][lane] = __builtin_fmaf(lv, kLog2e, -up);
+        rowstat[buf][1][lane] = dv0;
+    };
     auto stage = [&](int i) {
         const int at_tile = G * i + turn;
         if (at_tile >= tiles) return;
@@ -529,7 +593,7 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
         const int head = w.head * group + part * share + g;
         _Float16* t = lds + buf * 2 * kTile;
         const int qq = 64 * tile + lane;
-        float lv = 0.0f, dv0 = 0.0f;
+        lv = dv0 = 0.0f;
         if (wave == 0 && qq < length) {
             const size_t at = size_t(head) * tokens + w.begin + qq;
             lv = lse[at];
@@ -539,10 +603,6 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
         load_tile<HD, W>(t, q + row * st.q + size_t(head) * HD, length - 64 * tile, st.q, wave, lane);
         load_tile<HD, W>(t + kTile, dout + row * st.o + size_t(head) * HD, length - 64 * tile, st.o,
                          wave, lane);
-        if (wave == 0) {
-            (&rowstat[0][0])[buf][0][lane] = lv * kLog2e;
-            (&rowstat[0][0])[buf][1][lane] = dv0;
-        }
     };
     // K and V go through the buffers: the second step's, and the first's for
     // want of room with one turn.
@@ -562,69 +622,81 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
         block_sync();
         stage(0);
     }
-    int tile = first + turn % per_head;
-    for (int i = 0; i < steps; ++i) {
-        const int buf = (i & 1) * G + turn;
-        wait_vmcnt<0>();
-        __syncthreads();
-        const _Float16* qt = lds + buf * 2 * kTile;
-        const _Float16* gt = qt + kTile;
-        const float* l2 = (&rowstat[0][0])[buf][0];
-        const float* dd = (&rowstat[0][0])[buf][1];
-        if (i + 1 < steps) stage(i + 1);
-        const int qbase = 64 * tile;
-        tile += G;
-        while (tile >= first + per_head) tile -= per_head;
-        if (G * i + turn >= tiles) break;
-        if (qbase + 63 < k0) continue;        // every query before every key of the wave
-        const bool masked = qbase < k0 + 31 || qbase + 63 >= length;
+    for (;;) {
 #pragma unroll
-        for (int qh = 0; qh < 2; ++qh) {
-            f32x16 s = {}, dp = {};
+        for (int db = 0; db < DB; ++db) dka[db] = dva[db] = f32x16{};
+        int tile = first + turn % per_head;
+        for (int i = 0; i < steps; ++i) {
+            const int buf = (i & 1) * G + turn;
+            wait_vmcnt<0>();
+            note(i);
+            __syncthreads();
+            const _Float16* qt = lds + buf * 2 * kTile;
+            const _Float16* gt = qt + kTile;
+            const float* l2 = rowstat[buf][0];
+            const float* dd = rowstat[buf][1];
+            if (i + 1 < steps) stage(i + 1);
+            const int qbase = 64 * tile;
+            tile += G;
+            while (tile >= first + per_head) tile -= per_head;
+            if (G * i + turn >= tiles) break;
+            if (qbase + 63 < k0) continue;        // every query before every key of the wave
+            const bool masked = qbase < k0 + 31 || qbase + 63 >= length;
 #pragma unroll
-            for (int kk = 0; kk < KK; ++kk) {
-                s = mfma(fo.row(qt, qh, kk), kf[kk], s);
-                dp = mfma(fo.row(gt, qh, kk), vf[kk], dp);
-            }
-            f16x8 pf[2], sf[2];
-            auto form = [&](auto mask) {
+            for (int qh = 0; qh < 2; ++qh) {
+                f32x16 s = {}, dp = {};
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    const int qr = 32 * qh + 8 * a + 4 * h;   // query row in the tile, + e
-                    const f32x4 l4 = *reinterpret_cast<const f32x4*>(l2 + qr);
-                    const f32x4 d4 = *reinterpret_cast<const f32x4*>(dd + qr);
+                for (int kk = 0; kk < KK; ++kk) {
+                    s = mfma(fo.row(qt, qh, kk), kf[kk], s);
+                    dp = mfma(fo.row(gt, qh, kk), vf[kk], dp);
+                }
+                f16x8 pf[2], sf[2];
+                auto form = [&](auto mask) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int r = 4 * a + e;
-                        float p = __builtin_amdgcn_exp2f(s[r] * c - l4[e]);
-                        if constexpr (mask) {
-                            if (ki > qbase + qr + e || qbase + qr + e >= length) p = 0.0f;
+                    for (int a = 0; a < 4; ++a) {
+                        const int qr = 32 * qh + 8 * a + 4 * h;   // query row in the tile, + e
+                        const f32x4 l4 = *reinterpret_cast<const f32x4*>(l2 + qr);
+                        const f32x4 d4 = *reinterpret_cast<const f32x4*>(dd + qr);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int r = 4 * a + e;
+                            float p = __builtin_amdgcn_exp2f(s[r] * c - l4[e]);
+                            if constexpr (mask) {
+                                if (ki > qbase + qr + e || qbase + qr + e >= length) p = 0.0f;
+                            }
+                            pf[a >> 1][4 * (a & 1) + e] = _Float16(p);
+                            sf[a >> 1][4 * (a & 1) + e] = _Float16(p * (dp[r] - d4[e]));
                         }
-                        pf[a >> 1][4 * (a & 1) + e] = _Float16(p);
-                        sf[a >> 1][4 * (a & 1) + e] = _Float16(p * (dp[r] - d4[e]));
                     }
-                }
-            };
-            if (masked) form(std::true_type{});
-            else form(std::false_type{});
-            // dV^T += dO^T P^T and dK^T += Q^T dS^T, a 16-query slice at a time.
+                };
+                if (masked) form(std::true_type{});
+                else form(std::false_type{});
+                // dV^T += dO^T P^T and dK^T += Q^T dS^T, a 16-query slice at a time.
 #pragma unroll
-            for (int cs = 0; cs < 2; ++cs) {
-                TrFrag gf[DB], tf[DB];
+                for (int cs = 0; cs < 2; ++cs) {
+                    TrFrag gf[DB], tf[DB];
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    gf[db] = fo.transposed(gt, 2 * qh + cs, db);
-                    tf[db] = fo.transposed(qt, 2 * qh + cs, db);
-                }
-                wait_lds();
+                    for (int db = 0; db < DB; ++db) {
+                        gf[db] = fo.transposed(gt, 2 * qh + cs, db);
+                        tf[db] = fo.transposed(qt, 2 * qh + cs, db);
+                    }
+                    wait_lds();
 #pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    dva[db] = mfma(as_f16x8(gf[db]), pf[cs], dva[db]);
-                    dka[db] = mfma(as_f16x8(tf[db]), sf[cs], dka[db]);
+                    for (int db = 0; db < DB; ++db) {
+                        dva[db] = mfma(as_f16x8(gf[db]), pf[cs], dva[db]);
+                        dka[db] = mfma(as_f16x8(tf[db]), sf[cs], dka[db]);
+                    }
                 }
             }
         }
+        if (up == 0.0f) break;
+        if (__any(non_finite(dka)) && lane == 0) overflow = 1;
+        __syncthreads();
+        if (overflow == 0) break;
+        up = 0.0f;
+        stage(0);
     }
+    const float down = down_by(up);
     const size_t at = kv_at + size_t(row0) * st.kv;
     _Float16* rows = lds + (G - 1) * W * HD * 32 * 2;   // behind the turns' sums
     bool mine = false;
@@ -633,9 +705,9 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
         f32x16* acc = which == 0 ? dka : dva;
         mine = join_turns<HD, W, G>(reinterpret_cast<float*>(lds), acc, wave, turn, lane);
         if (parts > 1) continue;
-        if (mine) write_rows<HD>(rows, acc, which == 0 ? scale : 1.0f, wave * 32 + fr, h);
+        if (mine) write_rows<HD>(rows, acc, which == 0 ? scale * down : down, wave * 32 + fr, h);
         __syncthreads();
-        copy_rows<HD, kKey<HD>.threads()>(rows, length - row0, [&](int row) {
+        copy_rows<HD, threads_of(kKeyTurns<HD>)>(rows, length - row0, [&](int row) {
             return (which == 0 ? dk : dv) + at + size_t(row) * st.kv;
         });
     }
@@ -647,10 +719,11 @@ packed_backward_dkdv(_Float16* __restrict__ dk, _Float16* __restrict__ dv,
 #pragma unroll
         for (int a = 0; a < 4; ++a) {
             const int d = 32 * db + 8 * a + 4 * h;
-            *reinterpret_cast<f32x4*>(to + d) = f32x4{dka[db][4 * a], dka[db][4 * a + 1],
-                                                      dka[db][4 * a + 2], dka[db][4 * a + 3]};
-            *reinterpret_cast<f32x4*>(to + dv_at + d) =
-                f32x4{dva[db][4 * a], dva[db][4 * a + 1], dva[db][4 * a + 2], dva[db][4 * a + 3]};
+            auto four = [&](const f32x16& acc) {
+                return f32x4{acc[4 * a], acc[4 * a + 1], acc[4 * a + 2], acc[4 * a + 3]} * down;
+            };
+            *reinterpret_cast<f32x4*>(to + d) = four(dka[db]);
+            *reinterpret_cast<f32x4*>(to + dv_at + d) = four(dva[db]);
         }
 }
 
@@ -709,9 +782,9 @@ template <int HD>
 hipError_t forward(void* o, void* lse, const void* q, const void* k, const void* v,
                    const void* plan, const flint_packed_shape& s, float scale,
                    hipStream_t stream) {
-    hipLaunchKernelGGL(packed_forward<HD>,
-                       dim3(unsigned(packed_items(s) * s.heads * kForward.parts())),
-                       dim3(kForward.threads()), 0, stream, static_cast<_Float16*>(o), static_cast<float*>(lse),
+    hipLaunchKernelGGL(packed_forward<HD>, dim3(unsigned(packed_items(s) * s.heads)),
+                       dim3(threads_of(kForwardTurns)), 0, stream, static_cast<_Float16*>(o),
+                       static_cast<float*>(lse),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const int4*>(plan),
                        int(s.tokens), int(s.heads), int(s.heads / s.kv_heads),
@@ -727,9 +800,8 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     const Strides st{int(s.q_stride), int(s.kv_stride), int(s.o_stride)};
     auto* dsum = static_cast<float*>(workspace);
     const int group = int(s.heads / s.kv_heads);
-    hipLaunchKernelGGL(packed_backward_dq<HD>,
-                       dim3(unsigned(packed_items(s) * s.heads * kQuery.parts())),
-                       dim3(kQuery.threads()), 0, stream, static_cast<_Float16*>(dq), dsum,
+    hipLaunchKernelGGL(packed_backward_dq<HD>, dim3(unsigned(packed_items(s) * s.heads)),
+                       dim3(threads_of(kQueryTurns)), 0, stream, static_cast<_Float16*>(dq), dsum,
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(o),
                        static_cast<const _Float16*>(dout), static_cast<const float*>(lse),
@@ -738,8 +810,9 @@ hipError_t backward(void* dq, void* dk, void* dv, const void* dout, const void* 
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     const size_t parts = group_parts(s), blocks = packed_items(s) * s.kv_heads;
     float* sums = dsum + dsum_values(s);
-    hipLaunchKernelGGL(packed_backward_dkdv<HD>, 
-                       dim3(unsigned(blocks * parts * kKey<HD>.parts())), dim3(kKey<HD>.threads()), 0, stream, static_cast<_Float16*>(dk), static_cast<_Float16*>(dv),
+    hipLaunchKernelGGL(packed_backward_dkdv<HD>, dim3(unsigned(blocks * parts)),
+                       dim3(threads_of(kKeyTurns<HD>)), 0, stream, static_cast<_Float16*>(dk),
+                       static_cast<_Float16*>(dv),
                        static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                        static_cast<const _Float16*>(v), static_cast<const _Float16*>(dout),
                        static_cast<const float*>(lse), static_cast<const float*>(dsum),

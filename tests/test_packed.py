@@ -185,6 +185,17 @@ def test_large_scores(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv_heads,width,size", [(2, 2, 64, 400.0), (4, 1, 128, 400.0),
+                                                       (4, 2, 64, 2e-4)])
+def test_large_and_small_gradients(flint, cuda, heads, kv_heads, width, size):
+    """dS past what FP16 holds at 2^8 times its size, and far below its normal
+    values."""
+    b = Batch([300, 65, 700], heads, kv_heads, width, seed=20)
+    b.dout = (b.dout.float() * (2 * size)).half()
+    check(Run(flint, cuda, b).run())
+
+
+@pytest.mark.gpu
 def test_offsets_outside_the_tokens_are_taken_inside(flint, cuda):
     b = Batch([40, 60], 2, 2, 64, seed=15)
     r = Run(flint, cuda, b)
