@@ -54,7 +54,8 @@ __device__ __forceinline__ void keep_packed(h8& v) { asm volatile("" : "+v"(v));
 
 // One workgroup of THREADS a row, which it reads once into registers (thread t
 // holds the 16-byte chunks t, t + THREADS, ...: at most CPT). Reading bounds it:
-// 7 VALU slots a word against 2 bytes.
+// 7 VALU slots a word against 2 bytes. 8,192 rows of 50,257 words: 133 to 149 us
+// on different cards, 5.5 to 6.2 TB/s; with 5 alternatives 178.
 //
 // Alternatives: the row falls into 64 groups of threads. The top-th largest of
 // the groups' maxima is a border that at least `top` words reach, and few more
@@ -296,14 +297,17 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
 }
 
 // A streaming pass (log p of a word of probability 0 is -1e4: no 0 x inf, however
-// large dH is): kAhead chunks of a thread are read before the first of
-// them is written (dlogits may be logits, so the compiler keeps that order).
+// large dH is): a workgroup takes kAhead chunks a thread of a row, all read before
+// the first is written (dlogits may be logits, so the compiler keeps that order).
+// HBM bounds it: 8,192 rows of 50,257 words 311 us, 5.3 TB/s. Shares of a row
+// instead of whole ones are for few rows: 16 of 50,257 words take 5.0 us, and 10.1
+// in one workgroup each.
+constexpr int kAhead = 9;
 __global__ void __launch_bounds__(kThreads)
 logprobs_backward(h8* dlogits, const float* __restrict__ dlogprob,
                   const float* __restrict__ dentropy, const h8* logits,
                   const uint16_t* __restrict__ targets, const float* __restrict__ entropy,
                   const float* __restrict__ stats, float scale, int vocab, int chunks) {
-    constexpr int kAhead = 5;
     const size_t row = blockIdx.x;
     const int t = targets[row];
     const float mx = stats[2 * row], log_sum = stats[2 * row + 1];
@@ -312,35 +316,34 @@ logprobs_backward(h8* dlogits, const float* __restrict__ dlogprob,
     const float ent = dentropy != nullptr ? entropy[row] : 0.0f;
     const h8* from = logits + row * chunks;
     h8* to = dlogits + row * chunks;
-    for (int c0 = threadIdx.x; c0 < chunks; c0 += kThreads * kAhead) {
-        h8 l[kAhead];
+    const int c0 = int(blockIdx.y) * kThreads * kAhead + int(threadIdx.x);
+    h8 l[kAhead];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k)
-            if (c0 + k * kThreads < chunks) l[k] = from[c0 + k * kThreads];
+    for (int k = 0; k < kAhead; ++k)
+        if (c0 + k * kThreads < chunks) l[k] = from[c0 + k * kThreads];
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            const int c = c0 + k * kThreads;
-            if (c >= chunks) break;
-            float d[8];
+    for (int k = 0; k < kAhead; ++k) {
+        const int c = c0 + k * kThreads;
+        if (c >= chunks) break;
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float lp = __builtin_fmaf(scale, float(l[k][i]) - mx, -log_sum);
+            const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
+            d[i] = -scale * p * __builtin_fmaf(dh, fmaxf(lp, -1e4f) + ent, dlp);
+        }
+        if (c == t >> 3 || c == (vocab - 1) >> 3 || c > (vocab - 1) >> 3) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float lp = __builtin_fmaf(scale, float(l[k][i]) - mx, -log_sum);
-                const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
-                d[i] = -scale * p * __builtin_fmaf(dh, fmaxf(lp, -1e4f) + ent, dlp);
+                const int j = 8 * c + i;
+                if (j == t) d[i] += scale * dlp;
+                if (j >= vocab) d[i] = 0.0f;
             }
-            if (c == t >> 3 || c == (vocab - 1) >> 3 || c > (vocab - 1) >> 3) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int j = 8 * c + i;
-                    if (j == t) d[i] += scale * dlp;
-                    if (j >= vocab) d[i] = 0.0f;
-                }
-            }
-            h8 out;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) out[i] = _Float16(d[i]);
-            store_stream(to + c, out);
         }
+        h8 out;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) out[i] = _Float16(d[i]);
+        store_stream(to + c, out);
     }
 }
 
@@ -350,8 +353,10 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
                                    void* top_logprobs, const void* logits, const void* targets,
                                    float scale, size_t rows, size_t vocab, size_t cols, size_t top,
                                    hipStream_t stream) {
-    // A wave a row while it holds at most 4 chunks a lane, else 256 threads, or
-    // 1,024 where the rows leave CUs idle and a row is long enough.
+    // A wave a row while it holds at most 4 chunks a lane (8,192 rows of 997 words:
+    // 10.3 us, and 21.8 with 256 threads), else 256 threads, or 1,024 where the rows
+    // leave CUs idle and are long (16 rows of 50,257 words and 5 alternatives: 8.7
+    // us, and 13.0 with 256; 1,024 rows the other way 33 and 24).
     const size_t held = (vocab + 7) / 8;
     const bool few = rows <= 256 && held > 1024;
     for (size_t done = 0; done < rows;) {
@@ -391,11 +396,13 @@ hipError_t launch_logprobs_backward(void* dlogits, const void* dlogprob, const v
                                     const void* logits, const void* targets, const void* entropy,
                                     const void* stats, float scale, size_t rows, size_t vocab,
                                     size_t cols, hipStream_t stream) {
+    constexpr size_t kShare = kThreads * kAhead;
+    const auto shares = unsigned((cols / 8 + kShare - 1) / kShare);
     for (size_t done = 0; done < rows;) {
         const size_t n = std::min<size_t>(rows - done, size_t{1} << 22);
         const auto* dh = static_cast<const float*>(dentropy);
         const auto* ent = static_cast<const float*>(entropy);
-        hipLaunchKernelGGL(logprobs_backward, dim3(unsigned(n)), dim3(kThreads), 0, stream,
+        hipLaunchKernelGGL(logprobs_backward, dim3(unsigned(n), shares), dim3(kThreads), 0, stream,
                            static_cast<h8*>(dlogits) + done * (cols / 8),
                            static_cast<const float*>(dlogprob) + done,
                            dh == nullptr ? nullptr : dh + done,
