@@ -607,7 +607,8 @@ __device__ __forceinline__ bool parts_of_row(const PagedArgs& a, const Sequence&
 // take 4 columns of a row each.
 //
 // Few rows: four waves a row, whose sets take the parts in turn (a sequence may
-// have a thousand) and then add up.
+// have a thousand) and then add up. The grid is sequences x heads and places, so
+// that no search stands before the parts (16 sequences of 100: 8.0 -> 7.5 us).
 template <int HD>
 __global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a) {
     constexpr int kLanes = HD / 4, kSets = 64 / kLanes, kWaves = kThreads / 64;
@@ -615,11 +616,13 @@ __global__ void __launch_bounds__(kThreads) paged_join_few(PagedArgs a) {
     __shared__ float wave_sums[kWaves];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, d = lane % kLanes * 4;
     const int set = wave * kSets + lane / kLanes;
-    const int t = int(blockIdx.x / unsigned(a.heads)), head = int(blockIdx.x % unsigned(a.heads));
-    const int s = sequence_at(a, t, lane);
-    if (s < 0) return;
+    const int s = int(blockIdx.x / unsigned(a.heads)), head = int(blockIdx.x % unsigned(a.heads));
+    const Sequence q = sequence_of(a, s);
+    const int2 split = a.splits[s];
+    if (int(blockIdx.y) >= q.count) return;
+    const int t = q.first + int(blockIdx.y);
     Parts p;
-    if (!parts_of_row(a, sequence_of(a, s), a.splits[s], t, head, &p)) return;
+    if (!parts_of_row(a, q, split, t, head, &p)) return;
     float m = kFloor;
     for (int i = lane; i < p.count; i += 64) m = fmaxf(m, a.sums[p.at + i * p.step].x);
 #pragma unroll
@@ -760,11 +763,12 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                               : (wide ? paged_few<128> : paged_few<64>);
     hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kFewThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess || z.slots == 0) return e;
-    // Waves enough for the GPU without sharing a row out.
-    const size_t rows = s.tokens * s.heads, sets = 256 / s.head_width;
-    if (rows <= 4096) {
+    // Past some 4,096 rows there are waves enough without sharing a row out.
+    const size_t sets = 256 / s.head_width, places = std::min(s.max_new, s.tokens);
+    if (s.sequences * places * s.heads <= 4096) {
         auto* const join = wide ? paged_join_few<128> : paged_join_few<64>;
-        hipLaunchKernelGGL(join, dim3(unsigned(rows)), dim3(kThreads), 0, stream, a);
+        hipLaunchKernelGGL(join, dim3(unsigned(s.sequences * s.heads), unsigned(places)),
+                           dim3(kThreads), 0, stream, a);
     } else {
         auto* const join = wide ? paged_join_many<128> : paged_join_many<64>;
         const size_t waves = s.tokens * ((s.heads + sets - 1) / sets);
