@@ -55,7 +55,7 @@ __device__ __forceinline__ void keep_packed(h8& v) { asm volatile("" : "+v"(v));
 // One workgroup of THREADS a row, which it reads once into registers (thread t
 // holds the 16-byte chunks t, t + THREADS, ...: at most CPT). Reading bounds it:
 // 7 VALU slots a word against 2 bytes. 8,192 rows of 50,257 words: 133 to 149 us
-// on different cards, 5.5 to 6.2 TB/s; with 5 alternatives 178.
+// on different cards, 5.5 to 6.2 TB/s; with 5 alternatives 170.
 //
 // Alternatives: the row falls into 64 groups of threads. The top-th largest of
 // the groups' maxima is a border that at least `top` words reach, and few more
@@ -113,10 +113,10 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
         constexpr int kGroup = THREADS / 64;
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0xB1, 0xF, 0xF, false)));
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x4E, 0xF, 0xF, false)));
-        if constexpr (kGroup == 16) {
+        if constexpr (kGroup >= 8)
             group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x141, 0xF, 0xF, false)));
+        if constexpr (kGroup >= 16)
             group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x140, 0xF, 0xF, false)));
-        }
         if (lane % kGroup == 0) group_max[tid / kGroup] = group;
         __syncthreads();
         group = group_max[lane];
@@ -137,11 +137,14 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
 
     unsigned limit = 0xffffu;   // the last column that an equal to the border may have
     if (top > 0) {
+        // (Not below the border's value, so that NaN passes; the words of the chunks
+        // are compared by their order.)
+        const auto least = _Float16(value_of(border));
         auto collect = [&]() {
 #pragma unroll
             for (int i = 0; i < CPT; ++i) {
                 keep_packed(raw[i]);
-                if (own >= border && order_of(max_of(raw[i])) >= border) {
+                if (own >= border && !(max_of(raw[i]) < least)) {
                     const int at = atomicAdd(&counts[0], 1);
                     if (at < kChunkList) {
                         list[at] = raw[i];
@@ -356,9 +359,11 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
     // A wave a row while it holds at most 4 chunks a lane (8,192 rows of 997 words:
     // 10.3 us, and 21.8 with 256 threads), else 256 threads, or 1,024 where the rows
     // leave CUs idle and are long (16 rows of 50,257 words and 5 alternatives: 8.7
-    // us, and 13.0 with 256; 1,024 rows the other way 33 and 24).
+    // us, and 13.0 with 256; 1,024 rows the other way 33 and 24), or 512 up to 4
+    // rows a CU, which hold more of them at once so (512 rows 16.1 us, and 17.9 with
+    // 256; 8,192 rows without alternatives the other way 168 and 149).
     const size_t held = (vocab + 7) / 8;
-    const bool few = rows <= 256 && held > 1024;
+    const bool few = rows <= 256 && held > 1024, some = rows <= 1024 && held > 4096;
     for (size_t done = 0; done < rows;) {
         const size_t n = std::min<size_t>(rows - done, size_t{1} << 22);
 #define FLINT_LP(TAKE, THREADS, CPT)                                                            \
@@ -379,6 +384,8 @@ hipError_t launch_logprobs_forward(void* logprob, void* entropy, void* stats, vo
         else FLINT_LP(few, 1024, 4);
         else FLINT_LP(few, 1024, 7);
         else FLINT_LP(few, 1024, 8);
+        else FLINT_LP(some, 512, 13);
+        else FLINT_LP(some, 512, 16);
         else FLINT_LP(true, 256, 2);
         else FLINT_LP(true, 256, 4);
         else FLINT_LP(true, 256, 8);

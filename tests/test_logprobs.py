@@ -160,6 +160,14 @@ def test_many_rows_of_long_ones(flint, cuda, vocab, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,top", [(33000, 7), (51208, 3)])
+def test_more_long_rows_than_four_a_compute_unit(flint, cuda, vocab, top):
+    r = Rows(cuda, 1026, vocab, vocab, top, seed=vocab)
+    r.logits[1020] = -2.0
+    check(r.run(flint), r.reference())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vocab", [900, 20000])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "lowest", "masked", "ramp", "ends"])
 def test_ties_and_masks(flint, cuda, kind, vocab):
