@@ -450,7 +450,7 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged_few(Paged
                 for (int e = 0; e < 8; ++e) v[e] = _Float16(sum[d + e] * inv);
                 *reinterpret_cast<f16x8*>(o + d) = v;
             }
-        } else {
+        } else if (it.slot + it.part < a.slots) {
             const size_t at = (size_t(it.slot + it.part) * a.kv_heads + head) * a.rows + row;
             if (d0 == 0) a.sums[at] = float2{m, l};
 #pragma unroll
@@ -553,7 +553,8 @@ __global__ void __launch_bounds__(kThreads * kGroups, HD == 64 ? 4 : 2) paged_ma
         });
         return;
     }
-    if (turn != 0 || first_row + fr >= rows) return;
+    // (Offsets that decrease can make more blocks, and parts, than there are slots.)
+    if (turn != 0 || first_row + fr >= rows || it.slot + it.part >= a.slots) return;
     const size_t slot =
         (size_t(it.slot + it.part) * a.kv_heads + head) * a.rows + wave * 32 + fr;
     if (h == 0) a.sums[slot] = float2{w.m, w.l};

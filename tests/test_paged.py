@@ -293,6 +293,20 @@ def test_offsets_that_decrease_stay_inside(flint, cuda, new):
 
 
 @pytest.mark.gpu
+def test_offsets_that_decrease_stay_inside_the_workspace(flint, cuda):
+    """Five times the same 100 tokens: 60 parts, where 48 is the most."""
+    c = Cache([700] * 10, [10] * 10, 3, 1, 64, 16, seed=32, max_new=100)
+    r = Run(flint, cuda, c)
+    need = flint.attention_paged_workspace(r.shape)
+    r.ws = torch.full((need + (1 << 20),), 0x5A, dtype=torch.uint8, device=cuda)
+    r.offsets = torch.tensor([0, 100] * 5 + [0], dtype=torch.int32, device=cuda)
+    flint.attention_paged(r.o, r.k_pages, r.v_pages, r.q, r.k, r.v, r.offsets, r.cached, r.table,
+                          r.shape, c.scale, r.ws, workspace_bytes=need)
+    torch.cuda.synchronize()
+    assert torch.all(r.ws[need:] == 0x5A)
+
+
+@pytest.mark.gpu
 def test_two_runs_are_bit_identical(flint, cuda):
     c = Cache([3000, 100, 800], [1, 1, 1], 8, 2, 128, 16, seed=16)
     one, two = Run(flint, cuda, c).run().o, Run(flint, cuda, c).run().o
