@@ -57,12 +57,16 @@ __device__ __forceinline__ void keep_packed(h8& v) { asm volatile("" : "+v"(v));
 // 7 VALU slots a word against 2 bytes. 8,192 rows of 50,257 words: 133 to 149 us
 // on different cards, 5.5 to 6.2 TB/s; with 5 alternatives 170.
 //
-// Alternatives: the row falls into 64 groups of threads. The top-th largest of
-// the groups' maxima is a border that at least `top` words reach, and few more
-// do (about top (1 + top / 128) of words in no order); the chunks holding them
-// go to a list in LDS, from there the words, and a word's place in the answer
-// is the number of listed words before it. The groups' maxima are a step of the
-// row's maximum anyway.
+// Alternatives: the row falls into 64 groups of threads, or 256 where many are
+// asked (a wave that has a row of its own: into its chunks). The top-th largest of
+// the n groups' maxima is a border that at least `top` words reach, and few more
+// do: about n ln(n / (n - top)) of words in no order. The chunks holding them go
+// to a list in LDS, from there the words, and a word's place in the answer is the
+// number of listed words before it. The 64 groups' maxima are a step of the row's
+// maximum anyway (16 rows of 50,257 words and 33 alternatives: 9.4 us, and 10.1
+// with 256), but 64 of 64 are 270 words on average, and past the list in 1 row of
+// 50: 64 rows took 193 us so, 11 with 256.
+constexpr int kFewTop = 40;
 template <int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS)
 logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
@@ -70,7 +74,7 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
                  float* __restrict__ top_logprobs, const h8* __restrict__ logits,
                  const uint16_t* __restrict__ targets, float scale, int vocab, int chunks, int top) {
     constexpr int kWaves = THREADS / 64;
-    __shared__ unsigned group_max[64];
+    __shared__ unsigned group_max[64], fine_max[256];
     __shared__ __attribute__((aligned(16))) h8 list[kChunkList];
     __shared__ int list_chunk[kChunkList];
     __shared__ unsigned words[kWordList];
@@ -110,9 +114,13 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
     const unsigned own = order_of(max_of(m8));
     unsigned group = own;
     if constexpr (THREADS > 64) {   // groups of THREADS / 64 neighbouring lanes
-        constexpr int kGroup = THREADS / 64;
+        constexpr int kGroup = THREADS / 64, kFine = THREADS / 256;
+        const bool fine = top > kFewTop && lane % kFine == 0;
+        if (kFine == 1 && fine) fine_max[tid] = group;
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0xB1, 0xF, 0xF, false)));
+        if (kFine == 2 && fine) fine_max[tid / 2] = group;
         group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x4E, 0xF, 0xF, false)));
+        if (kFine == 4 && fine) fine_max[tid / 4] = group;
         if constexpr (kGroup >= 8)
             group = max(group, unsigned(__builtin_amdgcn_update_dpp(0, int(group), 0x141, 0xF, 0xF, false)));
         if constexpr (kGroup >= 16)
@@ -124,11 +132,28 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
         __syncthreads();
     }
     unsigned border = 0;
-    const int wanted = max(top, 1);
+    constexpr int kFineOfLane = THREADS > 64 ? 4 : CPT;   // (one wave: its chunks)
+    if (kFineOfLane > 1 && top > kFewTop) {
+        unsigned f[kFineOfLane];
 #pragma unroll
-    for (int bit = 15; bit >= 0; --bit) {
-        const unsigned higher = border | 1u << bit;
-        if (__popcll(__ballot(group >= higher)) >= wanted) border = higher;
+        for (int k = 0; k < kFineOfLane; ++k) {
+            if constexpr (THREADS > 64) f[k] = fine_max[lane + 64 * k];
+            else f[k] = order_of(max_of(raw[k]));
+        }
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned higher = border | 1u << bit;
+            int n = 0;
+#pragma unroll
+            for (int k = 0; k < kFineOfLane; ++k) n += __popcll(__ballot(f[k] >= higher));
+            if (n >= top) border = higher;
+        }
+    } else {
+        const int wanted = max(top, 1);
+#pragma unroll
+        for (int bit = 15; bit >= 0; --bit) {
+            const unsigned higher = border | 1u << bit;
+            if (__popcll(__ballot(group >= higher)) >= wanted) border = higher;
+        }
     }
     unsigned top_order = group;
 #pragma unroll

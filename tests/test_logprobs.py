@@ -168,6 +168,17 @@ def test_more_long_rows_than_four_a_compute_unit(flint, cuda, vocab, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [500, 1000, 2000, 9000, 50257])
+@pytest.mark.parametrize("top", [40, 41, 64])
+def test_many_alternatives(flint, cuda, vocab, top):
+    """On both sides of the finer groups, for each size of workgroup."""
+    r = Rows(cuda, 40, vocab, (vocab + 7) // 8 * 8, top, seed=vocab + top)
+    r.logits[3, 50:] = float("-inf")
+    r.targets[3] = 49
+    check(r.run(flint), r.reference())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vocab", [900, 20000])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "lowest", "masked", "ramp", "ends"])
 def test_ties_and_masks(flint, cuda, kind, vocab):
