@@ -22,7 +22,8 @@ constexpr int kThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.69314718055994531f;
 // Chunks (of 8 columns) and words that may hold an alternative, as LDS keeps
-// them. Rows with more (many equal logits) find the exact border first.
+// them. Rows with more take the words above the border and then the first of those
+// at it, or find the exact border first.
 constexpr int kChunkList = 512, kWordList = 512;
 
 // The place of an FP16 value among all values: -0 with +0, NaN above +inf.
@@ -190,7 +191,62 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
             __syncthreads();
         };
         collect();
-        if (counts[0] > kChunkList || counts[1] > kWordList) {
+        bool full = counts[0] > kChunkList || counts[1] > kWordList;
+        if (full) {
+            // Many words equal to the border (a mask that leaves fewer than are
+            // asked, say): the words above it, then the lowest columns of those at
+            // it, a slice of THREADS chunks at a time until there are enough. (64
+            // rows of 50,257 words with 3 left take 14 us so, 192 by halving.)
+            __syncthreads();
+            if (tid < 2) counts[tid] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < CPT; ++i) {
+                keep_packed(raw[i]);
+                if (order_of(max_of(raw[i])) <= border) continue;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const unsigned order = order_of(raw[i][j]);
+                    if (order <= border) continue;
+                    const int at = atomicAdd(&counts[1], 1);
+                    if (at < kWordList)
+                        words[at] = order << 16 | (0xffffu - unsigned((tid + i * THREADS) * 8 + j));
+                }
+            }
+            __syncthreads();
+            int have = counts[1];
+            full = have > kWordList;
+            if (!full && have < top) {
+#pragma unroll
+                for (int i = 0; i < CPT; ++i) {
+                    if (have >= top) continue;   // for all threads alike
+                    const int first = (tid + i * THREADS) * 8;
+                    unsigned equal = 0;   // bit j: word j of the chunk
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        equal |= unsigned(order_of(raw[i][j]) == border && first + j < vocab) << j;
+                    int upto = __popc(equal);
+#pragma unroll
+                    for (int d = 1; d < 64; d *= 2) {
+                        const int v = __shfl_up(upto, d);
+                        upto += lane >= d ? v : 0;
+                    }
+                    if (lane == 63) red_count[wave] = upto;
+                    __syncthreads();
+                    int at = have + upto - __popc(equal);
+                    for (int w = 0; w < kWaves; ++w) {
+                        at += w < wave ? red_count[w] : 0;
+                        have += red_count[w];
+                    }
+                    for (; equal != 0 && at < top; equal &= equal - 1, ++at)
+                        words[at] = border << 16 | (0xffffu - unsigned(first + __ffs(equal) - 1));
+                    __syncthreads();
+                }
+                if (tid == 0) counts[1] = top;
+                __syncthreads();
+            }
+        }
+        if (full) {
             // The exact border by halving: the value, then among the words of
             // that value the column, counting over the whole row each time. (What
             // pads the row is -inf behind its last column: after every word.)

@@ -179,6 +179,31 @@ def test_many_alternatives(flint, cuda, vocab, top):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab,period", [(50257, 1024), (2000, 64), (12000, 256)])
+def test_largest_words_close_together(flint, cuda, vocab, period):
+    """The largest words in half the threads' columns: the groups' maxima say
+    little, and more words pass the border than are listed."""
+    r = Rows(cuda, 4, vocab, (vocab + 7) // 8 * 8, 40, seed=vocab)
+    chunk = torch.arange(r.cols) // 8 % period
+    r.logits[:, chunk >= period // 2] -= 30
+    check(r.run(flint), r.reference())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("left", [1, 3, 39])
+@pytest.mark.parametrize("vocab", [997, 9000, 50257])
+def test_a_mask_that_leaves_fewer_words_than_asked(flint, cuda, left, vocab):
+    r = Rows(cuda, 5, vocab, (vocab + 7) // 8 * 8, 40, seed=vocab + left)
+    keep = torch.randperm(vocab, generator=torch.Generator().manual_seed(left))[:left]
+    masked = torch.full_like(r.logits, float("-inf"))
+    masked[:, keep] = r.logits[:, keep]
+    masked[4, :] = -1.0
+    r.logits[:] = masked
+    r.targets[:] = int(keep[0])
+    check(r.run(flint), r.reference())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("vocab", [900, 20000])
 @pytest.mark.parametrize("kind", ["equal", "zeros", "few values", "lowest", "masked", "ramp", "ends"])
 def test_ties_and_masks(flint, cuda, kind, vocab):
