@@ -191,6 +191,15 @@ struct Strides {
     int q, kv, o;
 };
 
+// Whether a wave of the 32 queries from q0 on leaves the tile of keys from kbase on
+// out: every key after every query, or no query in the sequence. What it takes is
+// a tile that was loaded: kbase is a multiple of 64 and q0 of 32, so kbase is in the
+// tile of q0 or before. (Past the sequence a turn may have no tile at all, and LDS
+// holds what was there before: not a number, mostly.)
+__device__ __forceinline__ bool unseen(int kbase, int q0, int length) {
+    return kbase > q0 + 31 || q0 >= length;
+}
+
 // The backward kernels form 2^kUp P and with it 2^kUp dS, and take the factor
 // out of their sums again: over thousands of keys, or from a small dO, dS is
 // often below FP16's normal values (one head over 3,000 tokens, dO of 0.01: dQ
@@ -298,7 +307,7 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         const _Float16* vt = kt + kTile;
         if (i + 1 < steps) load(i + 1);
         const int kbase = 64 * (G * i + turn);
-        if (kbase > q0 + 31) continue;          // every key after every query of the wave
+        if (unseen(kbase, q0, length)) continue;
         // Scores are scaled by c inside the exponent's FMA; where the tile holds
         // keys after a query (a uniform branch), before it, and masked.
         auto scores = [&](f32x16 (&s)[2], unsigned zero) __attribute__((always_inline)) {
@@ -463,7 +472,7 @@ packed_backward_dq(_Float16* __restrict__ dq, float* __restrict__ dsum,
             const _Float16* vt = kt + kTile;
             if (i + 1 < steps) load(i + 1);
             const int kbase = 64 * (G * i + turn);
-            if (kbase > q0 + 31) continue;
+            if (unseen(kbase, q0, length)) continue;
             const bool masked = kbase + 63 > q0;
             // Two halves of 32 keys, each through all of its products before the
             // next (fewer registers live at once).
