@@ -405,28 +405,43 @@ logprobs_backward(h8* dlogits, const float* __restrict__ dlogprob,
 #pragma unroll
     for (int k = 0; k < kAhead; ++k)
         if (c0 + k * kThreads < chunks) l[k] = from[c0 + k * kThreads];
+    auto logprob_of = [&](_Float16 v) { return __builtin_fmaf(scale, float(v) - mx, -log_sum); };
+    auto by_probability = [&](float lp, float by) {   // -p (by + dH (log p + H))
+        return -__builtin_amdgcn_exp2f(lp * kLog2e) * __builtin_fmaf(dh, fmaxf(lp, -1e4f) + ent, by);
+    };
+    // The target's, by the thread that has it: 1 - p as -expm1(log p). Of a word
+    // that takes most of its row, the difference of 1 and p keeps the rounding of p
+    // (2^-24 of 1) and little else: at log p = -1e-6 it is 10% off.
+    float d_target = 0.0f;
+    const int ahead = (t >> 3) - c0;
+    if (t < vocab && ahead >= 0 && ahead % kThreads == 0 && ahead < kThreads * kAhead) {
+        _Float16 v{};
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (ahead == k * kThreads && (t & 7) == i) v = l[k][i];
+        const float lp = logprob_of(v);
+        d_target = __builtin_fmaf(-dlp, expm1f(lp), by_probability(lp, 0.0f));
+    }
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
         const int c = c0 + k * kThreads;
         if (c >= chunks) break;
         float d[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float lp = __builtin_fmaf(scale, float(l[k][i]) - mx, -log_sum);
-            const float p = __builtin_amdgcn_exp2f(lp * kLog2e);
-            d[i] = -scale * p * __builtin_fmaf(dh, fmaxf(lp, -1e4f) + ent, dlp);
-        }
+        for (int i = 0; i < 8; ++i) d[i] = by_probability(logprob_of(l[k][i]), dlp);
         if (c == t >> 3 || c == (vocab - 1) >> 3 || c > (vocab - 1) >> 3) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int j = 8 * c + i;
-                if (j == t) d[i] += scale * dlp;
+                if (j == t) d[i] = d_target;
                 if (j >= vocab) d[i] = 0.0f;
             }
         }
         h8 out;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = _Float16(d[i]);
+        for (int i = 0; i < 8; ++i) out[i] = _Float16(scale * d[i]);
         store_stream(to + c, out);
     }
 }

@@ -254,6 +254,29 @@ def test_peaked_rows_keep_their_small_values(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [1000, 30000])
+def test_peaked_rows_keep_their_gradient(flint, cuda, vocab):
+    """dlogprob (1 - p) at a target of probability near 1, right relative to
+    itself: log p's relative error, two steps of FP32 for 1 - p, and FP16's."""
+    r = Rows(cuda, 7, vocab, vocab, 0, seed=18, spread=0.5)
+    lead = torch.tensor([8.0, 12.0, 16.0, 18.0, 20.0, 24.0, 30.0]) + math.log(vocab / 1000)
+    r.logits[torch.arange(7), r.targets] = lead.half()
+    r.dlp[:] = 6e4 * torch.tensor([1.0, -1.0, 1.0, 1.0, -1.0, 1.0, 1.0])
+    got, ref = r.run(flint, entropy_gradient=False), r.reference(entropy_gradient=False)
+    check(got, ref)
+    at = torch.arange(7), r.targets
+    # 1 - p from the sum of the others' exponentials: float64 keeps it whole.
+    others = r.logits.double()
+    others = torch.exp(others - others[at][:, None])
+    others[at] = 0.0
+    others = others.sum(1)
+    want = r.dlp.double() * others / (1 + others)
+    bound = ((10 * lead.double() + 1110) * W + U) * want.abs() + Z
+    off = (got["d"][at].double() - want).abs()
+    assert bool((off <= bound).all()), off / bound
+
+
+@pytest.mark.gpu
 def test_not_a_number_and_infinity(flint, cuda):
     r = Rows(cuda, 5, 700, 704, 4, seed=9)
     r.logits[1, 13] = float("nan")
