@@ -318,8 +318,12 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
     // e = 2^(x - mx c), c = scale log2 e: one fma of the exact product, and the
     // rounding of mx c (common to every word) put right in the sums below.
     // -1e4 keeps words of probability 0 out of 0 x inf.
-    const float c = scale * kLog2e, shift = mx * c;
-    const float off = __builtin_fmaf(mx, c, -shift);
+    // Large scales: FP16 values are 2^-24 apart at least, so from c = 2^32 on every
+    // e is 0, and c stops at 2^40, where mx c is finite. Values next to mx differ
+    // from it by 2^-11 of its size at least and `off` is at most 2^-24 of mx c, so
+    // where off passes 1 every e is 0 too, and off stops there: 2^-off is finite.
+    const float c = fminf(scale * kLog2e, 0x1p40f), shift = mx * c;
+    const float off = fminf(fmaxf(__builtin_fmaf(mx, c, -shift), -1.0f), 1.0f);
     float rest = 0.0f, weighted = 0.0f;
 #pragma unroll
     for (int i = 0; i < CPT; ++i) {

@@ -142,6 +142,30 @@ def test_scales(flint, cuda, scale, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e5, 1e8, 1e9, 1e30, 3e38])
+@pytest.mark.parametrize("vocab", [300, 12000])
+def test_scales_that_leave_the_largest_words_alone(flint, cuda, vocab, scale):
+    """1 / scale is a temperature near 0: one word, or equal ones, take the row.
+    What passes FP32 (a log probability) or FP16 (a gradient) is infinite."""
+    r = Rows(cuda, 60, vocab, vocab + 8 - vocab % 8, 10, seed=vocab, scale=scale)
+    r.logits[20:40] -= 40                   # negative maxima
+    r.logits[40:45] *= 1e-3                 # around 0, close together
+    r.logits[45] = 0.0
+    r.logits[46] = -65504.0
+    r.logits[47] = 65504.0
+    r.logits[48, 7] = r.logits[48, 90] = 30.0
+    r.logits[49, 5:] = float("-inf")
+    r.dh[:] = 0.0       # of equal words log p + entropy is 0, and scale times float64's roundings
+    r.targets[:10] = r.logits[:10, :vocab].float().argmax(1)
+    r.targets[48], r.targets[49] = 90, 2
+    got, ref = r.run(flint), r.reference()
+    for name, kind in (("logprob", torch.float32), ("values", torch.float32), ("d", torch.float16)):
+        past = ref[name].abs() > torch.finfo(kind).max
+        ref[name] = torch.where(past, ref[name] * math.inf, ref[name])
+    check(got, ref)
+
+
+@pytest.mark.gpu
 def test_many_rows(flint, cuda):
     r = Rows(cuda, 3001, 250, 256, 5, seed=5)
     check(r.run(flint), r.reference())
