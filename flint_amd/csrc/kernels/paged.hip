@@ -596,12 +596,16 @@ struct Parts {
 __device__ __forceinline__ bool parts_of_row(const PagedArgs& a, const Sequence& q, int2 split,
                                              int t, int head, Parts* p) {
     const int kv = head / a.group, row = (t - q.first) * a.group + head - kv * a.group;
-    const int block = row / a.rows, first = split.x + block * split.y;
+    // Offsets that decrease make more blocks than the grid has workgroups. A
+    // sequence that got none has what lay in the workspace as its split: any two
+    // numbers, so the parts are looked for in 64 bits, inside the slots alone.
+    const int block = row / a.rows;
+    const long long first = split.x + (long long)(block) * split.y;
+    if (split.y <= 1 || split.y > a.slots || first < 0 || first > a.slots - split.y) return false;
     p->step = size_t(a.kv_heads) * a.rows;
     p->at = (size_t(first) * a.kv_heads + kv) * a.rows + (row - block * a.rows);
     p->count = split.y;
-    // Slots outside the workspace can come from offsets that decrease only.
-    return split.y > 1 && first >= 0 && first + split.y <= a.slots;
+    return true;
 }
 
 // The parts' results, weighted by their maxima's distance; HD / 4 lanes (a set)

@@ -24,7 +24,8 @@
  *     not seen, and new rows that would go there are not stored (they are still
  *     seen by this call's tokens);
  *   - positions past max_pages x page_size have no page either; cached[s] is
- *     taken into 0 .. max_pages x page_size, offsets into 0 .. tokens;
+ *     taken into 0 .. max_pages x page_size, offsets into 0 .. tokens (where
+ *     they decrease, any row of o may hold anything);
  *   - new tokens of a sequence past max_new are ignored, their rows of o left.
  * Rows of o outside every sequence stay as they were. Pages may be shared by
  * sequences as long as no call stores into a row that another sequence of the

@@ -307,6 +307,30 @@ def test_offsets_that_decrease_stay_inside_the_workspace(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("word", [0x3F800000, 0x00000002, 0x7FFFFFFF])
+def test_offsets_that_decrease_past_the_grid_join_inside_the_workspace(flint, cuda, word):
+    """3,968 blocks a head of K and V for 1,014 workgroups: the last sequence gets
+    none, so its entry in the workspace is the word that lay there."""
+    heads, S, n = 64, 999, 1000
+    qkv = normal((n, 3 * heads * 64), 35, 1.0, torch.float16).to(cuda)
+    q, k, v = (qkv[:, i * heads * 64:(i + 1) * heads * 64] for i in range(3))
+    pages = torch.zeros((2, 70, heads, 16, 64), dtype=torch.float16, device=cuda)
+    table = torch.arange(70, dtype=torch.int32, device=cuda).repeat(S, 1)
+    shape = flint.paged_shape(n, S, n, heads, heads, 64, *[qkv.shape[1]] * 2, heads * 64, 70, 16, 70)
+    offsets = torch.tensor([0, n] * 496 + [0] * 7 + [n], dtype=torch.int32, device=cuda)
+    need = flint.attention_paged_workspace(shape)
+    assert need > 0
+    ws = torch.full((need // 4 + (1 << 18),), word, dtype=torch.int32, device=cuda)
+    o = torch.full((n + 8, heads * 64), SENTINEL, dtype=torch.float16, device=cuda)
+    flint.attention_paged(o, pages[0], pages[1], q, k, v, offsets,
+                          torch.zeros(S, dtype=torch.int32, device=cuda), table, shape, 0.125, ws,
+                          workspace_bytes=need)
+    torch.cuda.synchronize()
+    assert torch.all(ws[need // 4:] == word)
+    assert torch.all(o[n:] == SENTINEL)
+
+
+@pytest.mark.gpu
 def test_two_runs_are_bit_identical(flint, cuda):
     c = Cache([3000, 100, 800], [1, 1, 1], 8, 2, 128, 16, seed=16)
     one, two = Run(flint, cuda, c).run().o, Run(flint, cuda, c).run().o
