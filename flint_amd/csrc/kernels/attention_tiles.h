@@ -171,6 +171,11 @@ constexpr float kFloor = -3e38f;
 // What a lane's probabilities of a tile may add up to before the running
 // maximum is moved: none of them is above it then, and FP16 holds 2^16.
 constexpr float kSumLimit = 32768.0f;
+// How far below a tile's maximum the reference lies, in log2 units: the largest
+// probability is 2^8, so that those down to 2^-33 of it stay above 0 in FP16. (At
+// 1 the 130,000 keys at 2^-25.5 beside one were in the sum l and 0 in the product
+// with V: 0.3% of o.) A lane's 32 add up to 2^13 at most.
+constexpr float kBelow = 8.0f, kBelowFactor = 0x1p-8f;
 
 // P = 2^(ce s - m) as FP16, and the FP32 sum of this lane's (its half of the
 // keys).
@@ -192,9 +197,9 @@ __device__ __forceinline__ float exponentials(f16x8 (&p)[2 * HB], const f32x16 (
 // A tile's probabilities and their sum. m, a query's reference in log2 units,
 // need not be its maximum: O and l share it, and it only has to keep P inside
 // FP16. So past the wave's first tile (started) the tile's maximum is not taken
-// unless the sum passes kSumLimit, or overflows, for some query; then m moves
-// to the maximum, rescale(2^(m_old - m_new)) is called and the tile is taken
-// again (scores() gives s and ce once more, so that no register holds s
+// unless the sum passes kSumLimit, or overflows, for some query; then m moves to
+// kBelow under the maximum, rescale(2^(m_old - m_new)) is called and the tile is
+// taken again (scores() gives s and ce once more, so that no register holds s
 // meanwhile).
 // (scores uses an offset of 0 that the compiler cannot see through: otherwise it
 // moves the products and the masks out of the loop and keeps them after all.)
@@ -215,7 +220,7 @@ __device__ __forceinline__ float probabilities(f16x8 (&p)[2 * HB], const Scores&
 #pragma unroll
                 for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[hb][r]);
             mx *= ce;
-            const float m_new = fmaxf(*m, fmaxf(mx, xor32(mx)));
+            const float m_new = fmaxf(*m, fmaxf(mx, xor32(mx)) - kBelow);
             rescale(__builtin_amdgcn_exp2f(*m - m_new));
             *m = m_new;
         }

@@ -381,7 +381,8 @@ packed_forward(_Float16* __restrict__ out, float* __restrict__ lse, const _Float
         }
         write_rows<HD>(rows, acc, 1.0f / l, wave * 32 + fr, h);
         if (qi < length && h == 0)
-            lse[size_t(w.head) * tokens + w.begin + qi] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+            lse[size_t(w.head) * tokens + w.begin + qi] =
+                (m + kBelow + __builtin_amdgcn_logf(l * kBelowFactor)) * kLn2;
     }
     __syncthreads();
     copy_rows<HD, threads_of(kForwardTurns)>(rows, length - row0, [&](int row) {

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from attention_bounds import attend, causal, worst
+from attention_bounds import Z, attend, causal, worst
 from flint_amd import flint_lib
 from inputs import normal
 
@@ -182,6 +182,26 @@ def test_large_scores(flint, cuda):
     b = Batch([300], 1, 1, 64, seed=14, scale=1.0)
     b.qkv[:, :128] *= 4.0
     check(Run(flint, cuda, b).run(backward=False), names=("o", "lse"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 128])
+def test_a_key_that_outweighs_the_others_by_far(flint, cuda, width):
+    """The first key is 2^25 to 2^29 times as likely as each other one and its
+    value is 0: o is what the others add up to. Probabilities are rounded at 2^8
+    times their size, so half a step among FP16's subnormals is 2^-33."""
+    b = Batch([600, 90], 2, 1, width, seed=35, scale=8.0 / width)   # scores: 8 k
+    q, k, v = b.parts(b.qkv)
+    q[:] = 1.0
+    k[:] = -0.3 * torch.rand(k.shape[0], 1, generator=torch.Generator().manual_seed(36))
+    v[:] = 64.0
+    for first in b.offsets[:-1]:
+        k[first], v[first] = 2.21, 0.0
+    ref = b.reference(backward=False)
+    for first, end in zip(b.offsets, b.offsets[1:]):
+        reach = v[first:end].double().cumsum(0).repeat(1, 2)
+        ref["o"][1][first:end] -= 1.05 * (Z - 2.0 ** -33) * reach
+    check(Run(flint, cuda, b).run(backward=False), names=("o", "lse"), reference=ref)
 
 
 @pytest.mark.gpu

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from attention_bounds import attend, worst
+from attention_bounds import Z, attend, worst
 from flint_amd import flint_lib
 from inputs import gen, normal
 
@@ -236,6 +236,26 @@ def test_a_shared_prefix(flint, cuda):
 @pytest.mark.parametrize("scale", [-0.2, 0.0, 1.0])
 def test_any_finite_scale(flint, cuda, scale):
     check(Run(flint, cuda, Cache([300, 10], [1, 40], 2, 1, 64, 16, seed=12, scale=scale)).run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("width", [64, 128])
+@pytest.mark.parametrize("new", [1, 40])
+def test_a_key_that_outweighs_the_others_by_far(flint, cuda, new, width):
+    """The first key is 2^25 to 2^29 times as likely as each other one and its
+    value is 0: o is what the others add up to. Probabilities are rounded at 2^8
+    times their size, so half a step among FP16's subnormals is 2^-33."""
+    c = Cache([600], [new], 1, 1, width, 64, seed=33, scale=8.0 / width)   # scores: 8 k
+    spread = torch.rand(600 + new, generator=gen(34)) * -0.3
+    spread[0] = 2.21
+    q, k, v = c.parts(c.qkv)
+    q[:], k[:], v[:] = 1.0, spread[600:, None], 64.0
+    for p in range(600):
+        c.k_pages[c.page(0, p), :, p % 64] = spread[p]
+        c.v_pages[c.page(0, p), :, p % 64] = 64.0 if p else 0.0
+    o, bound, kp, vp, done = c.reference()
+    reach = 64.0 * torch.arange(600, 600 + new, dtype=torch.float64)[:, None]
+    check(Run(flint, cuda, c).run(), (o, bound - 1.05 * (Z - 2.0 ** -33) * reach, kp, vp, done))
 
 
 @pytest.mark.gpu
