@@ -172,10 +172,14 @@ constexpr float kFloor = -3e38f;
 // maximum is moved: none of them is above it then, and FP16 holds 2^16.
 constexpr float kSumLimit = 32768.0f;
 // How far below a tile's maximum the reference lies, in log2 units: the largest
-// probability is 2^8, so that those down to 2^-33 of it stay above 0 in FP16. (At
-// 1 the 130,000 keys at 2^-25.5 beside one were in the sum l and 0 in the product
-// with V: 0.3% of o.) A lane's 32 add up to 2^13 at most.
-constexpr float kBelow = 8.0f, kBelowFactor = 0x1p-8f;
+// probability is 2^5, so that those down to 2^-30 of it stay above 0 in FP16. (At
+// 1 the keys under 2^-25 of a row's largest are in the sum l and 0 in the product
+// with V: 0.3% of o where 130,000 are at 2^-25.5; at 2^5 so many lose 2^-13, a
+// quarter of o's own rounding.) A lane's 32 add up to 2^10 at most. What it costs is
+// moves where scores spread wide: 16,384 tokens, scores of deviation 1, 2, 4 and 8
+// take 355, 355, 372 and 396 us; at 1 352, 355, 356 and 367, at 2^8 353, 361, 389
+// and 418.
+constexpr float kBelow = 5.0f, kBelowFactor = 0x1p-5f;
 
 // P = 2^(ce s - m) as FP16, and the FP32 sum of this lane's (its half of the
 // keys).

@@ -242,20 +242,21 @@ def test_any_finite_scale(flint, cuda, scale):
 @pytest.mark.parametrize("width", [64, 128])
 @pytest.mark.parametrize("new", [1, 40])
 def test_a_key_that_outweighs_the_others_by_far(flint, cuda, new, width):
-    """The first key is 2^25 to 2^29 times as likely as each other one and its
-    value is 0: o is what the others add up to. Probabilities are rounded at 2^8
-    times their size, so half a step among FP16's subnormals is 2^-33."""
-    c = Cache([600], [new], 1, 1, width, 64, seed=33, scale=8.0 / width)   # scores: 8 k
-    spread = torch.rand(600 + new, generator=gen(34)) * -0.3
+    """The first key is 2^25 to 2^27 times as likely as each other one and its
+    value is 0: o is what the others add up to. Probabilities are rounded at 2^5
+    times their size, so half a step among FP16's subnormals is 2^-30."""
+    n = 250
+    c = Cache([n], [new], 1, 1, width, 64, seed=33, scale=8.0 / width)   # scores: 8 k
+    spread = torch.rand(n + new, generator=gen(34)) * -0.09
     spread[0] = 2.21
     q, k, v = c.parts(c.qkv)
-    q[:], k[:], v[:] = 1.0, spread[600:, None], 64.0
-    for p in range(600):
+    q[:], k[:], v[:] = 1.0, spread[n:, None], 64.0
+    for p in range(n):
         c.k_pages[c.page(0, p), :, p % 64] = spread[p]
         c.v_pages[c.page(0, p), :, p % 64] = 64.0 if p else 0.0
     o, bound, kp, vp, done = c.reference()
-    reach = 64.0 * torch.arange(600, 600 + new, dtype=torch.float64)[:, None]
-    check(Run(flint, cuda, c).run(), (o, bound - 1.05 * (Z - 2.0 ** -33) * reach, kp, vp, done))
+    reach = 64.0 * torch.arange(n, n + new, dtype=torch.float64)[:, None]
+    check(Run(flint, cuda, c).run(), (o, bound - 1.05 * (Z - 2.0 ** -30) * reach, kp, vp, done))
 
 
 @pytest.mark.gpu
