@@ -213,6 +213,21 @@ def library_path():
     return Path(override) if override else LIBRARY
 
 
+def scratch(nbytes, stream=None):
+    """A workspace for one call on `stream`, allocated there: torch hands memory
+    that a call lets go of to the next user of the stream it was allocated on,
+    which is the one that comes after the call's kernels only if it is theirs."""
+    import torch
+
+    make = lambda: torch.empty(max(nbytes, 16), dtype=torch.uint8, device="cuda")  # noqa: E731
+    if stream is None or stream_handle(stream) == stream_handle(None):
+        return make()
+    if isinstance(stream, int):
+        stream = torch.cuda.ExternalStream(stream)
+    with torch.cuda.stream(stream):
+        return make()
+
+
 class Flint:
     """The loaded library with every C signature declared."""
 
@@ -339,9 +354,7 @@ class Flint:
         if workspace is None:
             need = self.gemm_tn_workspace(m, n, k)
             if need:
-                import torch
-
-                workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
+                workspace = scratch(need, stream)
         if workspace_bytes is None:
             workspace_bytes = 0 if workspace is None or isinstance(workspace, int) else (
                 workspace.numel() * workspace.element_size())
@@ -381,11 +394,8 @@ class Flint:
     def attention_backward(self, dq, dk, dv, dout, q, k, v, o, lse, batches, length, head_width,
                            scale, workspace=None, workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            workspace = torch.empty(max(self.attention_backward_workspace(batches, length,
-                                                                          head_width), 16),
-                                    dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.attention_backward_workspace(batches, length, head_width),
+                                stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_attention_backward(
@@ -425,10 +435,7 @@ class Flint:
     def attention_packed_backward(self, dq, dk, dv, dout, q, k, v, o, lse, plan, shape, scale,
                                   workspace=None, workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            workspace = torch.empty(max(self.attention_packed_backward_workspace(shape), 16),
-                                    dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.attention_packed_backward_workspace(shape), stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_attention_packed_backward(
@@ -451,10 +458,7 @@ class Flint:
     def attention_paged(self, o, k_pages, v_pages, q, k, v, offsets, cached, table, shape, scale,
                         workspace=None, workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            workspace = torch.empty(max(self.attention_paged_workspace(shape), 16),
-                                    dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.attention_paged_workspace(shape), stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_attention_paged(
@@ -470,10 +474,7 @@ class Flint:
     def bias_gradient(self, dbias, dy, rows, cols, accumulate=False, workspace=None,
                       workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            workspace = torch.empty(max(self.bias_gradient_workspace(rows, cols), 16),
-                                    dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.bias_gradient_workspace(rows, cols), stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_bias_gradient(pointer(dbias), pointer(dy), rows, cols,
@@ -495,10 +496,7 @@ class Flint:
                            accumulate_dx=False, accumulate_params=False, workspace=None,
                            workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            workspace = torch.empty(max(self.layernorm_backward_workspace(rows, cols), 16),
-                                    dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.layernorm_backward_workspace(rows, cols), stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_layernorm_backward(
@@ -568,10 +566,8 @@ class Flint:
                            accumulate_wte=False, accumulate_wpe=False, workspace=None,
                            workspace_bytes=None, stream=None):
         if workspace is None:
-            import torch
-
-            need = self.embedding_backward_workspace(sequences, length, vocab, width)
-            workspace = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+            workspace = scratch(self.embedding_backward_workspace(sequences, length, vocab, width),
+                                stream)
         if workspace_bytes is None:
             workspace_bytes = workspace.numel() * workspace.element_size()
         self.check(self.lib.flint_embedding_backward(
