@@ -36,9 +36,12 @@ Checker& paged_sizes(Checker& c, const flint_paged_shape* s) {
         .require(s->max_pages != 0 && s->max_pages <= columns, "max_pages (%zu) must be from 1 to %zu",
                  s->max_pages, columns);
     if (c.ok())
-        c.require(s->tokens * s->heads <= flint::kPagedMaxRows,
-                  "tokens x heads (%zu) can be up to %zu", s->tokens * s->heads,
-                  flint::kPagedMaxRows)
+        c.require(s->pages <= flint::kPagedMaxPool / (s->page_size * s->kv_heads * s->head_width),
+                  "pages (%zu) x page_size x kv_heads x head_width can be up to %zu", s->pages,
+                  flint::kPagedMaxPool)
+            .require(s->tokens * s->heads <= flint::kPagedMaxRows,
+                     "tokens x heads (%zu) can be up to %zu", s->tokens * s->heads,
+                     flint::kPagedMaxRows)
             .require(s->sequences * s->kv_heads <= flint::kPagedMaxRows / 8,
                      "sequences x kv_heads (%zu) can be up to %zu", s->sequences * s->kv_heads,
                      flint::kPagedMaxRows / 8);

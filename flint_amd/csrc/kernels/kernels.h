@@ -194,6 +194,7 @@ constexpr size_t kPagedMaxTokens = size_t{1} << 20;
 constexpr size_t kPagedMaxSequences = 65535;
 constexpr size_t kPagedMaxPageSize = 65536;
 constexpr size_t kPagedMaxPositions = size_t{1} << 30;
+constexpr size_t kPagedMaxPool = size_t{1} << 46;   // values: all of a device's addresses
 constexpr size_t kPagedMaxRows = size_t{1} << 25;   // workgroups: below 2^32 threads
 size_t paged_workspace(const flint_paged_shape& s);
 hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const void* q,

@@ -52,7 +52,7 @@ typedef struct {
     size_t q_stride;    /* values from a row to the next; multiples of 8 */
     size_t kv_stride;
     size_t o_stride;
-    size_t pages;       /* of k_pages and v_pages, up to 2^31 - 1 */
+    size_t pages;       /* of k_pages and v_pages, up to 2^31 - 1, and 2^46 values in all */
     size_t page_size;   /* positions a page: a multiple of 8 up to 65,536 */
     size_t max_pages;   /* columns of table; max_pages x page_size up to 2^30 */
 } flint_paged_shape;

@@ -455,6 +455,16 @@ def test_buffers_refused(flint):
     fails(flint, fn, *good, None, f, 10 * A, 1 << 24, None, message="shape is null")
 
 
+def test_a_pool_past_the_addresses_is_refused(flint):
+    """Sizes whose bytes pass 2^64: nothing would be left for the overlap checks."""
+    s = shape_of(flint, pages=(1 << 31) - 1, page_size=65536, heads=1024, kv_heads=1024,
+                 head_width=128, q_stride=131072, kv_stride=131072, o_stride=131072, max_pages=1)
+    fails(flint, "flint_attention_paged_workspace", s, ctypes.c_size_t(0),
+          message="pages (2147483647) x page_size x kv_heads x head_width can be up to 70368744177664")
+    s = shape_of(flint, pages=(1 << 31) - 1)
+    assert flint.lib.flint_attention_paged_workspace(s, ctypes.c_size_t(0)) == 0
+
+
 def test_nothing_to_do(flint):
     f = ctypes.c_float(0.125)
     for none in (dict(tokens=0), dict(sequences=0), dict(max_new=0)):
