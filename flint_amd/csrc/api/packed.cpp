@@ -12,6 +12,13 @@ namespace {
 using flint::Checker;
 using flint::View;
 
+Checker& scale_in_range(Checker& c, float scale) {
+    return c
+        .require(std::isfinite(scale), "scale (%g) must be finite", double(scale))
+        .require(std::fabs(scale) <= flint::kAttentionMaxScale, "scale (%g) can be up to %g in size",
+                 double(scale), double(flint::kAttentionMaxScale));
+}
+
 // The shape itself; every later check reads it only once these have passed.
 Checker& packed_sizes(Checker& c, const flint_packed_shape* s) {
     if (!c.require(s != nullptr, "shape is null").ok()) return c;
@@ -93,9 +100,7 @@ FLINT_API flint_status flint_attention_packed_forward(void* o, void* lse, const 
                                                       const flint_packed_shape* shape, float scale,
                                                       flint_stream stream) {
     Checker c("flint_attention_packed_forward");
-    packed_sizes(c, shape).require(std::isfinite(scale), "scale (%g) must be finite",
-                                   double(scale));
-    if (!c.ok() || empty(*shape)) return c.status();
+    if (!scale_in_range(packed_sizes(c, shape), scale).ok() || empty(*shape)) return c.status();
     c.views({o_view("o", o, *shape), lse_view(lse, *shape), q_view("q", q, *shape),
              kv_view("k", k, *shape), kv_view("v", v, *shape), plan_view(plan, *shape)},
             2);
@@ -118,9 +123,7 @@ FLINT_API flint_status flint_attention_packed_backward(
     const void* o, const void* lse, const void* plan, const flint_packed_shape* shape, float scale,
     void* workspace, size_t workspace_bytes, flint_stream stream) {
     Checker c("flint_attention_packed_backward");
-    packed_sizes(c, shape).require(std::isfinite(scale), "scale (%g) must be finite",
-                                   double(scale));
-    if (!c.ok() || empty(*shape)) return c.status();
+    if (!scale_in_range(packed_sizes(c, shape), scale).ok() || empty(*shape)) return c.status();
     const flint_packed_shape& s = *shape;
     const size_t needed = flint::packed_backward_workspace(s);
     c.require(workspace_bytes >= needed, "needs %zu bytes of workspace, given %zu", needed,

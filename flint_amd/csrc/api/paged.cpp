@@ -81,7 +81,10 @@ FLINT_API flint_status flint_attention_paged(void* o, void* k_pages, void* v_pag
                                              void* workspace, size_t workspace_bytes,
                                              flint_stream stream) {
     Checker c("flint_attention_paged");
-    paged_sizes(c, shape).require(std::isfinite(scale), "scale (%g) must be finite", double(scale));
+    paged_sizes(c, shape)
+        .require(std::isfinite(scale), "scale (%g) must be finite", double(scale))
+        .require(std::fabs(scale) <= flint::kAttentionMaxScale, "scale (%g) can be up to %g in size",
+                 double(scale), double(flint::kAttentionMaxScale));
     if (!c.ok() || empty(*shape)) return c.status();
     const flint_paged_shape& s = *shape;
     const size_t needed = flint::paged_workspace(s);

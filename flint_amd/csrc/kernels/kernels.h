@@ -165,6 +165,7 @@ hipError_t launch_attention_backward(void* dq, void* dk, void* dv, const void* d
 constexpr size_t kPackedMaxTokens = size_t{1} << 26;
 constexpr size_t kPackedMaxSequences = size_t{1} << 20;
 constexpr size_t kHeadsMax = 1024;
+constexpr float kAttentionMaxScale = 0x1p64f;   // times log2 e and any q . k finite in FP32
 constexpr size_t kStrideMax = size_t{1} << 23;
 constexpr size_t kPackedMaxBlocks = size_t{1} << 22;   // workgroups of 512: below 2^32 threads
 constexpr int kPackedBlock = 128;

@@ -54,7 +54,10 @@ FLINT_API flint_status flint_attention_packed_plan(void* plan, const void* offse
 /* o[t] = sum over visible t' of softmax(scale q[t] k^T)[t'] v[t'] (RN16 of an
  * FP32 result; probabilities enter the product with v as FP16), and lse[t] =
  * log(sum over visible t' of exp(scale q[t] . k[t'])). plan must be the one of
- * this shape's tokens and sequences. */
+ * this shape's tokens and sequences. scale is up to 2^64 in size. Scores past
+ * 2^25 in size, where FP32 is 4 apart, may give a row NaN; and lse is an FP32
+ * value, which leaves the backward pass's probabilities |lse| 2^-23 of themselves
+ * off. */
 FLINT_API flint_status flint_attention_packed_forward(void* o, void* lse, const void* q,
                                                       const void* k, const void* v,
                                                       const void* plan,

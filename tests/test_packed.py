@@ -185,6 +185,21 @@ def test_large_scores(flint, cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("width", [64, 128])
+def test_scores_of_millions_stay_finite(flint, cuda, width, sign):
+    """Scores around 2^24.9, where FP32 is 2 apart: what weights they give is
+    rounding, but o lies among the values and lse beside the scores."""
+    b = Batch([300, 70], 2, 1, width, seed=37, scale=sign * 1.0)
+    q, k, v = b.parts(b.qkv)
+    q[:], k[:] = 700.0, (2.0 ** 24.9 / (700.0 * width)) * (1 + 1e-3 * k.float()).half()
+    got = Run(flint, cuda, b).run(backward=False).outputs()
+    most = v.float().abs().amax(0).repeat(2) * (1 + 2.0 ** -10)   # P's rounding and o's
+    assert bool((got["o"].float().abs() <= most).all())
+    assert bool((got["lse"] * sign > 2.0 ** 24.8).all() and (got["lse"] * sign < 2.0 ** 25).all())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("width", [64, 128])
 def test_a_key_that_outweighs_the_others_by_far(flint, cuda, width):
     """The first key is 2^25 to 2^27 times as likely as each other one and its
@@ -408,6 +423,16 @@ def test_buffers_refused(flint):
     fails(flint, fn, *good, s, f, 11 * A, 100, None,
           message=f"needs {need.value} bytes of workspace, given 100")
     fails(flint, fn, A, A + 64, *good[2:], s, f, 11 * A, 1 << 20, None, message="dq and dk overlap")
+
+
+@pytest.mark.parametrize("scale", [1e30, -3.4e38, 2.0 ** 64 * 1.001])
+def test_scales_whose_scores_pass_fp32_are_refused(flint, scale):
+    s, f = shape_of(flint), ctypes.c_float(scale)
+    message = f"scale ({f.value:g}) can be up to 1.84467e+19 in size"
+    fails(flint, "flint_attention_packed_forward", *[(i + 1) * A for i in range(6)], s, f, None,
+          message=message)
+    fails(flint, "flint_attention_packed_backward", *[(i + 1) * A for i in range(10)], s, f, 11 * A,
+          1 << 20, None, message=message)
 
 
 def test_column_slices_of_one_tensor_do_not_overlap(flint):

@@ -455,6 +455,13 @@ def test_buffers_refused(flint):
     fails(flint, fn, *good, None, f, 10 * A, 1 << 24, None, message="shape is null")
 
 
+@pytest.mark.parametrize("scale", [1e30, -3.4e38])
+def test_scales_whose_scores_pass_fp32_are_refused(flint, scale):
+    f = ctypes.c_float(scale)
+    fails(flint, "flint_attention_paged", *[(i + 1) * A for i in range(9)], shape_of(flint), f, 10 * A,
+          1 << 24, None, message=f"scale ({f.value:g}) can be up to 1.84467e+19 in size")
+
+
 def test_a_pool_past_the_addresses_is_refused(flint):
     """Sizes whose bytes pass 2^64: nothing would be left for the overlap checks."""
     s = shape_of(flint, pages=(1 << 31) - 1, page_size=65536, heads=1024, kv_heads=1024,
