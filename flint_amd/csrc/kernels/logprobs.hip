@@ -61,12 +61,12 @@ __device__ __forceinline__ void keep_packed(h8& v) { asm volatile("" : "+v"(v));
 // Alternatives: the row falls into 64 groups of threads, or 256 where many are
 // asked (a wave that has a row of its own: into its chunks). The top-th largest of
 // the n groups' maxima is a border that at least `top` words reach, and few more
-// do: about n ln(n / (n - top)) of words in no order. The chunks holding them go
-// to a list in LDS, from there the words, and a word's place in the answer is the
-// number of listed words before it. The 64 groups' maxima are a step of the row's
-// maximum anyway (16 rows of 50,257 words and 33 alternatives: 9.4 us, and 10.1
-// with 256), but 64 of 64 are 270 words on average, and past the list in 1 row of
-// 50: 64 rows took 193 us so, 11 with 256.
+// do: n (1 / (n - top + 1) + ... + 1 / n) on average of words in no order. The
+// chunks holding them go to a list in LDS, from there the words, and a word's place
+// in the answer is the number of listed words before it. The 64 groups' maxima are a
+// step of the row's maximum anyway (16 rows of 50,257 words and 33 alternatives: 9.4
+// us, and 10.1 with 256), but 64 of 64 are 304 words on average, and past the list
+// in 1 row of 50: 64 rows took 193 us so, 11 with 256.
 constexpr int kFewTop = 40;
 template <int THREADS, int CPT>
 __global__ void __launch_bounds__(THREADS)
@@ -161,36 +161,32 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
     for (int d = 32; d > 0; d /= 2) top_order = max(top_order, unsigned(__shfl_xor(int(top_order), d)));
     const float mx = value_of(top_order);
 
-    unsigned limit = 0xffffu;   // the last column that an equal to the border may have
     if (top > 0) {
         // (Not below the border's value, so that NaN passes; the words of the chunks
         // are compared by their order.)
         const auto least = _Float16(value_of(border));
-        auto collect = [&]() {
 #pragma unroll
-            for (int i = 0; i < CPT; ++i) {
-                keep_packed(raw[i]);
-                if (own >= border && !(max_of(raw[i]) < least)) {
-                    const int at = atomicAdd(&counts[0], 1);
-                    if (at < kChunkList) {
-                        list[at] = raw[i];
-                        list_chunk[at] = tid + i * THREADS;
-                    }
+        for (int i = 0; i < CPT; ++i) {
+            keep_packed(raw[i]);
+            if (own >= border && !(max_of(raw[i]) < least)) {
+                const int at = atomicAdd(&counts[0], 1);
+                if (at < kChunkList) {
+                    list[at] = raw[i];
+                    list_chunk[at] = tid + i * THREADS;
                 }
             }
-            __syncthreads();
-            const int n = min(counts[0], kChunkList);
-            for (int e = tid; e < 8 * n; e += THREADS) {
-                const unsigned order = order_of(list[e >> 3][e & 7]);
-                const int column = list_chunk[e >> 3] * 8 + (e & 7);
-                if (column < vocab && (order > border || (order == border && unsigned(column) <= limit))) {
-                    const int at = atomicAdd(&counts[1], 1);
-                    if (at < kWordList) words[at] = order << 16 | (0xffffu - unsigned(column));
-                }
+        }
+        __syncthreads();
+        const int listed = min(counts[0], kChunkList);
+        for (int e = tid; e < 8 * listed; e += THREADS) {
+            const unsigned order = order_of(list[e >> 3][e & 7]);
+            const int column = list_chunk[e >> 3] * 8 + (e & 7);
+            if (column < vocab && order >= border) {
+                const int at = atomicAdd(&counts[1], 1);
+                if (at < kWordList) words[at] = order << 16 | (0xffffu - unsigned(column));
             }
-            __syncthreads();
-        };
-        collect();
+        }
+        __syncthreads();
         bool full = counts[0] > kChunkList || counts[1] > kWordList;
         if (full) {
             // Many words equal to the border (a mask that leaves fewer than are
@@ -281,7 +277,6 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
                 if (count([&](unsigned o, unsigned c) { return o == border && c < higher; }) < more)
                     below = higher;
             }
-            limit = below;
             // Words now, without the chunks: exactly `top`.
             if (tid < 2) counts[tid] = 0;
             __syncthreads();
@@ -292,7 +287,7 @@ logprobs_forward(float* __restrict__ logprob, float* __restrict__ entropy,
                 for (int j = 0; j < 8; ++j) {
                     const unsigned order = order_of(raw[i][j]);
                     const unsigned column = unsigned(tid + i * THREADS) * 8 + j;
-                    if (order > border || (order == border && column <= limit))
+                    if (order > border || (order == border && column <= below))
                         words[atomicAdd(&counts[1], 1)] = order << 16 | (0xffffu - column);
                 }
             }
