@@ -165,6 +165,29 @@ def test_one_sequence_much_longer(flint, cuda, heads, kv_heads, width):
 
 
 @pytest.mark.gpu
+def test_more_blocks_than_the_plan_has_buckets(flint, cuda):
+    """Places go two to a bucket from 1,024 blocks on: every block is listed
+    once, the longest bucket first, and rows along the long sequence are right."""
+    lengths = [700, 140000, 0, 260, 5000]
+    b = Batch(lengths, 1, 1, 64, seed=38, scale=0.125)
+    r = Run(flint, cuda, b).run(backward=False)
+    got = r.outputs()
+    plan = r.plan.view(torch.int32).view(-1, 4).cpu()
+    listed = plan[plan[:, 1] > plan[:, 0], :3].tolist()
+    blocks = [[a, e, i] for a, e in zip(b.offsets, b.offsets[1:]) for i in range(-(-(e - a) // 128))]
+    assert sorted(listed) == sorted(blocks)
+    places = [i // 2 for _, _, i in listed]
+    assert places == sorted(places, reverse=True)
+    q, k, v = b.parts(b.qkv)
+    first, end = b.offsets[1], b.offsets[2]
+    for row in (first, first + 131071, first + 70001, end - 1):
+        seen = torch.ones(1, row + 1 - first, dtype=torch.bool)
+        ref = attend(q[row:row + 1], k[first:row + 1], v[first:row + 1], b.scale, seen)
+        assert worst(got["o"][row:row + 1], *ref["o"]) <= 1.0
+        assert worst(got["lse"][row], *ref["lse"]) <= 1.0
+
+
+@pytest.mark.gpu
 def test_a_sequence_keeps_its_non_finite_values(flint, cuda):
     b = Batch([100, 90, 130], 2, 2, 64, seed=12)
     clean = Run(flint, cuda, b).run().outputs()
