@@ -9,14 +9,18 @@
 // the parts are joined by a second, small launch. Two kernels:
 //  * few rows (up to 32: generation). Reading the cache bounds it: 2 values of
 //    K and V a key and column against 4 FLOPs a row. Each wave streams tiles of
-//    its own through LDS, two in flight, with no barrier until the results of the
-//    workgroup's two waves are joined at the end. Until its first tile is there a
+//    its own through two buffers in LDS, with no barrier until the results of the
+//    workgroup's two waves are joined at the end. A tile's loads go out once the
+//    pages of the one behind it are known, and that lookup is waited for with the
+//    loads before it: other workgroups of the CU cover it, where there are any (long
+//    caches 4.9 to 5.3 TB/s, 64 short ones 3.1). Until its first tile is there a
 //    workgroup takes some 6 us (its item, the pages, the rows), so four small ones
 //    share a CU (two at width 128): 64 sequences of 512 positions, 12 heads of 64,
 //    take 29 us so, and 50 with one workgroup of four waves and tiles of 64 keys
 //    (16 sequences of 4,096: 46 and 66).
 //  * many rows (chunks of prompts). Each wave takes 32 of 128 rows, and the four
-//    share the tiles, as in packed.hip.
+//    share the tiles, as in packed.hip. Here the lookup comes behind the next tile's
+//    loads, so a tile's products wait for them.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -164,8 +168,9 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
 
 // Where the rows of a tile's loads lie in the pages: lane u has load u's offset
 // (halves) and the bytes there that hold cached positions with a page. One
-// vector load of the table serves a whole tile, and runs a tile ahead of its
-// use (taken load by load, the table's latency bound the kernel).
+// vector load of the table serves a whole tile, a tile ahead of its use (taken
+// load by load, the table's latency bound the kernel). The offsets are formed at
+// once, so the wave waits for the entries there, and for the loads before them.
 struct Where {
     unsigned low, high, held;
 };

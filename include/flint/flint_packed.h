@@ -66,7 +66,11 @@ FLINT_API flint_status flint_attention_packed_forward(void* o, void* lse, const 
 
 /* dq, dk, dv: the gradients of sum(dout * o) for the o and lse that
  * flint_attention_packed_forward returned with this q, k, v, plan and scale; dk
- * and dv sum over the query heads that share a head. Deterministic (fixed
+ * and dv sum over the query heads that share a head. RN16 of FP32 results; P and
+ * dS = P (dout v^T - D) enter the products as FP16, 2^8 times as large (as they
+ * are where that overflows; where dS itself passes 65,504, the gradients that take
+ * it are not finite). D = dout . o is that of the FP16 o; for dk it is put right by
+ * the sum of dS, which is 0 otherwise. Deterministic (fixed
  * summation order, no atomics). dq, dk and dv may be column slices of one
  * tensor; they overlap no input. */
 FLINT_API flint_status flint_attention_packed_backward_workspace(const flint_packed_shape* shape,

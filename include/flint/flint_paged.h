@@ -61,7 +61,7 @@ FLINT_API flint_status flint_attention_paged_workspace(const flint_paged_shape* 
                                                        size_t* bytes);
 
 /* o[t] = sum over visible positions of softmax(scale q[t] k^T) v, RN16 of an
- * FP32 result. scale is up to 2^64 in size; scores past 2^25 in size, where FP32
+ * FP32 result; probabilities enter the product with v as FP16. scale is up to 2^64 in size; scores past 2^25 in size, where FP32
  * is 4 apart, may give a row NaN. The workspace needs no preparation and keeps nothing between
  * calls. */
 FLINT_API flint_status flint_attention_paged(void* o, void* k_pages, void* v_pages, const void* q,
