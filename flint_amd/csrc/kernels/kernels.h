@@ -10,6 +10,7 @@
 
 #include "flint/flint_packed.h"
 #include "flint/flint_paged.h"
+#include "flint/flint_rotary.h"
 #include "flint/flint_train.h"
 
 namespace flint {
@@ -203,6 +204,12 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                                   const void* cached, const void* table,
                                   const flint_paged_shape& s, float scale, void* workspace,
                                   hipStream_t stream);
+// Rotary positions (rotary.hip).
+constexpr size_t kRotaryMaxWidth = 1024;
+hipError_t launch_rotary_plan(void* plan, const flint_rotary_angles& angles, hipStream_t stream);
+hipError_t launch_rotary(void* q_out, void* k_out, const void* q, const void* k,
+                         const void* positions, const void* plan, const flint_rotary_shape& s,
+                         bool backward, hipStream_t stream);
 // Rows of a causal tile and the k-step both divide this: a causal softmax
 // writing its zeros up to the end of each such block covers what the causal
 // GEMMs read.

@@ -23,6 +23,7 @@ NOALLOC_HEADER = ROOT / "include" / "flint" / "flint_noalloc.h"
 ATTENTION_HEADER = ROOT / "include" / "flint" / "flint_attention.h"
 PACKED_HEADER = ROOT / "include" / "flint" / "flint_packed.h"
 PAGED_HEADER = ROOT / "include" / "flint" / "flint_paged.h"
+ROTARY_HEADER = ROOT / "include" / "flint" / "flint_rotary.h"
 LOGPROBS_HEADER = ROOT / "include" / "flint" / "flint_logprobs.h"
 TUNING_HEADER = ROOT / "include" / "flint" / "flint_tuning.h"
 LIBRARY = ROOT / "build" / "release" / "bin" / "libflint.so"
@@ -87,6 +88,20 @@ class PagedShape(ctypes.Structure):
                 ("page_size", Z), ("max_pages", Z)]
 
 
+class RotaryAngles(ctypes.Structure):
+    """flint_rotary_angles (include/flint/flint_rotary.h)."""
+    _fields_ = [("width", Z), ("base", ctypes.c_double), ("factor", ctypes.c_double),
+                ("original", ctypes.c_double), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("magnitude", ctypes.c_double)]
+
+
+class RotaryShape(ctypes.Structure):
+    """flint_rotary_shape (include/flint/flint_rotary.h)."""
+    _fields_ = [("tokens", Z), ("heads", Z), ("kv_heads", Z), ("head_width", Z), ("width", Z),
+                ("layout", I), ("q_stride", Z), ("k_stride", Z), ("q_out_stride", Z),
+                ("k_out_stride", Z)]
+
+
 SIGNATURES = {
     "flint_version": (ctypes.c_char_p, []),
     "flint_status_string": (ctypes.c_char_p, [I]),
@@ -127,6 +142,10 @@ SIGNATURES = {
     # flint_logprobs.h (no counterpart in the reference)
     "flint_logprobs_forward": (I, [P] * 7 + [F, Z, Z, Z, Z, P]),
     "flint_logprobs_backward": (I, [P] * 7 + [F, Z, Z, Z, P]),
+    # flint_rotary.h (no counterpart in the reference)
+    "flint_rotary_plan_bytes": (I, [Z, ctypes.POINTER(Z)]),
+    "flint_rotary_plan": (I, [P, ctypes.POINTER(RotaryAngles), P]),
+    "flint_rotary": (I, [P] * 6 + [ctypes.POINTER(RotaryShape), I, P]),
     # flint_tuning.h (no counterpart in the reference)
     "flint_set_tuning": (I, [ctypes.c_char_p, ctypes.c_char_p]),
     "flint_gemm_nt_batched": (I, [P, P, P, Z, Z, Z, Z, F, P]),
@@ -466,6 +485,33 @@ class Flint:
             pointer(offsets), pointer(cached), pointer(table), shape, scale, pointer(workspace),
             workspace_bytes, stream_handle(stream)))
 
+    # -- rotary positions (flint_rotary.h) ------------------------------------
+    @staticmethod
+    def rotary_angles(width, base=10000.0, factor=1.0, original=0.0, low=1.0, high=32.0,
+                      magnitude=1.0):
+        return RotaryAngles(width, base, factor, original, low, high, magnitude)
+
+    def rotary_plan_bytes(self, width):
+        out = Z(0)
+        self.check(self.lib.flint_rotary_plan_bytes(width, ctypes.byref(out)))
+        return out.value
+
+    def rotary_plan(self, plan, angles, stream=None):
+        self.check(self.lib.flint_rotary_plan(pointer(plan), angles, stream_handle(stream)))
+
+    @staticmethod
+    def rotary_shape(tokens, heads, kv_heads, head_width, width, pairs, q_stride, k_stride,
+                     q_out_stride=None, k_out_stride=None):
+        """The outputs' strides are the inputs' where none are given (in place)."""
+        return RotaryShape(tokens, heads, kv_heads, head_width, width, int(pairs), q_stride,
+                           k_stride, q_stride if q_out_stride is None else q_out_stride,
+                           k_stride if k_out_stride is None else k_out_stride)
+
+    def rotary(self, q_out, k_out, q, k, positions, plan, shape, backward=False, stream=None):
+        self.check(self.lib.flint_rotary(pointer(q_out), pointer(k_out), pointer(q), pointer(k),
+                                         pointer(positions), pointer(plan), shape,
+                                         int(bool(backward)), stream_handle(stream)))
+
     def bias_gradient_noalloc(self, dbias, dy, rows, cols, accumulate=False, stream=None):
         """flint_bias_gradient with the library's own scratch array (no workspace)."""
         self.check(self.lib.flint_bias_gradient_noalloc(pointer(dbias), pointer(dy), rows, cols,
@@ -670,6 +716,6 @@ def declared_functions(header=None):
 
     headers = ([header] if header is not None
                else [HEADER, TRAIN_HEADER, NOALLOC_HEADER, ATTENTION_HEADER, PACKED_HEADER,
-                     PAGED_HEADER, LOGPROBS_HEADER, TUNING_HEADER])
+                     PAGED_HEADER, LOGPROBS_HEADER, ROTARY_HEADER, TUNING_HEADER])
     text = "".join(Path(h).read_text() for h in headers)
     return re.findall(r"FLINT_API\s+[^;(]*?\b(flint_\w+)\s*\(", text)
