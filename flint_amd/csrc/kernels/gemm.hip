@@ -888,6 +888,34 @@ hipError_t launch_gemm_nn(void* y, const void* x, const void* w, const void* aux
     }
 }
 
+// The gated products run on the pipeline or the few-tile kernels, which take every
+// size where the pipeline does not.
+hipError_t launch_gemm_nt_gated(void* y, void* pre, const void* x, const void* w, const void* bias,
+                                bool gelu, size_t m, size_t n, size_t k, hipStream_t stream) {
+    const Epilogue e = pre != nullptr ? Epilogue::kGatedPre : Epilogue::kGated;
+    const size_t wide = gated_width(n);
+    SmallPlan small;
+    if (gemm_small_plan(GemmLayout::kNT, e, 1, m, wide, k, 1, &small))
+        return launch_gemm_small(small, GemmLayout::kNT, e, y, x, w, bias, pre, 1.0f, 1, m, n, k,
+                                 false, nullptr, stream, false, nullptr, nullptr, gelu);
+    if (!gemm_pipe_eligible(GemmLayout::kNT, e, m, wide, k)) return hipErrorInvalidValue;
+    return launch_gemm_pipe(GemmLayout::kNT, e, y, x, w, bias, pre, 1.0f, 1, m, n, k, false, nullptr,
+                            0, stream, false, nullptr, nullptr, gelu);
+}
+
+hipError_t launch_gemm_nn_dgated(void* dpre, const void* x, const void* w, const void* pre,
+                                 bool gelu, size_t m, size_t n, size_t k, hipStream_t stream) {
+    const Epilogue e = Epilogue::kDGated;
+    SmallPlan small;
+    if (gemm_small_plan(GemmLayout::kNN, e, 1, m, n, k, 1, &small))
+        return launch_gemm_small(small, GemmLayout::kNN, e, dpre, x, w, nullptr,
+                                 const_cast<void*>(pre), 1.0f, 1, m, n, k, false, nullptr, stream,
+                                 false, nullptr, nullptr, gelu);
+    if (!gemm_pipe_eligible(GemmLayout::kNN, e, m, n, k)) return hipErrorInvalidValue;
+    return launch_gemm_pipe(GemmLayout::kNN, e, dpre, x, w, nullptr, const_cast<void*>(pre), 1.0f, 1,
+                            m, n, k, false, nullptr, 0, stream, false, nullptr, nullptr, gelu);
+}
+
 hipError_t launch_gemm_tn_split(void* y, const void* x, const void* w, size_t m, size_t n,
                                 size_t k, bool accumulate, void* workspace, int* splits_used,
                                 hipStream_t stream) {

@@ -50,8 +50,14 @@ __host__ __device__ constexpr int kmajor_key(int k) { return 2 * (k & 3); }
 
 enum class Layout { kNT, kNN, kTN };
 // What the kernel's store stage does. kTn writes FP32 (plain, accumulate or a
-// split's partial); kTnHalf is the batched TN's FP16 output.
-enum class Store { kNone, kBias, kBiasGelu, kBiasResidual, kDGelu, kScale, kTn, kTnHalf };
+// split's partial); kTnHalf is the batched TN's FP16 output. kGated and kGatedPre
+// (which keeps the projections too) and kDGated: the gated product and its
+// gradient, below.
+enum class Store {
+    kNone, kBias, kBiasGelu, kBiasResidual, kDGelu, kScale, kTn, kTnHalf,
+    kGated, kGatedPre, kDGated
+};
+constexpr bool is_gated(Store st) { return st == Store::kGated || st == Store::kGatedPre; }
 
 // Position of 16-byte chunk `chunk` of LDS row `row` (BK / 8 chunks a row).
 // BK 64: 128-byte rows, key (row ^ row >> 3) & 7; BK 32: 64-byte rows, key
@@ -93,6 +99,57 @@ __device__ __forceinline__ float gelu_grad(float s) {
     asm volatile("" : "+v"(g));
     return __builtin_isinf(s) ? (s > 0.0f ? 1.0f : 0.0f) : g;
 }
+
+// The FP32 value itself, however it was formed: a conversion that follows
+// rounds it and not the exact product behind it.
+__device__ __forceinline__ float settled(float x) {
+    asm("" : "+v"(x));
+    return x;
+}
+
+// The gated product multiplies two projections, rows 0 .. n - 1 (gate) and n ..
+// 2n - 1 (up) of w. A 32-row block of the MFMA takes 16 rows of either, so that a
+// lane holds a column of both: register groups 0 and 1 (of 4) gate columns 4h .. and
+// 8 + 4h .., groups 2 and 3 the same columns' up. `row` of a tile that starts at
+// gate row 0 is row gate_row(row) of its projection.
+__host__ __device__ constexpr int gate_row(int row) { return (row >> 5) * 16 + (row & 15); }
+__host__ __device__ constexpr bool gate_is_up(int row) { return (row & 16) != 0; }
+// Columns of the interleaved product, whole 16s of either projection.
+__host__ __device__ constexpr size_t gated_width(size_t n) { return (n + 15) / 16 * 32; }
+
+// Activations s sigma(z(s)): SiLU z = s, the tanh GELU z = 2 sqrt(2/pi) (s +
+// 0.044715 s^3). Either is s / (1 + 2^(s (c0 + c1 s^2))), with slope sigma + s sigma
+// (1 - sigma) z'(s), z' = t0 + t1 s^2: four constants instead of a branch (s^2 is
+// kept finite for c1 = 0).
+struct Gate {
+    float c0, c1, t0, t1;
+    __device__ __forceinline__ explicit Gate(int gelu) {
+        c0 = gelu ? -2.3022082f : -1.4426950408889634f;
+        c1 = gelu ? -0.10294324f : 0.0f;
+        t0 = gelu ? 1.5957691216057308f : 1.0f;
+        t1 = gelu ? 0.21406444860866706f : 0.0f;
+    }
+    // About 1e-6 relative error; -inf gives NaN.
+    __device__ __forceinline__ float value(float s) const {
+        const float s2 = fminf(s * s, 0x1p120f);
+        const float e = __builtin_amdgcn_exp2f(s * __builtin_fmaf(c1, s2, c0));
+        return s * __builtin_amdgcn_rcpf(1.0f + e);
+    }
+    // Value and slope; at infinite s (an FP16 pre may be one) their limits. 1 - sigma
+    // as in gelu_grad.
+    __device__ __forceinline__ void both(float s, float* value, float* slope) const {
+        const float s2 = fminf(s * s, 0x1p120f);
+        const float e = __builtin_amdgcn_exp2f(s * __builtin_fmaf(c1, s2, c0));
+        const float sigma = __builtin_amdgcn_rcpf(1.0f + e);
+        const float one_minus = s < 0.0f ? 1.0f - sigma : e * sigma;
+        const float q = s * one_minus * __builtin_fmaf(t1, s2, t0);
+        float g = __builtin_fmaf(sigma, q, sigma), v = s * sigma;
+        asm volatile("" : "+v"(g), "+v"(v));
+        const bool inf = __builtin_isinf(s);
+        *slope = inf ? (s > 0.0f ? 1.0f : 0.0f) : g;
+        *value = inf && s < 0.0f ? -0.0f : v;
+    }
+};
 
 struct TileArgs {
     int tiles_m, tiles_n;     // macro-tiles per batch / split
@@ -161,8 +218,8 @@ struct Operands {
     void* y;
     const _Float16* x;
     const _Float16* w;
-    const float* bias;     // bias (n FP32)
-    void* aux;             // pre (GELU out / dGELU in) or residual
+    const float* bias;     // bias (n FP32; gated products 2n, or null)
+    void* aux;             // pre (GELU, gated out / their gradients in) or residual
     float* partials;       // TN split partials, or null
     float scale;
     int accumulate;        // TN: y += instead of y =
@@ -172,6 +229,7 @@ struct Operands {
                            // not wanted, above its diagonal
     HeadView wv, yv;       // batched NN / TN (not gemm.hip): w (k-major) and
                            // y as heads views
+    int gelu;              // gated products (not gemm.hip): the tanh GELU, or SiLU
 };
 
 }  // namespace

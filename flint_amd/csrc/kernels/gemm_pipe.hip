@@ -92,26 +92,37 @@ template <int WTN, Store ST, bool COMPACT = false>
 struct PipeEpi {
     // FP32 values are staged when the output is FP32 (residual, TN) or when
     // the rounding needs a value that only the store pass reads (dGELU's pre).
-    static constexpr bool kF32 =
-        ST == Store::kBiasResidual || ST == Store::kTn || ST == Store::kDGelu;
+    static constexpr bool kSlope = ST == Store::kDGelu || ST == Store::kDGated;
+    static constexpr bool kF32 = ST == Store::kBiasResidual || ST == Store::kTn || kSlope;
     static constexpr int kOutElem = ST == Store::kBiasResidual || ST == Store::kTn ? 4 : 2;
-    static constexpr int kWtn = WTN;
+    // (The gated product stages its outputs, half as many columns; with the
+    // projections kept, those, and then the outputs.)
+    static constexpr int kWtn = ST == Store::kGated ? WTN / 2 : WTN;
     // Values per chunk: a chunk is one 16-byte store (8 FP16 or 4 FP32
     // outputs); dGELU stages FP32 but stores FP16, 8 values a chunk.
-    static constexpr int kPerChunk = kF32 && ST != Store::kDGelu ? 4 : 8;
+    static constexpr int kPerChunk = kF32 && !kSlope ? 4 : 8;
     static constexpr int kRows = (kF32 ? 16 : 32) / (COMPACT ? 2 : 1);   // rows staged at a time
     static constexpr int kLdw = kWtn + kPerChunk;             // staged row stride (values)
     static constexpr int kHalves = kRows * kLdw * (kF32 ? 2 : 1);   // per wave, in halves
     static constexpr int kCpr = kWtn / kPerChunk;             // chunks per staged row
     static constexpr int kPerLane = kRows * kCpr / 64;        // chunks per lane per block
     static_assert(kRows * kCpr % 64 == 0, "whole store instructions");
-    static constexpr int kPasses = ST == Store::kBiasGelu ? 2 : 1;
+    static constexpr int kPasses = ST == Store::kBiasGelu || ST == Store::kGatedPre ? 2 : 1;
+    // The gated outputs' chunks per staged row, and per lane per block.
+    static constexpr int kYCpr = WTN / 2 / kPerChunk;
+    static constexpr int kYPerLane = kRows * kYCpr / 64;
+    static_assert(!is_gated(ST) || kRows * kYCpr % 64 == 0, "whole store instructions");
+    // Stores per staged block.
+    static constexpr int kBlockStores = ST == Store::kGatedPre ? kPerLane + kYPerLane
+                                        : ST == Store::kDGated ? 2 * kPerLane
+                                                               : kPerLane * kPasses;
     static constexpr int kSubs = 32 / kRows;                  // staged blocks per 32 rows
 };
 
 constexpr size_t kPipeMaxLds = 160 * 1024;
 constexpr bool is_bias_store(Store st) {
-    return st == Store::kBias || st == Store::kBiasGelu || st == Store::kBiasResidual;
+    return st == Store::kBias || st == Store::kBiasGelu || st == Store::kBiasResidual ||
+           is_gated(st);
 }
 // Two-stage tiles with 64-deep steps read fragments two sub-steps ahead (four
 // fragment buffers) where the accumulators and buffers fit in 320 registers;
@@ -231,15 +242,16 @@ gemm_pipe(Operands op, TileArgs ta) {
     // filled yet, since it cannot see that asm results are still in flight.
     using XFrag = std::conditional_t<kXM, TrFrag, f16x8>;
     using WFrag = std::conditional_t<kWM, TrFrag, f16x8>;
-    constexpr bool kBias =
-        ST == Store::kBias || ST == Store::kBiasGelu || ST == Store::kBiasResidual;
+    constexpr bool kBias = is_bias_store(ST);
+    constexpr bool kGate = is_gated(ST);
+    static_assert(!kGate || L == Layout::kNT, "both projections' rows are k-contiguous");
     using E = PipeEpi<WTN, ST, pipe_compact<BM, BN, S, BK, ST, NW>()>;
     constexpr int kStageHalves = S * (BM + BN) * BK;
     static_assert(WTM % 32 == 0 && WTN % 32 == 0, "whole 32 x 32 blocks per wave");
     static_assert(pipe_lds_bytes<BM, BN, S, BK, L, ST, NW>() <= kPipeMaxLds, "LDS");
     static_assert((S - 2) * PER + PER < 64, "vmcnt range");
     // Buffer stores per wave per tile, bias loads per wave per tile.
-    constexpr int kStores = FM * E::kSubs * E::kPerLane * E::kPasses;
+    constexpr int kStores = FM * E::kSubs * E::kBlockStores;
     constexpr bool kLook2 = pipe_look2(BM, BN, S, BK, NW);
     constexpr bool kBiasLds = kBias && kLook2;
     // Bias loads per wave per tile: FN * 4 into registers, or one 1 KB load
@@ -253,9 +265,10 @@ gemm_pipe(Operands op, TileArgs ta) {
     // dGELU's pre: the first staged block's chunks load at tile start, and
     // each later block's while the block before it is stored, so that no
     // block waits out a load's full latency.
-    constexpr bool kPreEarly = ST == Store::kDGelu;
+    constexpr bool kPreEarly = E::kSlope;
+    constexpr int kPreLoads = ST == Store::kDGated ? 2 * E::kPerLane : E::kPerLane;
     constexpr int kEarlyLoads =
-        kBiasLoads + (kResEarly ? kResAll : 0) + (kPreEarly ? E::kPerLane : 0);
+        kBiasLoads + (kResEarly ? kResAll : 0) + (kPreEarly ? kPreLoads : 0);
     // One LDS object for everything: with a second one, the compiler's LDS-DMA
     // alias tracking put a vmcnt(0) in front of every fragment read.
     __shared__ __attribute__((aligned(16)))
@@ -275,7 +288,7 @@ gemm_pipe(Operands op, TileArgs ta) {
     // op.wv.ld apart in a heads view); y's rows are n apart, or op.yv.ld.
     const int a_ld = kXM ? m : K;
     const int b_ld = kWM ? (HV ? op.wv.ld : n) : K;
-    const int y_ld = HV ? op.yv.ld : n;
+    const int y_ld = HV ? op.yv.ld : (ST == Store::kDGated ? 2 * n : n);
     _Float16* const cst = lds + kStageHalves + wave * E::kHalves;
 
     // This workgroup's tiles: ids blockIdx.x, + gridDim.x, ... (gridDim.x is a
@@ -350,6 +363,11 @@ gemm_pipe(Operands op, TileArgs ta) {
             t.b = ws + t.n0;
             t.b_bytes = HV ? unsigned((size_t(K - 1) * b_ld + n - t.n0) * 2)
                            : unsigned((size_t(K) * n - t.n0) * 2);
+        } else if (kGate) {
+            // From the tile's first gate row through the last up row. Gate rows
+            // past n are up rows, which reach no stored output.
+            t.b = ws + size_t(t.n0 / 2) * K;
+            t.b_bytes = unsigned(2 * n - t.n0 / 2) * unsigned(K) * 2u;
         } else {
             t.b = ws + size_t(t.n0) * K;
             t.b_bytes = unsigned(min(BN, n - t.n0)) * unsigned(K) * 2u;
@@ -368,7 +386,7 @@ gemm_pipe(Operands op, TileArgs ta) {
     // [u KB, u KB + 1 KB) of its region; lane l writes bytes l * 16 .. + 16.
     // voff: the lane's byte offset in the global operand for k = 0 (the
     // k-step goes in the scalar offset).
-    auto lane_voff = [&](int q, int rows, bool kmajor, int ld) {
+    auto lane_voff = [&](int q, int rows, bool kmajor, int ld, bool gate = false) {
         const int u = q * NLW + lw;
         if (kmajor) {
             const int p = u * 1024 + lane * 16;       // byte in the [32][rows] tile
@@ -379,12 +397,13 @@ gemm_pipe(Operands op, TileArgs ta) {
         }
         constexpr int kCpr = BK / 8;              // 16-byte chunks per row
         const int row = u * (64 / kCpr) + lane / kCpr;
-        return unsigned((row * ld + ((lane % kCpr) ^ row_key<BK>(row)) * 8) * 2);
+        const int from = gate ? gate_row(row) + (gate_is_up(row) ? n : 0) : row;
+        return (unsigned(from) * unsigned(ld) + unsigned(((lane % kCpr) ^ row_key<BK>(row)) * 8)) * 2u;
     };
     unsigned voff[PER];
 #pragma unroll
     for (int q = 0; q < PER; ++q)
-        voff[q] = q < IA ? lane_voff(q, BM, kXM, a_ld) : lane_voff(q - IA, BN, kWM, b_ld);
+        voff[q] = q < IA ? lane_voff(q, BM, kXM, a_ld) : lane_voff(q - IA, BN, kWM, b_ld, kGate);
     // The lane's k within a step in a row-major load. A load covers 8 rows
     // (BK 64) and every wave an even count of loads apart, so that the chunk
     // key is the same for all of the lane's loads.
@@ -594,6 +613,9 @@ gemm_pipe(Operands op, TileArgs ta) {
         const Tile t = tile(i);
         // Bias of this lane's columns, for the epilogue: buffer loads with the
         // resource ending at n (columns past it read 0), FN * 4 of them per wave.
+        // Gated products may have none (no bytes: all of it reads 0).
+        const unsigned bias_bytes =
+            kGate ? (op.bias != nullptr ? unsigned(n) * 8u : 0u) : unsigned(n) * 4u;
         f32x4 bias[kBias ? FN : 1][4];
         float* const bias_lds = reinterpret_cast<float*>(lds + kStageHalves + NW * E::kHalves) +
                                 wave * 256;
@@ -605,18 +627,24 @@ gemm_pipe(Operands op, TileArgs ta) {
             // covers the vector offset only, and it is what makes the lanes
             // past n read 0 instead of the memory after the bias.
             const auto rbias = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<float*>(op.bias), 0, unsigned(n) * 4u, 0x00020000);
+                const_cast<float*>(op.bias), 0, bias_bytes, 0x00020000);
+            const unsigned c = kGate ? unsigned((t.n0 + wn * WTN) / 2 + gate_row(4 * lane) +
+                                                (gate_is_up(4 * lane) ? n : 0))
+                                     : unsigned(t.n0 + wn * WTN + 4 * lane);
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                rbias, (__attribute__((address_space(3))) void*)(lds_half*)bias_lds, 16,
-                unsigned(t.n0 + wn * WTN) * 4u + unsigned(lane) * 16u, 0, 0, 0);
+                rbias, (__attribute__((address_space(3))) void*)(lds_half*)bias_lds, 16, c * 4u, 0,
+                0, 0);
         } else if constexpr (kBias) {
             const auto rbias = __builtin_amdgcn_make_buffer_rsrc(
-                const_cast<float*>(op.bias), 0, unsigned(n) * 4u, 0x00020000);
+                const_cast<float*>(op.bias), 0, bias_bytes, 0x00020000);
 #pragma unroll
             for (int ii = 0; ii < FN; ++ii)
 #pragma unroll
                 for (int g4 = 0; g4 < 4; ++g4) {
-                    const int c = t.n0 + wn * WTN + ii * 32 + g4 * 8 + fc * 4;
+                    const int in = ii * 32 + g4 * 8 + fc * 4;
+                    const int c = kGate ? (t.n0 + wn * WTN) / 2 + gate_row(in) +
+                                              (gate_is_up(in) ? n : 0)
+                                        : t.n0 + wn * WTN + in;
                     bias[ii][g4] = __builtin_bit_cast(
                         f32x4, __builtin_amdgcn_raw_buffer_load_b128(rbias, unsigned(c) * 4u, 0, 0));
                 }
@@ -626,9 +654,9 @@ gemm_pipe(Operands op, TileArgs ta) {
         // the end when the chunk is outside the output (n % 8 == 0 here, so a
         // chunk is whole once it starts).
         const int row_base = t.m0 + wm * WTM;
-        const int col_base = t.n0 + wn * WTN;
+        const int col_base = kGate ? (t.n0 + wn * WTN) / 2 : t.n0 + wn * WTN;
         const unsigned out_bytes = HV ? unsigned((size_t(m - 1) * y_ld + n) * E::kOutElem)
-                                      : unsigned(size_t(m) * n * E::kOutElem);
+                                      : unsigned(size_t(m) * y_ld * E::kOutElem);
         auto chunk_at = [&](int j, int h, int q, int elem, int* r, int* cc) {
             const int c = q * 64 + lane;
             *r = c / E::kCpr;
@@ -638,6 +666,21 @@ gemm_pipe(Operands op, TileArgs ta) {
             return gr < m && gc < n ? (unsigned(gr) * unsigned(y_ld) + unsigned(gc)) * unsigned(elem)
                                     : 0xfffffff0u;
         };
+        // The gated product's: chunk q of the staged outputs, or of the projections
+        // (the staged row holds the gate's chunks, then the up's).
+        auto gated_chunk_at = [&](int j, int h, int q, bool pre, int* r, int* cc) {
+            const int c = q * 64 + lane, cpr = pre ? 2 * E::kYCpr : E::kYCpr;
+            *r = c / cpr;
+            *cc = c % cpr;
+            const int gr = row_base + j * 32 + h * E::kRows + *r;
+            const bool up = *cc >= E::kYCpr;
+            const int gc = col_base + (*cc - (up ? E::kYCpr : 0)) * E::kPerChunk;
+            return gr < m && gc < n ? (unsigned(gr) * unsigned(pre ? 2 * n : n) +
+                                       unsigned(gc + (up ? n : 0))) * 2u
+                                    : 0xfffffff0u;
+        };
+        // dGated's second half of a row, n values after the first.
+        auto up_of = [&](unsigned off) { return off == 0xfffffff0u ? off : off + unsigned(n) * 2u; };
         f32x4 res_all[kResEarly ? FM : 1][kResEarly ? E::kSubs : 1][kResEarly ? E::kPerLane : 1];
         if constexpr (kResEarly) {
             const auto rs = __builtin_amdgcn_make_buffer_rsrc(
@@ -655,8 +698,8 @@ gemm_pipe(Operands op, TileArgs ta) {
                                        rs, chunk_at(j, h, q, 4, &r, &cc), 0, 0));
                     }
         }
-        // Block (j, h)'s pre chunks, 8 FP16 each.
-        auto load_pre = [&](int j, int h, f16x8 (&dst)[E::kPerLane]) {
+        // Block (j, h)'s pre chunks, 8 FP16 each (dGated: the gate's, then the up's).
+        auto load_pre = [&](int j, int h, f16x8 (&dst)[kPreLoads]) {
             const auto rs = __builtin_amdgcn_make_buffer_rsrc(
                 const_cast<void*>(static_cast<const void*>(
                     static_cast<const _Float16*>(op.aux) + t.y_off)),
@@ -664,12 +707,15 @@ gemm_pipe(Operands op, TileArgs ta) {
 #pragma unroll
             for (int q = 0; q < E::kPerLane; ++q) {
                 int r, cc;
-                dst[q] = __builtin_bit_cast(
-                    f16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, chunk_at(j, h, q, 2, &r, &cc),
-                                                                 0, 0));
+                const unsigned off = chunk_at(j, h, q, 2, &r, &cc);
+                dst[q] = __builtin_bit_cast(f16x8,
+                                            __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+                if constexpr (ST == Store::kDGated)
+                    dst[E::kPerLane + q] = __builtin_bit_cast(
+                        f16x8, __builtin_amdgcn_raw_buffer_load_b128(rs, up_of(off), 0, 0));
             }
         };
-        f16x8 pre_next[kPreEarly ? E::kPerLane : 1];
+        f16x8 pre_next[kPreEarly ? kPreLoads : 1];
         if constexpr (kPreEarly) load_pre(0, 0, pre_next);
         const int steps = whole_steps(t);
         for (int s = 0; s < steps; ++s) {
@@ -830,21 +876,61 @@ gemm_pipe(Operands op, TileArgs ta) {
                     const int nb = j * E::kSubs + h + 1;
                     if (nb < FM * E::kSubs) load_rd(nb / E::kSubs, nb % E::kSubs, rd_next);
                 }
-                f16x8 pre8[ST == Store::kDGelu ? E::kPerLane : 1];
-                if constexpr (ST == Store::kDGelu) {
+                f16x8 pre8[kPreEarly ? kPreLoads : 1];
+                if constexpr (kPreEarly) {
 #pragma unroll
-                    for (int q = 0; q < E::kPerLane; ++q) pre8[q] = pre_next[q];
+                    for (int q = 0; q < kPreLoads; ++q) pre8[q] = pre_next[q];
                     const int nb = j * E::kSubs + h + 1;
                     if (nb < FM * E::kSubs) load_pre(nb / E::kSubs, nb % E::kSubs, pre_next);
                 }
-                f16x4 ykeep[ST == Store::kBiasGelu ? FN : 1][4];
+                f16x4 ykeep[ST == Store::kBiasGelu || ST == Store::kGatedPre ? FN : 1][4];
 #pragma unroll
                 for (int pass = 0; pass < E::kPasses; ++pass) {
                     // GELU: pass 0 writes pre = RN16(s), pass 1 y = RN16(gelu(s)).
                     const bool gelu_pass = ST == Store::kBiasGelu && pass == 1;
                     // The lanes holding the block's rows (each lane holds one row).
                     const bool mine = E::kRows == 32 || fr / E::kRows == h;
-                    if (mine) {
+                    if constexpr (kGate) {
+                        if (mine) {
+                            const int srow = fr % E::kRows;
+                            const Gate gate(op.gelu);
+#pragma unroll
+                            for (int ii = 0; ii < FN; ++ii) {
+#pragma unroll
+                                for (int g = 0; g < 2; ++g) {
+                                    _Float16* at = cst + srow * E::kLdw + ii * 16 + g * 8 + fc * 4;
+                                    if (pass == 1) {
+                                        *reinterpret_cast<f16x4*>(at) = ykeep[ii][g];
+                                        continue;
+                                    }
+                                    f32x4 a = {acc[ii][j][g * 4 + 0], acc[ii][j][g * 4 + 1],
+                                               acc[ii][j][g * 4 + 2], acc[ii][j][g * 4 + 3]};
+                                    f32x4 b = {acc[ii][j][g * 4 + 8], acc[ii][j][g * 4 + 9],
+                                               acc[ii][j][g * 4 + 10], acc[ii][j][g * 4 + 11]};
+                                    a += bias_of(ii, g);
+                                    b += bias_of(ii, g + 2);
+                                    f16x4 y;
+#pragma unroll
+                                    for (int e = 0; e < 4; ++e) {
+                                        a[e] = settled(a[e]);
+                                        b[e] = settled(b[e]);
+                                        y[e] = _Float16(settled(gate.value(a[e]) * b[e]));
+                                    }
+                                    if constexpr (ST == Store::kGated) {
+                                        *reinterpret_cast<f16x4*>(at) = y;
+                                    } else {
+                                        ykeep[ii][g] = y;
+                                        *reinterpret_cast<f16x4*>(at) =
+                                            f16x4{_Float16(a[0]), _Float16(a[1]), _Float16(a[2]),
+                                                  _Float16(a[3])};
+                                        *reinterpret_cast<f16x4*>(at + WTN / 2) =
+                                            f16x4{_Float16(b[0]), _Float16(b[1]), _Float16(b[2]),
+                                                  _Float16(b[3])};
+                                    }
+                                }
+                            }
+                        }
+                    } else if (mine) {
                         const int srow = fr % E::kRows;
 #pragma unroll
                         for (int ii = 0; ii < FN; ++ii) {
@@ -882,15 +968,44 @@ gemm_pipe(Operands op, TileArgs ta) {
                     // it once, for the lanes that wrote only.
                     __builtin_amdgcn_wave_barrier();
                     asm volatile("" ::: "memory");
-                    void* out = ST == Store::kBiasGelu && pass == 0 ? op.aux : op.y;
+                    constexpr bool kTwoOut = ST == Store::kBiasGelu || ST == Store::kGatedPre;
+                    void* out = kTwoOut && pass == 0 ? op.aux : op.y;
                     if (split) out = op.partials;
                     out = static_cast<char*>(out) + t.y_off * E::kOutElem;
-                    const auto rout = __builtin_amdgcn_make_buffer_rsrc(out, 0, out_bytes,
-                                                                        0x00020000);
+                    const bool pre_pass = ST == Store::kGatedPre && pass == 0;
+                    const auto rout = __builtin_amdgcn_make_buffer_rsrc(
+                        out, 0, pre_pass ? 2 * out_bytes : out_bytes, 0x00020000);
 #pragma unroll
                     for (int q = 0; q < E::kPerLane; ++q) {
                         int r, cc;
-                        if constexpr (ST == Store::kDGelu) {
+                        if constexpr (kGate) {
+                            if (!pre_pass && q >= E::kYPerLane) continue;
+                            const unsigned off = gated_chunk_at(j, h, q, pre_pass, &r, &cc);
+                            const f16x8 v = *reinterpret_cast<const f16x8*>(cst + r * E::kLdw + cc * 8);
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rout,
+                                                                   off, 0, kStoreAux);
+                        } else if constexpr (ST == Store::kDGated) {
+                            // Gate: RN16(sum u act'(g)), up: RN16(sum act(g)).
+                            const unsigned off = chunk_at(j, h, q, 2, &r, &cc);
+                            const float* sp = reinterpret_cast<const float*>(cst) + r * E::kLdw + cc * 8;
+                            const f32x4 s0 = *reinterpret_cast<const f32x4*>(sp);
+                            const f32x4 s1 = *reinterpret_cast<const f32x4*>(sp + 4);
+                            const Gate gate(op.gelu);
+                            f16x8 dg, du;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float sum = e < 4 ? s0[e & 3] : s1[e & 3];
+                                float value, slope;
+                                gate.both(float(pre8[q][e]), &value, &slope);
+                                dg[e] = _Float16(
+                                    settled(sum * float(pre8[kPreLoads - E::kPerLane + q][e]) * slope));
+                                du[e] = _Float16(settled(sum * value));
+                            }
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, dg), rout,
+                                                                   off, 0, kStoreAux);
+                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, du), rout,
+                                                                   up_of(off), 0, kStoreAux);
+                        } else if constexpr (ST == Store::kDGelu) {
                             // y = RN16(sum * GELU'(pre)), 8 outputs = 16 bytes.
                             const unsigned off = chunk_at(j, h, q, 2, &r, &cc);
                             const float* sp = reinterpret_cast<const float*>(cst) + r * E::kLdw + cc * 8;
@@ -985,9 +1100,10 @@ bool pipe_forced(PipeConfig* out, bool* disabled) {
 // LDS bytes of a configuration at run time (the kernel's own static_assert
 // checks the same sum).
 size_t lds_bytes(const PipeConfig& c, Store st) {
-    const bool f32 = st == Store::kBiasResidual || st == Store::kTn || st == Store::kDGelu;
-    const int wtn = c.bn / pipe_waves_n(c.bn), per = f32 && st != Store::kDGelu ? 4 : 8,
-              rows = f32 ? 16 : 32;
+    const bool slope = st == Store::kDGelu || st == Store::kDGated;
+    const bool f32 = st == Store::kBiasResidual || st == Store::kTn || slope;
+    const int wtn = c.bn / pipe_waves_n(c.bn) / (st == Store::kGated ? 2 : 1),
+              per = f32 && !slope ? 4 : 8, rows = f32 ? 16 : 32;
     const size_t stages = size_t(c.stages) * (c.bm + c.bn) * c.bk * 2 +
                           pipe_bias_lds(c.bm, c.bn, c.stages, c.bk, st, c.waves);
     const size_t staging = size_t(c.waves) * rows * (wtn + per) * (f32 ? 4 : 2);
@@ -1001,12 +1117,22 @@ bool has_tail(const PipeConfig& c) { return c.same(PipeConfig{128, 192, 3, 64});
 // of each call showed in calls of a few us).
 size_t whole_k(const PipeConfig& c, size_t k) { return (k + c.bk - 1) & ~size_t(c.bk - 1); }
 
+// The gated products' configurations: those of which the tile choice takes one for
+// an epilogue like theirs (no loader waves or 64-wide tiles), but for 256 x 256,
+// whose epilogue does not fit the registers beside its accumulators.
+constexpr bool gated_config(int bn, int waves, int loaders) {
+    return bn >= 128 && bn < 256 && waves == 4 && loaders == 0;
+}
+
 // Whether a configuration can run an epilogue over k: it fits in LDS and k is
 // whole k-steps, or TN's FP32 output's, or the configuration takes tails (its
 // heads-view instances do not); the 8-wave configuration serves the NT layout
 // only.
 bool usable(const PipeConfig& c, Store st, size_t k, Layout l, bool views) {
     const bool tail = st == Store::kTn || (l != Layout::kTN && !views && has_tail(c));
+    if ((is_gated(st) || st == Store::kDGated) &&
+        !gated_config(c.bn, c.waves, c.loaders))
+        return false;
     return lds_bytes(c, st) <= kPipeMaxLds && (whole_k(c, k) == k || tail) &&
            (c.waves == 4 || l == Layout::kNT);
 }
@@ -1157,10 +1283,11 @@ template <Layout L, Store ST>
 hipError_t launch_pipe(const PipeConfig& c, const Operands& op, size_t slices, int split_len,
                        int cus, hipStream_t stream) {
     constexpr bool kViews = L != Layout::kNT && (ST == Store::kNone || ST == Store::kTnHalf);
+    constexpr bool kGatedOp = is_gated(ST) || ST == Store::kDGated;
     const bool hv = op.wv.heads != 0;
     TileArgs ta{};
     ta.tiles_m = (op.m + c.bm - 1) / c.bm;
-    ta.tiles_n = (op.n + c.bn - 1) / c.bn;
+    ta.tiles_n = int(((is_gated(ST) ? gated_width(op.n) : size_t(op.n)) + c.bn - 1) / c.bn);
     ta.tiles_per_slice = ta.tiles_m * ta.tiles_n;
     if (L == Layout::kNT && op.causal) {
         ta.tiles_per_slice = 0;
@@ -1181,6 +1308,7 @@ hipError_t launch_pipe(const PipeConfig& c, const Operands& op, size_t slices, i
     // any other would drop the k past the whole ones.
     const bool whole = ST == Store::kTn || whole_k(c, size_t(op.k)) == size_t(op.k);
 #define FLINT_PIPE_CASE(BM_, BN_, S_, BK_, NW_, LD_)                                           \
+    if constexpr (!kGatedOp || gated_config(BN_, NW_, LD_))                                    \
     if constexpr (pipe_lds_bytes<BM_, BN_, S_, BK_, L, ST, NW_>() <= kPipeMaxLds) {            \
         if (c.same(PipeConfig{BM_, BN_, S_, BK_, NW_, LD_})) {                                 \
             if (hv && !whole) return hipErrorInvalidValue;                                     \
@@ -1236,6 +1364,9 @@ Store store_of(Epilogue e, Layout l) {
     case Epilogue::kBiasResidual: return Store::kBiasResidual;
     case Epilogue::kDGelu: return Store::kDGelu;
     case Epilogue::kScale: return Store::kScale;
+    case Epilogue::kGated: return Store::kGated;
+    case Epilogue::kGatedPre: return Store::kGatedPre;
+    case Epilogue::kDGated: return Store::kDGated;
     }
     return Store::kNone;
 }
@@ -1257,6 +1388,10 @@ hipError_t dispatch_pipe(const PipeConfig& c, Store st, const Operands& op, size
             return launch_pipe<L, Store::kBiasResidual>(c, op, slices, split_len, cus, stream);
         case Store::kScale:
             return launch_pipe<L, Store::kScale>(c, op, slices, split_len, cus, stream);
+        case Store::kGated:
+            return launch_pipe<L, Store::kGated>(c, op, slices, split_len, cus, stream);
+        case Store::kGatedPre:
+            return launch_pipe<L, Store::kGatedPre>(c, op, slices, split_len, cus, stream);
         default: break;
         }
     } else if constexpr (L == Layout::kNN) {
@@ -1264,6 +1399,8 @@ hipError_t dispatch_pipe(const PipeConfig& c, Store st, const Operands& op, size
         case Store::kNone: return launch_pipe<L, Store::kNone>(c, op, slices, split_len, cus, stream);
         case Store::kDGelu:
             return launch_pipe<L, Store::kDGelu>(c, op, slices, split_len, cus, stream);
+        case Store::kDGated:
+            return launch_pipe<L, Store::kDGated>(c, op, slices, split_len, cus, stream);
         default: break;
         }
     } else {
@@ -1322,14 +1459,17 @@ bool gemm_pipe_eligible(GemmLayout gl, Epilogue e, size_t m, size_t n, size_t k)
     // Only the epilogues each layout serves.
     const bool served = l == Layout::kNT ? (st == Store::kNone || st == Store::kBias ||
                                             st == Store::kBiasGelu || st == Store::kBiasResidual ||
-                                            st == Store::kScale)
-                        : l == Layout::kNN ? (st == Store::kNone || st == Store::kDGelu)
+                                            st == Store::kScale || is_gated(st))
+                        : l == Layout::kNN ? (st == Store::kNone || st == Store::kDGelu ||
+                                              st == Store::kDGated)
                                            : (st == Store::kTn || st == Store::kTnHalf);
     if (!served) return false;
     // k-major operands come in 16-byte chunks of their columns.
     if (l == Layout::kTN && m % 8 != 0) return false;
     // Buffer offsets are 32-bit: one slice's output and each operand.
-    const size_t out_elem = st == Store::kBiasResidual || st == Store::kTn ? 4 : 2;
+    // (The gated products come with n as their w's rows, or half of dpre's columns.)
+    const size_t out_elem =
+        st == Store::kBiasResidual || st == Store::kTn || st == Store::kDGated ? 4 : 2;
     if (m * n * out_elem >= (size_t{1} << 31) || m * k * 2 >= (size_t{1} << 31) ||
         n * k * 2 >= (size_t{1} << 31)) {
         return false;
@@ -1376,9 +1516,10 @@ PipeEstimate gemm_pipe_estimate(GemmLayout gl, Epilogue e, size_t slices, size_t
     const double step_us = double(c.bm) * double(c.bn) / 65536.0 / pipe_eff(c, st, l) * layout *
                            lines * crowd;
     const double fixed = l == Layout::kTN ? 4.56 : (l == Layout::kNT ? 2.81 : 2.68);
-    const double epilogue = st == Store::kDGelu                                       ? 3.0
-                            : st == Store::kBiasGelu || st == Store::kBiasResidual ? 2.0
-                                                                                   : 0.0;
+    const double epilogue = st == Store::kDGelu || st == Store::kDGated ? 3.0
+                            : st == Store::kBiasGelu || st == Store::kBiasResidual || is_gated(st)
+                                ? 2.0
+                                : 0.0;
     PipeEstimate out;
     out.load = load;
     out.us = rounds * steps * step_us + fixed * (1.0 + 1.34 * (rounds - 1.0));
@@ -1395,7 +1536,7 @@ hipError_t launch_gemm_pipe(GemmLayout gl, Epilogue e, void* y, const void* x, c
                             const void* bias, void* aux, float scale, size_t slices, size_t m,
                             size_t n, size_t k, bool accumulate, void* partials, int split_len,
                             hipStream_t stream, bool causal, const HeadView* wv,
-                            const HeadView* yv) {
+                            const HeadView* yv, bool gelu) {
     // Heads views: batched NN / TN with FP16 outputs only, every slice a
     // whole (sequence, head) pair.
     if (wv != nullptr || yv != nullptr) {
@@ -1425,6 +1566,7 @@ hipError_t launch_gemm_pipe(GemmLayout gl, Epilogue e, void* y, const void* x, c
     op.n = int(n);
     op.k = int(k);
     const Layout l = layout_of(gl);
+    op.gelu = gelu ? 1 : 0;
     // Causal needs the square operand, and no TN split (k-ranges of its own).
     op.causal = causal && split_len == 0 &&
                         (l == Layout::kNT ? m == n : m == k) ? 1 : 0;
@@ -1447,7 +1589,8 @@ hipError_t launch_gemm_pipe(GemmLayout gl, Epilogue e, void* y, const void* x, c
     bool disabled = false;
     const bool views = op.wv.heads != 0;
     if (!pipe_forced(&c, &disabled) || !usable(c, st, k, l, views))
-        c = pick_pipe(m, n, k, slices, cus, st, l, views, op.causal != 0);
+        c = pick_pipe(m, is_gated(st) ? gated_width(n) : n, k, slices, cus, st, l, views,
+                      op.causal != 0);
     switch (l) {
     case Layout::kNT: return dispatch_pipe<Layout::kNT>(c, st, op, slices, split_len, cus, stream);
     case Layout::kNN: return dispatch_pipe<Layout::kNN>(c, st, op, slices, split_len, cus, stream);

@@ -60,13 +60,6 @@ constexpr double kSplitSumUs = 3.0;
 // A buffer offset past every resource: the load returns zeros.
 constexpr unsigned kOutside = 0xfffffff0u;
 
-// The FP32 value itself, however it was formed: a conversion that follows
-// rounds it and not the exact product behind it.
-__device__ __forceinline__ float settled(float x) {
-    asm("" : "+v"(x));
-    return x;
-}
-
 template <int WM, int WN, int NW, int S, int U, bool LD, Layout L, Store ST, bool HV = false>
 __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) {
     // The host pass only needs a kernel to emit a launch stub for.
@@ -81,8 +74,9 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
     constexpr bool kWM = L != Layout::kNT;
     using XFrag = std::conditional_t<kXM, TrFrag, f16x8>;
     using WFrag = std::conditional_t<kWM, TrFrag, f16x8>;
-    constexpr bool kBias =
-        ST == Store::kBias || ST == Store::kBiasGelu || ST == Store::kBiasResidual;
+    constexpr bool kGate = is_gated(ST);
+    constexpr bool kBias = ST == Store::kBias || ST == Store::kBiasGelu ||
+                           ST == Store::kBiasResidual || kGate;
     constexpr bool kF32 = ST == Store::kBiasResidual || ST == Store::kTn;
     // A step's 1 KB loads, x's first, dealt to the waves in turn.
     constexpr int NL = LD ? NW - WM * WN : NW;   // waves that load
@@ -143,10 +137,11 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
     // Offsets within a tile fit in 32 bits: the entry points take k up to 65,536
     // (kGemmMaxK) and m and n up to 8,388,480 (kGemmMaxMN).
     const _Float16* const a = kXM ? xs + m0 : xs + size_t(m0) * K;
-    const _Float16* const b = kWM ? ws + n0 : ws + size_t(n0) * K;
+    // (A gated product's tile: rows n0 / 2 on of the gate, and the same of the up.)
+    const _Float16* const b = kWM ? ws + n0 : ws + size_t(kGate ? n0 / 2 : n0) * K;
     const size_t a_bytes = kXM ? (size_t(K) * m - m0) * 2 : size_t(min(BM, m - m0)) * K * 2;
     const size_t b_bytes = kWM ? (size_t(K - 1) * b_ld + n - n0) * 2
-                               : size_t(min(BN, n - n0)) * K * 2;
+                               : size_t(kGate ? min(BN / 2, n - n0 / 2) : min(BN, n - n0)) * K * 2;
     // Load v = q NL + lw of a step fills LDS bytes [v KB, v KB + 1 KB) of its
     // stage (x's region, then w's); lane l writes bytes 16 l .. + 15 of it.
     unsigned voff[PER];
@@ -154,7 +149,8 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
     auto of_x = [&](int q) {
         return kLoadsA % NL == 0 ? q < kLoadsA / NL : q * NL + lw < kLoadsA;
     };
-    auto place = [&](int q, bool kmajor, int rows, int u, int ld) {
+    bool up[kGate ? PER : 1];   // a load of 8 rows of the up projection
+    auto place = [&](int q, bool kmajor, int rows, int u, int ld, bool gate = false) {
         if (kmajor) {
             const int cpr = rows / 8;                 // chunks per k row
             const int c = u * 64 + lane;
@@ -165,15 +161,16 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
         } else {
             const int row = u * 8 + lane / 8;
             const int chunk = (lane % 8) ^ row_key<kStep>(row);
-            voff[q] = unsigned(row) * unsigned(ld) * 2u + unsigned(chunk) * 16u;
+            voff[q] = unsigned(gate ? gate_row(row) : row) * unsigned(ld) * 2u + unsigned(chunk) * 16u;
             kofs[q] = chunk * 8;
+            if constexpr (kGate) up[q] = gate && gate_is_up(u * 8);
         }
     };
 #pragma unroll
     for (int q = 0; q < PER; ++q) {
         const int v = q * NL + lw;
         if (of_x(q)) place(q, kXM, BM, v, a_ld);
-        else place(q, kWM, BN, v - kLoadsA, b_ld);
+        else place(q, kWM, BN, v - kLoadsA, b_ld, kGate);
     }
     auto clamp32 = [](size_t v) { return v < 0xffffffffu ? unsigned(v) : 0xffffffffu; };
     // Loads step k0 into stage st. Steps past the last one load nothing (an
@@ -186,6 +183,9 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
             uniform_ptr(a + ka), 0, live ? clamp32(a_bytes - ka * 2) : 0u, 0x00020000);
         const auto rb = __builtin_amdgcn_make_buffer_rsrc(
             uniform_ptr(b + kb), 0, live ? clamp32(b_bytes - kb * 2) : 0u, 0x00020000);
+        const auto ru = __builtin_amdgcn_make_buffer_rsrc(
+            uniform_ptr(kGate ? b + size_t(n) * K : b), 0,
+            kGate && live ? clamp32(b_bytes) : 0u, 0x00020000);
         const int left = k_end - k0;
 #pragma unroll
         for (int q = 0; q < PER; ++q) {
@@ -198,28 +198,44 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
                     kmajor ? 0u : unsigned(k0) * 2u, 0, 0);
             };
             if (of_x(q)) load(ra, kXM);
+            else if (kGate && up[kGate ? q : 0]) load(ru, kWM);
             else load(rb, kWM);
         }
     };
 
     // ---- the epilogue's chunks: kCh consecutive columns of a row, each
     // thread kChunks of them; their inputs load now.
-    constexpr int kCh = BM * BN >= 8 * T ? 8 : 4;
-    constexpr int kCpr = BN / kCh, kTileChunks = BM * BN / kCh;
+    // (Of a gated product's outputs, half as many as its tile has columns.)
+    constexpr int kCols = kGate ? BN / 2 : BN;
+    constexpr int kCh = BM * kCols >= 8 * T ? 8 : 4;
+    constexpr int kCpr = kCols / kCh, kTileChunks = BM * kCols / kCh;
     constexpr int kChunks = (kTileChunks + T - 1) / T;
     // Whole chunks only, unless n leaves a partial one (NT alone; others have
     // n % 8 == 0).
     const bool whole = L != Layout::kNT || n % kCh == 0;
     const bool accumulate = ST == Store::kTn && !split && op.accumulate;
-    float aux[kF32 || ST == Store::kDGelu ? kChunks : 1][kCh];
-    float bias[kBias ? kChunks : 1][kCh];
+    constexpr bool kSlope = ST == Store::kDGelu || ST == Store::kDGated;
+    // Inputs of a second kind: the up projection's bias, or pre.
+    constexpr int kPairs = kGate || ST == Store::kDGated ? 2 : 1;
+    float aux[kF32 || kSlope ? kChunks : 1][kCh * kPairs];
+    float bias[kBias ? kChunks : 1][kCh * kPairs];
 #pragma unroll
     for (int i = 0; i < kChunks; ++i) {
         const int c = i * T + tid;
-        const int row = c < kTileChunks ? m0 + c / kCpr : m, col = n0 + c % kCpr * kCh;
+        const int row = c < kTileChunks ? m0 + c / kCpr : m;
+        const int col = (kGate ? n0 / 2 : n0) + c % kCpr * kCh;
         const int cols = row < m ? n - col : 0;       // valid columns from col on
         const size_t at = y_off + size_t(row) * y_ld + col;
-        if constexpr (kBias) {
+        if constexpr (kGate) {
+#pragma unroll
+            for (int e = 0; e < 2 * kCh; e += 4) {
+                f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                if (op.bias != nullptr && cols > 0)
+                    v = *reinterpret_cast<const f32x4*>(op.bias + (e < kCh ? 0 : n) + col + e % kCh);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) bias[i][e + j] = v[j];
+            }
+        } else if constexpr (kBias) {
             if (whole) {
 #pragma unroll
                 for (int e = 0; e < kCh; e += 4) {
@@ -250,12 +266,14 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
                 for (int e = 0; e < kCh; ++e) aux[i][e] = reads && e < cols ? src[at + e] : 0.0f;
             }
         }
-        if constexpr (ST == Store::kDGelu) {
-            const _Float16* src = static_cast<const _Float16*>(op.aux) + at;
+        if constexpr (kSlope) {
+            // dGated: the gate's, then the up's (kPairs), n values further on.
+            const _Float16* src = static_cast<const _Float16*>(op.aux) +
+                                  (ST == Store::kDGated ? size_t(row) * 2 * n + col : at);
 #pragma unroll
-            for (int e = 0; e < kCh; e += 4) {
+            for (int e = 0; e < kCh * kPairs; e += 4) {
                 f16x4 v = {};
-                if (cols > 0) v = *reinterpret_cast<const f16x4*>(src + e);
+                if (cols > 0) v = *reinterpret_cast<const f16x4*>(src + (e < kCh ? 0 : n) + e % kCh);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) aux[i][e + j] = float(v[j]);
             }
@@ -387,8 +405,30 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
     for (int i = 0; i < kChunks; ++i) {
         const int c = i * T + tid;
         const int r = c / kCpr, cc = c % kCpr * kCh;
-        const int row = m0 + r, col = n0 + cc;
+        const int row = m0 + r, col = (kGate ? n0 / 2 : n0) + cc;
         if (c >= kTileChunks || row >= m || col >= n) continue;
+        if constexpr (kGate) {
+            // Gate columns cc .. of the tile, and 16 behind them the up's.
+            typedef _Float16 hch __attribute__((ext_vector_type(kCh)));
+            const float* at = sums + r * kLd + cc / 16 * 32 + cc % 16;
+            const Gate gate(op.gelu);
+            hch y, pg, pu;
+#pragma unroll
+            for (int e = 0; e < kCh; ++e) {
+                const float g = settled(at[e] + bias[i][e]);
+                const float u = settled(at[16 + e] + bias[i][kCh + e]);
+                y[e] = _Float16(settled(gate.value(g) * u));
+                pg[e] = _Float16(g);
+                pu[e] = _Float16(u);
+            }
+            *reinterpret_cast<hch*>(static_cast<_Float16*>(op.y) + size_t(row) * n + col) = y;
+            if constexpr (ST == Store::kGatedPre) {
+                _Float16* pre = static_cast<_Float16*>(op.aux) + size_t(row) * 2 * n + col;
+                *reinterpret_cast<hch*>(pre) = pg;
+                *reinterpret_cast<hch*>(pre + n) = pu;
+            }
+            continue;
+        }
         float v[kCh];
 #pragma unroll
         for (int e = 0; e < kCh; e += 4) {
@@ -440,6 +480,21 @@ __global__ void __launch_bounds__(NW * 64) gemm_small(Operands op, TileArgs ta) 
             if constexpr (ST == Store::kDGelu) {
 #pragma unroll
                 for (int e = 0; e < kCh; ++e) v[e] = settled(v[e] * gelu_grad(aux[i][e]));
+            }
+            if constexpr (ST == Store::kDGated) {
+                const Gate gate(op.gelu);
+                _Float16* dpre = static_cast<_Float16*>(op.y) + size_t(row) * 2 * n + col;
+                hch du;
+#pragma unroll
+                for (int e = 0; e < kCh; ++e) {
+                    float value, slope;
+                    gate.both(aux[i][e], &value, &slope);
+                    h[e] = _Float16(settled(v[e] * aux[i][kCh * (kPairs - 1) + e] * slope));
+                    du[e] = _Float16(settled(v[e] * value));
+                }
+                *reinterpret_cast<hch*>(dpre) = h;
+                *reinterpret_cast<hch*>(dpre + n) = du;
+                continue;
             }
 #pragma unroll
             for (int e = 0; e < kCh; ++e) h[e] = _Float16(v[e]);
@@ -496,7 +551,13 @@ constexpr double kMostPipeLoad = 1.25;
 
 // Bytes a product writes per output value.
 double out_bytes(Epilogue e) {
-    return e == Epilogue::kBiasGelu || e == Epilogue::kBiasResidual || e == kTnFloat ? 4.0 : 2.0;
+    // (Gated products are planned as one of twice as many columns as outputs.)
+    return e == Epilogue::kBiasGelu || e == Epilogue::kBiasResidual || e == Epilogue::kDGated ||
+                   e == kTnFloat
+               ? 4.0
+           : e == Epilogue::kGated    ? 1.0
+           : e == Epilogue::kGatedPre ? 3.0
+                                      : 2.0;
 }
 
 // Up to how many rounds of 128 x 64 tiles these kernels are faster than
@@ -511,6 +572,8 @@ double out_bytes(Epilogue e) {
 // 520 x 520 672 and 188, 96 x 1000 x 1000 x 520 250 and 273). Either was measured
 // up to 96 rounds (NT 8192 x 50257 x 768, 196 of them: 1486 us and 1592).
 double most_rounds(GemmLayout l, Epilogue e, size_t n, size_t k) {
+    // The gated products, which gemm.hip does not have, past the pipeline's sizes.
+    if (is_gated_epilogue(e)) return kNoEstimate;
     const size_t odd_k = e == Epilogue::kBiasGelu ? 2048
                          : e == Epilogue::kNone || e == Epilogue::kScale ? 1280
                                                                          : 640;
@@ -567,7 +630,7 @@ template <Layout L, Store ST, bool HV>
 hipError_t launch(const SmallPlan& c, const Operands& op, size_t slices, hipStream_t stream) {
     TileArgs ta{};
     ta.tiles_m = (op.m + c.bm - 1) / c.bm;
-    ta.tiles_n = (op.n + c.bn - 1) / c.bn;
+    ta.tiles_n = int(((is_gated(ST) ? gated_width(op.n) : size_t(op.n)) + c.bn - 1) / c.bn);
     const size_t per = size_t(ta.tiles_m) * size_t(ta.tiles_n);
     if (!fits_a_launch(double(per) * double(slices), c.waves)) return hipErrorInvalidValue;
     ta.tiles_per_slice = int(per);
@@ -602,9 +665,11 @@ bool gemm_small_plan(GemmLayout l, Epilogue e, size_t slices, size_t m, size_t n
     SmallConfig forced;
     bool disabled = false;
     const bool force = small_forced(&forced, &disabled);
-    if (disabled || m == 0 || n == 0 || k == 0) return false;
+    // What the pipeline does not take of the gated products nothing else has.
+    const bool only = is_gated_epilogue(e) && !gemm_pipe_eligible(l, e, m, n, k);
+    if ((disabled && !only) || m == 0 || n == 0 || k == 0) return false;
     // A forced pipeline tile means the pipeline, and no pipeline gemm.hip.
-    if (!force && gemm_pipe_override(l, e, m, n, k, views)) return false;
+    if (!force && !only && gemm_pipe_override(l, e, m, n, k, views)) return false;
     int cus = 256;
     if (device_cus(&cus) != hipSuccess) return false;
     const PipeEstimate pipe =
@@ -651,7 +716,7 @@ hipError_t launch_gemm_small(const SmallPlan& c, GemmLayout l, Epilogue e, void*
                              const void* w, const void* bias, void* aux, float scale,
                              size_t slices, size_t m, size_t n, size_t k, bool accumulate,
                              void* partials, hipStream_t stream, bool causal, const HeadView* wv,
-                             const HeadView* yv) {
+                             const HeadView* yv, bool gelu) {
     Operands op{};
     op.y = y;
     op.x = static_cast<const _Float16*>(x);
@@ -665,6 +730,7 @@ hipError_t launch_gemm_small(const SmallPlan& c, GemmLayout l, Epilogue e, void*
     op.n = int(n);
     op.k = int(k);
     op.causal = causal ? 1 : 0;
+    op.gelu = gelu ? 1 : 0;
     const bool hv = wv != nullptr && yv != nullptr;
     if (hv) {
         op.wv = *wv;
@@ -679,11 +745,16 @@ hipError_t launch_gemm_small(const SmallPlan& c, GemmLayout l, Epilogue e, void*
         case Epilogue::kBiasResidual:
             return launch<Layout::kNT, Store::kBiasResidual, false>(c, op, slices, stream);
         case Epilogue::kScale: return launch<Layout::kNT, Store::kScale, false>(c, op, slices, stream);
+        case Epilogue::kGated: return launch<Layout::kNT, Store::kGated, false>(c, op, slices, stream);
+        case Epilogue::kGatedPre:
+            return launch<Layout::kNT, Store::kGatedPre, false>(c, op, slices, stream);
         default: return hipErrorInvalidValue;
         }
     }
     if (l == GemmLayout::kNN) {
         if (e == Epilogue::kDGelu) return launch<Layout::kNN, Store::kDGelu, false>(c, op, slices, stream);
+        if (e == Epilogue::kDGated)
+            return launch<Layout::kNN, Store::kDGated, false>(c, op, slices, stream);
         if (e != Epilogue::kNone) return hipErrorInvalidValue;
         return hv ? launch<Layout::kNN, Store::kNone, true>(c, op, slices, stream)
                   : launch<Layout::kNN, Store::kNone, false>(c, op, slices, stream);

@@ -22,7 +22,12 @@ constexpr size_t kGemmBatchedMaxM = 1024;
 constexpr size_t kGemmMaxBatches = 65535;
 
 // GEMM epilogues (what happens to the FP32 sums before the single rounding).
-enum class Epilogue { kNone, kBias, kBiasGelu, kBiasResidual, kDGelu, kScale };
+enum class Epilogue {
+    kNone, kBias, kBiasGelu, kBiasResidual, kDGelu, kScale, kGated, kGatedPre, kDGated
+};
+constexpr bool is_gated_epilogue(Epilogue e) {
+    return e == Epilogue::kGated || e == Epilogue::kGatedPre || e == Epilogue::kDGated;
+}
 
 hipError_t launch_gemm_nt(void* y, const void* x, const void* w, const void* bias,
                           void* aux, Epilogue e, size_t m, size_t n, size_t k,
@@ -50,7 +55,8 @@ hipError_t launch_gemm_pipe(GemmLayout l, Epilogue e, void* y, const void* x, co
                             const void* bias, void* aux, float scale, size_t slices, size_t m,
                             size_t n, size_t k, bool accumulate, void* partials, int split_len,
                             hipStream_t stream, bool causal = false,
-                            const HeadView* wv = nullptr, const HeadView* yv = nullptr);
+                            const HeadView* wv = nullptr, const HeadView* yv = nullptr,
+                            bool gelu = false);
 // The pipeline's estimated time for a product, us past a launch's own, with
 // the tile (and TN split, up to max_splits) it would choose, and that tile's
 // count per CU; infinite where it does not take the shape. views: the product
@@ -82,9 +88,19 @@ hipError_t launch_gemm_small(const SmallPlan& plan, GemmLayout l, Epilogue e, vo
                              const void* w, const void* bias, void* aux, float scale,
                              size_t slices, size_t m, size_t n, size_t k, bool accumulate,
                              void* partials, hipStream_t stream, bool causal = false,
-                             const HeadView* wv = nullptr, const HeadView* yv = nullptr);
+                             const HeadView* wv = nullptr, const HeadView* yv = nullptr,
+                             bool gelu = false);
 hipError_t launch_gemm_nn(void* y, const void* x, const void* w, const void* aux, Epilogue e,
                           size_t m, size_t n, size_t k, hipStream_t stream);
+// The gated product y = act(gate) up of both projections of x, w holding n rows of
+// either, and its gradient dpre = [s up act'(gate), s act(gate)] of s = x w. The plans
+// and limits above take the gated product as one of gated_width(n) columns. Up to
+// kGatedMaxOutputs outputs, whose tiles fit a launch.
+constexpr size_t kGatedMaxOutputs = size_t{1} << 34;
+hipError_t launch_gemm_nt_gated(void* y, void* pre, const void* x, const void* w, const void* bias,
+                                bool gelu, size_t m, size_t n, size_t k, hipStream_t stream);
+hipError_t launch_gemm_nn_dgated(void* dpre, const void* x, const void* w, const void* pre,
+                                 bool gelu, size_t m, size_t n, size_t k, hipStream_t stream);
 // Number of k splits TN uses for m x n x k on this device (1 = none).
 hipError_t gemm_tn_splits(size_t m, size_t n, size_t k, int* splits, int* split_len);
 hipError_t gemm_tn_workspace(size_t m, size_t n, size_t k, size_t* bytes);

@@ -24,6 +24,7 @@ ATTENTION_HEADER = ROOT / "include" / "flint" / "flint_attention.h"
 PACKED_HEADER = ROOT / "include" / "flint" / "flint_packed.h"
 PAGED_HEADER = ROOT / "include" / "flint" / "flint_paged.h"
 ROTARY_HEADER = ROOT / "include" / "flint" / "flint_rotary.h"
+GATED_HEADER = ROOT / "include" / "flint" / "flint_gated.h"
 LOGPROBS_HEADER = ROOT / "include" / "flint" / "flint_logprobs.h"
 TUNING_HEADER = ROOT / "include" / "flint" / "flint_tuning.h"
 LIBRARY = ROOT / "build" / "release" / "bin" / "libflint.so"
@@ -146,6 +147,9 @@ SIGNATURES = {
     "flint_rotary_plan_bytes": (I, [Z, ctypes.POINTER(Z)]),
     "flint_rotary_plan": (I, [P, ctypes.POINTER(RotaryAngles), P]),
     "flint_rotary": (I, [P] * 6 + [ctypes.POINTER(RotaryShape), I, P]),
+    # flint_gated.h (no counterpart in the reference)
+    "flint_gemm_nt_gated": (I, [P, P, P, P, P, Z, Z, Z, I, P]),
+    "flint_gemm_nn_dgated": (I, [P, P, P, P, Z, Z, Z, I, P]),
     # flint_tuning.h (no counterpart in the reference)
     "flint_set_tuning": (I, [ctypes.c_char_p, ctypes.c_char_p]),
     "flint_gemm_nt_batched": (I, [P, P, P, Z, Z, Z, Z, F, P]),
@@ -485,6 +489,20 @@ class Flint:
             pointer(offsets), pointer(cached), pointer(table), shape, scale, pointer(workspace),
             workspace_bytes, stream_handle(stream)))
 
+    # -- the gated feed-forward product (flint_gated.h) -------------------------
+    ACTIVATIONS = {"silu": 0, "gelu": 1}
+
+    def gemm_nt_gated(self, y, pre, x, w, bias, m, n, k, activation="silu", stream=None):
+        """pre and bias may be None; activation is "silu", "gelu" or the C value."""
+        self.check(self.lib.flint_gemm_nt_gated(
+            pointer(y), pointer(pre), pointer(x), pointer(w), pointer(bias), m, n, k,
+            self.ACTIVATIONS.get(activation, activation), stream_handle(stream)))
+
+    def gemm_nn_dgated(self, dpre, x, w, pre, m, n, k, activation="silu", stream=None):
+        self.check(self.lib.flint_gemm_nn_dgated(
+            pointer(dpre), pointer(x), pointer(w), pointer(pre), m, n, k,
+            self.ACTIVATIONS.get(activation, activation), stream_handle(stream)))
+
     # -- rotary positions (flint_rotary.h) ------------------------------------
     @staticmethod
     def rotary_angles(width, base=10000.0, factor=1.0, original=0.0, low=1.0, high=32.0,
@@ -716,6 +734,6 @@ def declared_functions(header=None):
 
     headers = ([header] if header is not None
                else [HEADER, TRAIN_HEADER, NOALLOC_HEADER, ATTENTION_HEADER, PACKED_HEADER,
-                     PAGED_HEADER, LOGPROBS_HEADER, ROTARY_HEADER, TUNING_HEADER])
+                     PAGED_HEADER, LOGPROBS_HEADER, ROTARY_HEADER, GATED_HEADER, TUNING_HEADER])
     text = "".join(Path(h).read_text() for h in headers)
     return re.findall(r"FLINT_API\s+[^;(]*?\b(flint_\w+)\s*\(", text)
