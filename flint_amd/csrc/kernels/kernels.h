@@ -220,6 +220,14 @@ hipError_t launch_attention_paged(void* o, void* k_pages, void* v_pages, const v
                                   const void* cached, const void* table,
                                   const flint_paged_shape& s, float scale, void* workspace,
                                   hipStream_t stream);
+// The same over a cache of 8-bit values (paged8.hip).
+constexpr size_t kPaged8MaxBlock = 128;
+size_t paged8_workspace(const flint_paged_shape& s);
+hipError_t launch_attention_paged8(void* o, void* k_pages, void* k_scales, void* v_pages,
+                                   void* v_scales, const void* q, const void* k, const void* v,
+                                   const void* offsets, const void* cached, const void* table,
+                                   const flint_paged_shape& s, size_t block, float scale,
+                                   void* workspace, hipStream_t stream);
 // Rotary positions (rotary.hip).
 constexpr size_t kRotaryMaxWidth = 1024;
 hipError_t launch_rotary_plan(void* plan, const flint_rotary_angles& angles, hipStream_t stream);

@@ -25,6 +25,7 @@ PACKED_HEADER = ROOT / "include" / "flint" / "flint_packed.h"
 PAGED_HEADER = ROOT / "include" / "flint" / "flint_paged.h"
 ROTARY_HEADER = ROOT / "include" / "flint" / "flint_rotary.h"
 GATED_HEADER = ROOT / "include" / "flint" / "flint_gated.h"
+PAGED8_HEADER = ROOT / "include" / "flint" / "flint_paged8.h"
 LOGPROBS_HEADER = ROOT / "include" / "flint" / "flint_logprobs.h"
 TUNING_HEADER = ROOT / "include" / "flint" / "flint_tuning.h"
 LIBRARY = ROOT / "build" / "release" / "bin" / "libflint.so"
@@ -150,6 +151,9 @@ SIGNATURES = {
     # flint_gated.h (no counterpart in the reference)
     "flint_gemm_nt_gated": (I, [P, P, P, P, P, Z, Z, Z, I, P]),
     "flint_gemm_nn_dgated": (I, [P, P, P, P, Z, Z, Z, I, P]),
+    # flint_paged8.h (no counterpart in the reference)
+    "flint_attention_paged8_workspace": (I, [ctypes.POINTER(PagedShape), Z, ctypes.POINTER(Z)]),
+    "flint_attention_paged8": (I, [P] * 11 + [ctypes.POINTER(PagedShape), Z, F, P, Z, P]),
     # flint_tuning.h (no counterpart in the reference)
     "flint_set_tuning": (I, [ctypes.c_char_p, ctypes.c_char_p]),
     "flint_gemm_nt_batched": (I, [P, P, P, Z, Z, Z, Z, F, P]),
@@ -489,6 +493,24 @@ class Flint:
             pointer(offsets), pointer(cached), pointer(table), shape, scale, pointer(workspace),
             workspace_bytes, stream_handle(stream)))
 
+    # -- the same over a cache of 8-bit values (flint_paged8.h) -----------------
+    def attention_paged8_workspace(self, shape, block):
+        out = Z(0)
+        self.check(self.lib.flint_attention_paged8_workspace(shape, block, ctypes.byref(out)))
+        return out.value
+
+    def attention_paged8(self, o, k_pages, k_scales, v_pages, v_scales, q, k, v, offsets, cached,
+                         table, shape, block, scale, workspace=None, workspace_bytes=None,
+                         stream=None):
+        if workspace is None:
+            workspace = scratch(self.attention_paged8_workspace(shape, block), stream)
+        if workspace_bytes is None:
+            workspace_bytes = workspace.numel() * workspace.element_size()
+        self.check(self.lib.flint_attention_paged8(
+            pointer(o), pointer(k_pages), pointer(k_scales), pointer(v_pages), pointer(v_scales),
+            pointer(q), pointer(k), pointer(v), pointer(offsets), pointer(cached), pointer(table),
+            shape, block, scale, pointer(workspace), workspace_bytes, stream_handle(stream)))
+
     # -- the gated feed-forward product (flint_gated.h) -------------------------
     ACTIVATIONS = {"silu": 0, "gelu": 1}
 
@@ -734,6 +756,7 @@ def declared_functions(header=None):
 
     headers = ([header] if header is not None
                else [HEADER, TRAIN_HEADER, NOALLOC_HEADER, ATTENTION_HEADER, PACKED_HEADER,
-                     PAGED_HEADER, LOGPROBS_HEADER, ROTARY_HEADER, GATED_HEADER, TUNING_HEADER])
+                     PAGED_HEADER, LOGPROBS_HEADER, ROTARY_HEADER, GATED_HEADER, PAGED8_HEADER,
+                     TUNING_HEADER])
     text = "".join(Path(h).read_text() for h in headers)
     return re.findall(r"FLINT_API\s+[^;(]*?\b(flint_\w+)\s*\(", text)
