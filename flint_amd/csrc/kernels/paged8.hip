@@ -8,11 +8,11 @@
 // paged.hip's products read, and only the cache's own rounding is left.
 //
 // Reading the cache bounds few rows, at half of paged.hip's bytes. Codes go to LDS
-// directly, two tiles ahead of their use: held in registers so long they spilled. K's
-// are decoded as they become operands (a lane has one row, and its scale), V's into a
-// tile of halves, for the transposing reads. Where rows are many, a tile's four waves
-// decode a quarter of it each. The new rows, FP16 as they were given, lie in tiles of
-// their own in front of the cached ones, so that no tile mixes the two.
+// directly, two tiles ahead of their use (held in registers so long they spilled), and
+// are decoded as they become operands, V's behind a transposing read of bytes. Where
+// rows are many, a tile's four waves decode a quarter of it each, to halves in LDS. The
+// new rows, FP16 as they were given, lie in tiles of their own in front of the cached
+// ones, so that no tile mixes the two.
 //
 // The rows are stored behind the attention by the launch that joins the parts: a block's
 // scale may grow with a new row, which rewrites rows that the attention reads.
@@ -41,23 +41,39 @@ __device__ __forceinline__ float scale_of(int b) {
     return __builtin_bit_cast(float, scale_byte(b) << 23);
 }
 
-// 16 codes of a row, and their values.
-__device__ __forceinline__ void decode(const i32x4& codes, float scale, f16x8* low, f16x8* high) {
+// 8 codes' values, at one scale or at one each.
+__device__ __forceinline__ f16x8 decode(const i32x2& codes, float scale) {
+    f16x8 out;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < 2; ++j) {
         const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale, false);
         const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale, true);
-        f16x8& to = j < 2 ? *low : *high;
-        to[4 * (j & 1)] = a[0];
-        to[4 * (j & 1) + 1] = a[1];
-        to[4 * (j & 1) + 2] = b[0];
-        to[4 * (j & 1) + 3] = b[1];
+        out[4 * j] = a[0];
+        out[4 * j + 1] = a[1];
+        out[4 * j + 2] = b[0];
+        out[4 * j + 3] = b[1];
     }
+    return out;
+}
+__device__ __forceinline__ f16x8 decode(const i32x2& codes, const float (&scale)[8]) {
+    f16x8 out;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        out[4 * j] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale[4 * j], false)[0];
+        out[4 * j + 1] =
+            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale[4 * j + 1], false)[1];
+        out[4 * j + 2] =
+            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale[4 * j + 2], true)[0];
+        out[4 * j + 3] =
+            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], scale[4 * j + 3], true)[1];
+    }
+    return out;
 }
 
 // Reads the cached rows of one sequence and kv head in tiles of KEYS positions. Codes
-// lie in LDS as rows of HD bytes, 16-byte chunk c of row r at position c ^ key(r): 8 bytes
-// of one chunk of 32 consecutive rows fall on each bank twice at most.
+// lie in LDS as rows of HD bytes, 16-byte chunk c of row r at position c ^ key(r). Two
+// reads have to spread over the banks, 32 lanes at a time: one chunk of 16 consecutive
+// rows (V), and one of the 16 rows whose bit 2 is the same (K).
 template <int HD, int KEYS>
 struct Cached {
     static constexpr int kLanes = HD / 16;           // of a row in a load
@@ -73,7 +89,8 @@ struct Cached {
           cached(it.seq.cached), lane(lane_) {}
 
     static __device__ __forceinline__ int key(int row) {
-        return HD == 64 ? (row >> 2) & 3 : (row >> 1) & 7;
+        const int top = (row >> 4 ^ row >> 2) & 1;
+        return HD == 64 ? top << 1 | (row >> 3 & 1) : top << 2 | (row >> 3 & 1) << 1 | (row >> 1 & 1);
     }
     // The row, and the first column of the 16, that this lane has of load u.
     __device__ __forceinline__ int row_of(int u) const { return u * kRows + lane / kLanes; }
@@ -121,8 +138,7 @@ struct Cached {
         i32x4 c = *reinterpret_cast<const i32x4*>(codes + lane * 16);
 #pragma unroll
         for (int j = 0; j < 4; ++j) c[j] = ok ? c[j] : 0;
-        f16x8 low, high;
-        decode(c, scale, &low, &high);
+        const f16x8 low = decode(i32x2{c[0], c[1]}, scale), high = decode(i32x2{c[2], c[3]}, scale);
         *reinterpret_cast<f16x8*>(tile + row * HD + (chunk ^ T::key(row)) * 8) = low;
         *reinterpret_cast<f16x8*>(tile + row * HD + ((chunk + 1) ^ T::key(row)) * 8) = high;
     }
@@ -153,22 +169,25 @@ __device__ __forceinline__ void load_new(const PagedArgs& a, const Item& it, int
     }
 }
 
-// A tile's softmax and product with V (halves): products(s, zero) gives the scores, of
-// which the keys up to `limit` (the lane's own) are seen, of the runs of 8 in `valid`; all
-// of them where `whole` says so.
-template <int HD, int KEYS, class Products>
-__device__ __forceinline__ void take_tile(Rows<HD, KEYS>& w, const Products& products,
-                                          const _Float16* vt, const Frags<HD>& fo, bool whole,
-                                          int limit, unsigned valid, float c, int h) {
-    constexpr int HB = KEYS / 32;
-    auto scores = [&](f32x16 (&s)[HB], unsigned zero) __attribute__((always_inline)) {
+// A tile of halves whose keys up to `limit` (the lane's own) are seen, of the runs of 8
+// in `valid`; all of them where `whole` says so.
+template <int HD, int KEYS>
+__device__ __forceinline__ void tile(Rows<HD, KEYS>& w, const _Float16* kt, const _Float16* vt,
+                                     const Frags<HD>& fo, bool whole, int limit, unsigned valid,
+                                     float c, int h) {
+    using R = Rows<HD, KEYS>;
+    auto scores = [&](f32x16 (&s)[R::HB], unsigned zero) __attribute__((always_inline)) {
 #pragma unroll
-        for (int hb = 0; hb < HB; ++hb) s[hb] = f32x16{};
-        products(s, zero);
+        for (int hb = 0; hb < R::HB; ++hb) s[hb] = f32x16{};
+#pragma unroll
+        for (int kk = 0; kk < R::KK; ++kk)
+#pragma unroll
+            for (int hb = 0; hb < R::HB; ++hb)
+                s[hb] = mfma(fo.row(kt + zero, hb, kk), w.q[kk], s[hb]);
         if (whole) return c;
         const int seen = limit - 4 * h + int(zero);
 #pragma unroll
-        for (int hb = 0; hb < HB; ++hb)
+        for (int hb = 0; hb < R::HB; ++hb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 s[hb][r] = 32 * hb + result_row(r, 0) <= seen && (valid >> (4 * hb + (r >> 2)) & 1)
@@ -177,21 +196,6 @@ __device__ __forceinline__ void take_tile(Rows<HD, KEYS>& w, const Products& pro
         return 1.0f;
     };
     w.take(vt, fo, scores);
-}
-
-// The same with K a tile of halves.
-template <int HD, int KEYS>
-__device__ __forceinline__ void tile(Rows<HD, KEYS>& w, const _Float16* kt, const _Float16* vt,
-                                     const Frags<HD>& fo, bool whole, int limit, unsigned valid,
-                                     float c, int h) {
-    using R = Rows<HD, KEYS>;
-    take_tile(w, [&](f32x16 (&s)[R::HB], unsigned zero) __attribute__((always_inline)) {
-#pragma unroll
-        for (int kk = 0; kk < R::KK; ++kk)
-#pragma unroll
-            for (int hb = 0; hb < R::HB; ++hb)
-                s[hb] = mfma(fo.row(kt + zero, hb, kk), w.q[kk], s[hb]);
-    }, vt, fo, whole, limit, valid, c, h);
 }
 
 // The tiles of a block's part: new rows' tiles, up to the one of the block's last row,
@@ -206,38 +210,163 @@ __device__ __forceinline__ void part_of8(const PagedArgs& a, const Item& it, int
     *to = int((long long)(tiles) * (it.part + 1) / it.parts);
 }
 
-// Few rows. A wave's LDS: kRing tiles of codes (K and V each), and one tile of V's
-// halves; the new rows' K goes through the last tile of codes.
-template <int HD>
-__global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged8_few(Paged8Args a) {
+// RB blocks of 16 rows and tiles of 32 keys: up to 16 rows (one token of up to 16 heads on
+// one) take half the registers and exponentials of 32. The 16 rows of K that an MFMA takes
+// are keys 8 i + 4 kb + 0 .. 3, i < 4: lane group g (of 16) then has the scores of keys
+// 8g .. 8g + 7 of its query, in order, which is what the product with V wants of it, and
+// one page and, from 8 positions a block on, one scale of V.
+template <int HD, int RB>
+struct FewRows {
+    static constexpr int KK = HD / 32, DB = HD / 16;
+    f16x8 q[RB][KK];
+    float m[RB], l[RB];
+    bool started = false;
+    f32x4 acc[RB][DB] = {};
+
+    __device__ __forceinline__ FewRows() {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) m[rb] = kFloor, l[rb] = 0.0f;
+    }
+
+    __device__ __forceinline__ void load_q(const PagedArgs& a, const Item& it, int head, int lane) {
+        const int first = it.block * kFewRows, rows = it.seq.count * a.group;
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            const int row = first + 16 * rb + (lane & 15), place = row / a.group;
+            const _Float16* at = a.q + size_t(it.seq.first + place) * a.q_stride +
+                                 size_t(head * a.group + row - place * a.group) * HD +
+                                 8 * (lane >> 4);
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk) {
+                q[rb][kk] = row < rows ? *reinterpret_cast<const f16x8*>(at + 32 * kk) : f16x8{};
+                if (a.negative) q[rb][kk] = -q[rb][kk];
+            }
+        }
+    }
+
+    // One tile: keys(kb, kk) and values(db) are operands of K and V; key 8g + i of the
+    // lane's group is seen where i <= seen[rb]. (The softmax is attention_tiles.h's: the
+    // reference moves at a wave's first tile and where a lane's sum passes kSumLimit.)
+    template <class Keys, class Values>
+    __device__ __forceinline__ void tile(const Keys& keys, const Values& values, bool whole,
+                                         const int (&seen)[RB], float c) {
+        f16x8 p[RB];
+        for (;;) {
+            f32x4 s[RB][2] = {};
+#pragma unroll
+            for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const f16x8 k = keys(kb, kk);
+#pragma unroll
+                    for (int rb = 0; rb < RB; ++rb)
+                        s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q[rb][kk], s[rb][kb],
+                                                                           0, 0, 0);
+                }
+            float by = c;
+            if (!whole) {
+                by = 1.0f;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        s[rb][i >> 2][i & 3] = i <= seen[rb] ? s[rb][i >> 2][i & 3] * c : -INFINITY;
+            }
+            const bool move = !started;
+            if (move) {
+                started = true;
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) {
+                    float mx = s[rb][0][0];
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) mx = fmaxf(mx, s[rb][i >> 2][i & 3]);
+                    mx *= by;
+                    mx = fmaxf(mx, __shfl_xor(mx, 16));
+                    const float m_new = fmaxf(m[rb], fmaxf(mx, xor32(mx)) - kBelow);
+                    const float scale = __builtin_amdgcn_exp2f(m[rb] - m_new);
+                    l[rb] *= scale;
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) acc[rb][db] *= scale;
+                    m[rb] = m_new;
+                }
+            }
+            float sum[RB] = {};
+            bool past = false;
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(
+                        __builtin_fmaf(s[rb][i >> 2][i & 3], by, -m[rb]));
+                    p[rb][i] = _Float16(e);
+                    sum[rb] += e;
+                }
+                past |= sum[rb] > kSumLimit;
+            }
+            if (move || !__any(past)) {
+#pragma unroll
+                for (int rb = 0; rb < RB; ++rb) l[rb] += sum[rb];
+                break;
+            }
+            started = false;
+        }
+#pragma unroll
+        for (int db = 0; db < DB; ++db) {
+            const f16x8 v = values(db);
+#pragma unroll
+            for (int rb = 0; rb < RB; ++rb)
+                acc[rb][db] =
+                    __builtin_amdgcn_mfma_f32_16x16x32_f16(v, p[rb], acc[rb][db], 0, 0, 0);
+        }
+    }
+
+    // Leaves O^T [HD][32] and the maxima and sums for few_joined.
+    __device__ __forceinline__ void leave(float* own, float2* sums, int lane) {
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) {
+            l[rb] += __shfl_xor(l[rb], 16);
+            l[rb] += xor32(l[rb]);
+            const int row = 16 * rb + (lane & 15);
+#pragma unroll
+            for (int db = 0; db < DB; ++db)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    own[(16 * db + 4 * (lane >> 4) + r) * 32 + row] = acc[rb][db][r];
+            if (lane < 16) sums[row] = float2{m[rb], l[rb]};
+        }
+    }
+};
+
+// Few rows. A wave's LDS: kRing tiles of codes, K and V each; the new rows, as halves,
+// take the place of the last two. FINE: blocks of fewer than 8 positions, so that each
+// of a lane's 8 keys may have its own scale of V.
+template <int HD, int RB, bool FINE>
+__global__ void __launch_bounds__(kFewThreads, HD == 64 ? 4 / RB : 2) paged8_few(Paged8Args a) {
     using P = Plan<HD, false>;
     constexpr int kKeys = P::kKeys, kW = kFewWaves, kRing = 3;
     using C = Cached<HD, kKeys>;
-    using R = Rows<HD, kKeys>;
+    using R = FewRows<HD, RB>;
     constexpr int kCodes = kKeys * HD;                      // bytes of a tile of K
-    constexpr int kWave = (kRing + 1) * 2 * kCodes;         // bytes of a wave
+    constexpr int kWave = kRing * 2 * kCodes;               // bytes of a wave
     constexpr int kBatch = 64 / C::kRuns;                   // tiles of a load of the table
     constexpr unsigned kAll = (1u << C::kRuns) - 1;
     // One LDS object: with several the compiler waits for the loads under way.
     __shared__ __attribute__((aligned(16))) unsigned char lds[kW * kWave + kW * 32 * sizeof(float2)];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int fr = lane & 31, h = lane >> 5;
+    const int g = lane >> 4, i16 = lane & 15;
     const int head = int(blockIdx.x % unsigned(a.p.kv_heads));
     Item it;
     if (!find_item<HD, false, true>(a.p, int(blockIdx.x / unsigned(a.p.kv_heads)), lane, &it))
         return;
     store_splits(a.p, it, head);
-    const int rows = it.seq.count * a.p.group, first_row = it.block * kFewRows;
     const int cached = it.seq.cached;
-    const Frags<HD> fo(lane);
     R w;
     const C reader(a, it, head, lane);
     int fresh, from, to;
     part_of8(a.p, it, kFewRows, kKeys, &fresh, &from, &to);
     unsigned char* const mine = lds + wave * kWave;
     auto codes_at = [&](int slot) { return mine + slot * 2 * kCodes; };
-    _Float16* const vt = reinterpret_cast<_Float16*>(codes_at(kRing));
     // Tile 0 of the list is the new rows' (few rows are at most 32 new ones); the wave's
     // n-th cached tile is first + kW n, up to `end`. Past it the loads take the last one
     // again, so that every wait counts the same loads.
@@ -249,41 +378,78 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged8_few(Page
     auto look = [&](int n) {
         return reader.entry(tile_of(n + lane / C::kRuns) * kKeys + lane % C::kRuns * 8);
     };
-    if (takes_new) {
-        _Float16* kt = reinterpret_cast<_Float16*>(codes_at(kRing - 1));
-        load_new<HD, kKeys>(a.p, it, head, 0, kt, vt, 0, 1, lane);
-    }
+    _Float16* const new_k = reinterpret_cast<_Float16*>(codes_at(kRing - 2));
+    _Float16* const new_v = reinterpret_cast<_Float16*>(codes_at(kRing - 1));
+    if (takes_new) load_new<HD, kKeys>(a.p, it, head, 0, new_k, new_v, 0, 1, lane);
     int entries = 0, ahead = 0;        // of this batch of tiles, of the next
     int scales[kRing];                 // of a tile: lane l K's row l, or V's row l - 32
     unsigned valid[kRing];
     auto issue = [&](int n, int slot) __attribute__((always_inline)) {
         const int t = tile_of(n), batch = n % kBatch * C::kRuns;
-        const int own = __shfl(entries, batch + fr / 8);
         const unsigned runs = unsigned(__ballot(reader.held(entries)) >> batch) & kAll;
-        const int left = cached - t * kKeys;   // a run past the cache counts as there
-        valid[slot] = runs | (left >= kKeys ? 0u : kAll << ((left + 7) / 8)) & kAll;
-        scales[slot] = (h ? a.v_scales : a.k_scales)[reader.place(own, t * kKeys + fr).scale];
+        valid[slot] = runs;
+        const int own = __shfl(entries, batch + (lane & 31) / 8);
+        scales[slot] =
+            (lane < 32 ? a.k_scales : a.v_scales)[reader.place(own, t * kKeys + (lane & 31)).scale];
         unsigned char *const k = codes_at(slot), *const v = k + kCodes;
 #pragma unroll
         for (int u = 0; u < C::kLoads; ++u)
             reader.load(k + u * 1024, v + u * 1024, __shfl(entries, batch + reader.row_of(u) / 8), t,
                         u);
     };
+    constexpr int kTileLoads = 2 * C::kLoads;
     if (count > 0) {
         entries = look(0);
         ahead = look(kBatch);
 #pragma unroll
-        for (int n = 0; n < kRing - 1; ++n) issue(n, n);
+        for (int n = 0; n < kRing - 2; ++n) issue(n, n);
+        if (!takes_new) issue(kRing - 2, kRing - 2);
     }
-    w.load_q(a.p, it, head, first_row + fr, rows, h);
+    w.load_q(a.p, it, head, lane);
     if (takes_new) {
-        if (count > 0) wait_vmcnt<(kRing - 1) * 2 * C::kLoads>();
+        if (count > 0) wait_vmcnt<(kRing - 2) * kTileLoads>();
         else wait_vmcnt<0>();
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
-        tile(w, reinterpret_cast<const _Float16*>(codes_at(kRing - 1)), vt, fo, false,
-             (first_row + fr) / a.p.group, kAll, a.p.c, h);
+        using T = Tile<HD>;
+        int seen[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb)
+            seen[rb] = (it.block * kFewRows + 16 * rb + i16) / a.p.group - 8 * g;
+        w.tile([&](int kb, int kk) {
+            const int row = i16 / 4 * 8 + kb * 4 + i16 % 4;
+            return *reinterpret_cast<const f16x8*>(new_k + row * HD + ((4 * kk + g) ^ T::key(row)) * 8);
+        }, [&](int db) {
+            f16x8 v;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int row = 8 * g + j, d = 16 * db + i16;
+                v[j] = new_v[row * HD + ((d / 8) ^ T::key(row)) * 8 + d % 8];
+            }
+            return v;
+        }, false, seen, a.p.c);
         asm volatile("" ::: "memory");
+        if (count > 0) issue(kRing - 2, kRing - 2);
+    }
+    // Where this lane's operands lie in the first tile of codes, the others' being a
+    // constant further on: 8 of row 8 (i / 4) + 4 kb + i % 4 of K; of V, for the transposing
+    // read, 8 of the 16 columns of row 8g + i / 2.
+    const unsigned base = unsigned(reinterpret_cast<uintptr_t>((lds_byte*)mine));
+    unsigned k_at[2][R::KK], v_at[R::DB];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int kk = 0; kk < R::KK; ++kk) {
+            const int row = i16 / 4 * 8 + kb * 4 + i16 % 4;
+            k_at[kb][kk] =
+                base + unsigned(row * HD + (((2 * kk + g / 2) ^ C::key(row)) * 16) + 8 * (g & 1));
+            asm volatile("" : "+v"(k_at[kb][kk]));
+        }
+#pragma unroll
+    for (int db = 0; db < R::DB; ++db) {
+        const int row = 8 * g + i16 / 2;
+        v_at[db] = base + unsigned(row * HD + ((db ^ C::key(row)) * 16) + 8 * (i16 & 1));
+        asm volatile("" : "+v"(v_at[db]));
     }
     auto step = [&](int n, auto slot_c) __attribute__((always_inline)) {
         constexpr int slot = decltype(slot_c)::value, next = (slot + kRing - 1) % kRing;
@@ -295,40 +461,57 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged8_few(Page
         // The slot's last reads were a step ago.
         asm volatile("" ::: "memory");
         issue(ahead_n, next);
-        wait_vmcnt<(kRing - 1) * 2 * C::kLoads>();   // the newer tiles' loads, at least
+        wait_vmcnt<(kRing - 1) * kTileLoads>();   // the newer tiles' loads, at least
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("" ::: "memory");
-        const unsigned char* const k = codes_at(slot);
-        const int t = tile_of(n), limit = cached - 1 - t * kKeys;
+        const int t = tile_of(n);
+        // The keys of the lane's group that are cached positions with a page: its first
+        // `keys`. V's codes behind them become zeros.
+        const int left = cached - t * kKeys;
+        const bool whole = left >= kKeys && valid[slot] == kAll;
+        const int keys = valid[slot] >> g & 1 ? min(max(left - 8 * g, 0), 8) : 0;
+        const unsigned low = keys >= 4 ? ~0u : (1u << 8 * keys) - 1;
+        const unsigned high = keys >= 8 ? ~0u : keys <= 4 ? 0u : (1u << 8 * (keys - 4)) - 1;
+        // V's are read under the softmax, where they have registers that long.
+        constexpr bool kEarly = HD * RB <= 128;
+        constexpr int kTogether = kEarly ? R::DB : 4;
+        i32x2 raw[kTogether];
+        auto read_v = [&](int first_db) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < C::kLoads; ++u) {
-            const int row = reader.row_of(u);
-            reader.put(k + kCodes + u * 1024, vt, u, row <= limit && (valid[slot] >> (row / 8) & 1),
-                       scale_of(__shfl(scales[slot], 32 + row)));
-        }
-        const float k_scale = scale_of(__shfl(scales[slot], fr));
-        __builtin_amdgcn_wave_barrier();
-        asm volatile("" ::: "memory");
-        take_tile(w, [&](f32x16 (&s)[1], unsigned zero) __attribute__((always_inline)) {
-            // 16 codes of a row are two k-steps' operands of either half of the wave:
-            // lane half h has columns 16 kk + 8h ..
-#pragma unroll
-            for (int kk = 0; kk < R::KK; ++kk) {
-                const i32x2 c = *reinterpret_cast<const i32x2*>(
-                    k + zero + fr * HD + ((kk ^ C::key(fr)) * 16 + 8 * h));
-                f16x8 f;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[j], k_scale, false);
-                    const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c[j], k_scale, true);
-                    f[4 * j] = lo[0];
-                    f[4 * j + 1] = lo[1];
-                    f[4 * j + 2] = hi[0];
-                    f[4 * j + 3] = hi[1];
-                }
-                s[0] = mfma(f, w.q[kk], s[0]);
+            for (int i = 0; i < kTogether; ++i) {
+                const unsigned at = v_at[first_db + i];
+                i32x2 r;
+                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2"
+                             : "=v"(r) : "v"(at), "i"((2 * slot + 1) * kCodes));
+                raw[i] = r;
             }
-        }, vt, fo, limit >= kKeys - 1 && valid[slot] == kAll, limit, valid[slot], a.p.c, h);
+        };
+        if constexpr (kEarly) read_v(0);
+        float k_scale[2], v_scale[FINE ? 8 : 1];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+            k_scale[kb] = scale_of(__shfl(scales[slot], i16 / 4 * 8 + kb * 4 + i16 % 4));
+#pragma unroll
+        for (int j = 0; j < (FINE ? 8 : 1); ++j)
+            v_scale[j] = scale_of(__shfl(scales[slot], 32 + 8 * g + j));
+        int seen[RB];
+#pragma unroll
+        for (int rb = 0; rb < RB; ++rb) seen[rb] = keys - 1;
+        w.tile([&](int kb, int kk) __attribute__((always_inline)) {
+            const auto* at = (__attribute__((address_space(3))) const i32x2*)(
+                uintptr_t(k_at[kb][kk] + unsigned(2 * slot * kCodes)));
+            const i32x2 c = *at;
+            return decode(c, k_scale[kb]);
+        }, [&](int db) __attribute__((always_inline)) {
+            if (db % kTogether == 0) {
+                if constexpr (!kEarly) read_v(db);
+                wait_lds();
+            }
+            const i32x2 r = raw[db % kTogether];
+            const i32x2 c = {int(unsigned(r[0]) & low), int(unsigned(r[1]) & high)};
+            if constexpr (!FINE) return decode(c, v_scale[0]);
+            else return decode(c, v_scale);
+        }, whole, seen, a.p.c);
     };
     for (int n = 0; n < count; n += kRing) {
         step(n, std::integral_constant<int, 0>{});
@@ -338,9 +521,10 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 2 : 1) paged8_few(Page
         step(n + 2, std::integral_constant<int, 2>{});
     }
     wait_vmcnt<0>();   // the loads past the last tile, before the LDS is used again
-    w.finish();
-    few_result<HD, kWave / 2>(a.p, it, head, w, reinterpret_cast<_Float16*>(lds),
-                              reinterpret_cast<float2(*)[32]>(lds + kW * kWave), wave, fr, h);
+    asm volatile("" ::: "memory");
+    auto* sums = reinterpret_cast<float2(*)[32]>(lds + kW * kWave);
+    w.leave(reinterpret_cast<float*>(mine), sums[wave], lane);
+    few_joined<HD, kWave / 2>(a.p, it, head, reinterpret_cast<const _Float16*>(lds), sums);
 }
 
 // Many rows. LDS: two buffers of tiles of halves for either group of waves, and each
@@ -570,8 +754,15 @@ hipError_t launch_attention_paged8(void* o, void* k_pages, void* k_scales, void*
                        shift, int(s.page_size >> shift)};
     const dim3 grid(unsigned((z.blocks + z.most) * s.kv_heads));
     const bool many = many_rows(s), wide = s.head_width == 128;
-    auto* const kernel = many ? (wide ? paged8_many<128> : paged8_many<64>)
-                              : (wide ? paged8_few<128> : paged8_few<64>);
+    const size_t rows = std::min(s.max_new, s.tokens) * (s.heads / s.kv_heads);
+    auto few_kernel = [&](auto hd) {
+        constexpr int HD = decltype(hd)::value;
+        return rows <= 16 ? (block < 8 ? paged8_few<HD, 1, true> : paged8_few<HD, 1, false>)
+                          : (block < 8 ? paged8_few<HD, 2, true> : paged8_few<HD, 2, false>);
+    };
+    auto* const kernel = many   ? (wide ? paged8_many<128> : paged8_many<64>)
+                         : wide ? few_kernel(std::integral_constant<int, 128>{})
+                                : few_kernel(std::integral_constant<int, 64>{});
     hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kFewThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     // As paged.hip joins them. Below 2^24 workgroups: tokens x heads is at most 2^25.

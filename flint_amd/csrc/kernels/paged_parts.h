@@ -22,7 +22,7 @@ constexpr int kFewRows = 32, kManyRows = 128;
 // Workgroups aimed at: what the GPU holds at once at width 64 (few rows: four a
 // CU, many: two), half of it at 128; and the fewest tiles that a part of a
 // sequence takes.
-constexpr int kFewTarget = 1024, kManyTarget = 512;
+constexpr int kFewTarget = 1024, kFewOwnTarget = 1536, kManyTarget = 512;
 constexpr int kFewTiles = 4, kManyTiles = 4;
 // From this many tiles a workgroup on, few rows are cut for two rounds of
 // workgroups, the second of which evens out what the first did not. 64 ragged
@@ -254,23 +254,15 @@ __device__ __forceinline__ void store_splits(const PagedArgs& a, const Item& it,
         a.splits[it.s] = int2{it.slot, it.parts};
 }
 
-// Few rows: joins the workgroup's waves and stores the rows, or the part's. A wave's
-// own tiles begin kWaveHalves halves after the one's before it.
+// Few rows: joins the workgroup's waves, which left O^T [HD][32], kWaveHalves halves
+// after the one's before, and their maxima and sums; stores the rows, or the part's.
 template <int HD, int kWaveHalves>
-__device__ __forceinline__ void few_result(const PagedArgs& a, const Item& it, int head,
-                                           const Rows<HD, Plan<HD, false>::kKeys>& w, _Float16* lds,
-                                           float2 (*wave_sums)[32], int wave, int fr, int h) {
+__device__ __forceinline__ void few_joined(const PagedArgs& a, const Item& it, int head,
+                                           const _Float16* lds, const float2 (*wave_sums)[32]) {
     constexpr int kW = kFewWaves;
     constexpr int kOut = HD * kFewRows / kFewThreads;   // values of a thread
     static_assert(kWaveHalves >= HD * 32 * 2, "O^T of a wave");
     const int rows = it.seq.count * a.group, first_row = it.block * kFewRows;
-    // Each leaves O^T [HD][32] in its own tiles.
-    float* own = reinterpret_cast<float*>(lds + wave * kWaveHalves);
-#pragma unroll
-    for (int db = 0; db < HD / 32; ++db)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) own[(32 * db + result_row(r, h)) * 32 + fr] = w.acc[db][r];
-    if (h == 0) wave_sums[wave][fr] = float2{w.m, w.l};
     __syncthreads();
     const int row = threadIdx.x & 31, d0 = (threadIdx.x >> 5) * kOut;
     if (first_row + row < rows) {
@@ -310,6 +302,21 @@ __device__ __forceinline__ void few_result(const PagedArgs& a, const Item& it, i
                     f32x4{sum[d], sum[d + 1], sum[d + 2], sum[d + 3]};
         }
     }
+}
+
+
+template <int HD, int kWaveHalves>
+__device__ __forceinline__ void few_result(const PagedArgs& a, const Item& it, int head,
+                                           const Rows<HD, Plan<HD, false>::kKeys>& w, _Float16* lds,
+                                           float2 (*wave_sums)[32], int wave, int fr, int h) {
+    // Each wave leaves O^T in its own tiles.
+    float* own = reinterpret_cast<float*>(lds + wave * kWaveHalves);
+#pragma unroll
+    for (int db = 0; db < HD / 32; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) own[(32 * db + result_row(r, h)) * 32 + fr] = w.acc[db][r];
+    if (h == 0) wave_sums[wave][fr] = float2{w.m, w.l};
+    few_joined<HD, kWaveHalves>(a, it, head, lds, wave_sums);
 }
 
 // Many rows: joins the two groups of waves and stores the rows, or the part's.
@@ -512,7 +519,8 @@ inline Sizes sizes_of(const flint_paged_shape& s, bool own = false) {
     Sizes z;
     z.rows = many ? kManyRows : new_rows;
     const size_t keys = many ? 64 : 32, least = many ? kManyTiles : kFewTiles;
-    const size_t target = (many ? kManyTarget : kFewTarget) * 64 / s.head_width;
+    const size_t target =
+        (many ? kManyTarget : own ? kFewOwnTarget : kFewTarget) * 64 / s.head_width;
     z.target = std::max<size_t>(1, target / s.kv_heads);
     z.most = many ? z.target : 2 * z.target;
     z.blocks = many ? std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
