@@ -643,30 +643,30 @@ __device__ __forceinline__ int encode(const float (&x)[4], float by, int e) {
     return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], low, true);
 }
 
-// The new rows of one kv head in the block that token t leads (its sequence's first new
-// token there), of K and then of V: the block's scale, its older rows rounded again where
-// that grows, the new ones. A wave takes it; HD / 8 lanes a row.
+// The new rows of sequence s from `place` on to the end of that one's block, of K or V of
+// a kv head: the block's scale, its older rows rounded again where that grows, the new ones.
+// A wave takes every `step`-th of the kv heads' K and V; HD / 8 lanes a row.
 template <int HD>
-__device__ __forceinline__ void store_block(const Paged8Args& a, int t, int head, int lane) {
+__device__ __forceinline__ void store_block(const Paged8Args& a, int s, const Sequence& q, int place,
+                                            int unit, int step, int lane) {
     constexpr int kLanes = HD / 8, kRows = 64 / kLanes;
-    const int s = sequence_at(a.p, t, lane);
-    if (s < 0) return;
-    const Sequence q = sequence_of(a.p, s);
-    const int place = t - q.first, p = q.cached + place, size = 1 << a.block_shift;
+    const int p = q.cached + place, size = 1 << a.block_shift;
     const int column = column_of(a.p, p), in = p - column * a.p.page_size, before = in & (size - 1);
-    if ((place != 0 && before != 0) || column >= a.p.max_pages) return;
+    if (column >= a.p.max_pages) return;
     const int page = a.p.table[size_t(s) * a.p.max_pages + column];
     if (page < 0 || page >= a.p.pages) return;
     const int fresh = min(size - before, q.count - place);
     const int lane_row = lane / kLanes, d = lane % kLanes * 8;
-    const size_t at = size_t(page) * a.p.kv_heads + head;
-    const size_t block = (at * a.p.page_size + (in - before)) * HD + d;
-    const size_t source = size_t(t) * a.p.kv_stride + size_t(head) * HD + d;
-    const size_t scale = at * a.blocks + (in >> a.block_shift);
-    for (int which = 0; which < 2; ++which) {
+    for (; unit < 2 * a.p.kv_heads; unit += step) {
+        const int head = unit >> 1, which = unit & 1;
+        const size_t at = size_t(page) * a.p.kv_heads + head;
+        const size_t block = (at * a.p.page_size + (in - before)) * HD + d;
+        const size_t scale = at * a.blocks + (in >> a.block_shift);
         unsigned char* const pages = which ? a.v_pages : a.k_pages;
         unsigned char* const scales = which ? a.v_scales : a.k_scales;
-        const _Float16* const x = (which ? a.p.v : a.p.k) + source;
+        const _Float16* const x =
+            (which ? a.p.v : a.p.k) + size_t(q.first + place) * a.p.kv_stride + size_t(head) * HD + d;
+        const int was = before != 0 ? scale_byte(scales[scale]) - 127 : kLeastByte - 127;
         float most = 0.0f;
         for (int r = lane_row; r < fresh; r += kRows) {
             const f16x8 v = *reinterpret_cast<const f16x8*>(x + size_t(r) * a.p.kv_stride);
@@ -678,32 +678,18 @@ __device__ __forceinline__ void store_block(const Paged8Args& a, int t, int head
         }
 #pragma unroll
         for (int i = 1; i < 64; i *= 2) most = fmaxf(most, __shfl_xor(most, i));
-        int e = exponent_of(most);
-        if (before != 0) {
-            const int was = scale_byte(scales[scale]) - 127;
-            if (e > was) {
-                const float up = scale_of(was + 127);
-                const float by = __builtin_bit_cast(float, (127 - e) << 23);
-                for (int r = lane_row; r < before; r += kRows) {
-                    auto* row = reinterpret_cast<i32x2*>(pages + block + size_t(r) * HD);
-                    const i32x2 codes = *row;
-                    i32x2 out;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const auto low =
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], up, false);
-                        const auto high =
-                            __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes[j], up, true);
-                        const float y[4] = {float(low[0]), float(low[1]), float(high[0]),
-                                            float(high[1])};
-                        out[j] = encode(y, by, e);
-                    }
-                    *row = out;
-                }
-            }
-            e = max(e, was);
-        }
+        const int e = max(exponent_of(most), was);
         const float by = __builtin_bit_cast(float, (127 - e) << 23);
+        if (e > was) {
+            const float up = scale_of(was + 127);
+            for (int r = lane_row; r < before; r += kRows) {
+                auto* row = reinterpret_cast<i32x2*>(pages + block + size_t(r) * HD);
+                const f16x8 v = decode(*row, up);
+                const float low[4] = {float(v[0]), float(v[1]), float(v[2]), float(v[3])};
+                const float high[4] = {float(v[4]), float(v[5]), float(v[6]), float(v[7])};
+                *row = i32x2{encode(low, by, e), encode(high, by, e)};
+            }
+        }
         for (int r = lane_row; r < fresh; r += kRows) {
             const f16x8 v = *reinterpret_cast<const f16x8*>(x + size_t(r) * a.p.kv_stride);
             const float low[4] = {float(v[0]), float(v[1]), float(v[2]), float(v[3])};
@@ -715,24 +701,44 @@ __device__ __forceinline__ void store_block(const Paged8Args& a, int t, int head
     }
 }
 
-// Joins the parts (the first `joins` workgroups) and stores the new rows.
+// Joins the parts (the first `joins` workgroups) and stores the new rows, `waves` waves a
+// block: `slots` blocks of each sequence, or, with slots 0, the block that each token leads
+// (its sequence's first new one there).
+struct Finish {
+    unsigned joins, places, waves, slots;
+};
 template <int HD, bool FEW>
-__global__ void __launch_bounds__(kThreads) paged8_finish(Paged8Args a, unsigned joins,
-                                                          unsigned places) {
-    if (blockIdx.x < joins) {
+__global__ void __launch_bounds__(kThreads) paged8_finish(Paged8Args a, Finish f) {
+    if (blockIdx.x < f.joins) {
         if constexpr (FEW) {
-            const unsigned row = blockIdx.x / places;
+            const unsigned row = blockIdx.x / f.places;
             join_few<HD>(a.p, int(row / unsigned(a.p.heads)), int(row % unsigned(a.p.heads)),
-                         int(blockIdx.x % places));
+                         int(blockIdx.x % f.places));
         } else {
             join_many<HD>(a.p, blockIdx.x);
         }
         return;
     }
-    const unsigned id = (blockIdx.x - joins) * (kThreads / 64) +
+    const int lane = threadIdx.x & 63;
+    const unsigned id = (blockIdx.x - f.joins) * (kThreads / 64) +
                         __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = int(id / unsigned(a.p.kv_heads)), head = int(id % unsigned(a.p.kv_heads));
-    if (t < a.p.tokens) store_block<HD>(a, t, head, threadIdx.x & 63);
+    const unsigned block = id / f.waves, size = 1u << a.block_shift;
+    int s, place;
+    Sequence q;
+    if (f.slots != 0) {
+        s = int(block / f.slots);
+        if (s >= a.p.sequences) return;
+        q = sequence_of(a.p, s);
+        place = max(0, int((unsigned(q.cached) / size + block % f.slots) * size) - q.cached);
+        if (place >= q.count) return;
+    } else {
+        s = int(block) < a.p.tokens ? sequence_at(a.p, int(block), lane) : -1;
+        if (s < 0) return;
+        q = sequence_of(a.p, s);
+        place = int(block) - q.first;
+        if (place != 0 && (unsigned(q.cached + place) & (size - 1)) != 0) return;
+    }
+    store_block<HD>(a, s, q, place, int(id % f.waves), int(f.waves), lane);
 }
 
 }  // namespace
@@ -765,9 +771,16 @@ hipError_t launch_attention_paged8(void* o, void* k_pages, void* k_scales, void*
                                 : few_kernel(std::integral_constant<int, 64>{});
     hipLaunchKernelGGL(kernel, grid, dim3(many ? kThreads * kGroups : kFewThreads), 0, stream, a);
     if (hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    // As paged.hip joins them. Below 2^24 workgroups: tokens x heads is at most 2^25.
+    // As paged.hip joins them. A wave stores K or V of one kv head's block; where the
+    // sequences' lengths leave more slots for blocks than there are tokens, the blocks are
+    // looked for token by token, four waves a token (2,000 tokens of one sequence, 8 kv heads
+    // of 128, blocks of 32: 11.5 us by sequence, 63 by token).
     const size_t sets = 256 / s.head_width, places = std::min(s.max_new, s.tokens);
-    const size_t stores = (s.tokens * s.kv_heads + 3) / 4;
+    const size_t units = 2 * s.kv_heads, slots = (places + block - 2) / block + 1;
+    const bool by_sequence =
+        s.sequences * slots <= s.tokens && s.sequences * slots * units <= (size_t{1} << 22);
+    const size_t waves = by_sequence ? units : std::min<size_t>(units, 4);
+    const size_t stores = ((by_sequence ? s.sequences * slots : s.tokens) * waves + 3) / 4;
     const bool few = s.sequences * places * s.heads <= 4096;
     const size_t joins = z.slots == 0 ? 0
                          : few ? s.sequences * places * s.heads
@@ -775,7 +788,8 @@ hipError_t launch_attention_paged8(void* o, void* k_pages, void* k_scales, void*
     auto* const finish = few ? (wide ? paged8_finish<128, true> : paged8_finish<64, true>)
                              : (wide ? paged8_finish<128, false> : paged8_finish<64, false>);
     hipLaunchKernelGGL(finish, dim3(unsigned(joins + stores)), dim3(kThreads), 0, stream, a,
-                       unsigned(joins), unsigned(places));
+                       Finish{unsigned(joins), unsigned(places), unsigned(waves),
+                              by_sequence ? unsigned(slots) : 0u});
     return hipGetLastError();
 }
 

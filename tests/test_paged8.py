@@ -245,6 +245,15 @@ def test_many_sequences(flint, cuda, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("block,page_size", [(1, 8), (8, 16), (32, 32)])
+def test_one_prompt_among_many_single_tokens(flint, cuda, block, page_size):
+    """More slots for blocks than tokens: the blocks are found token by token."""
+    cached = [(37 * i) % 90 for i in range(20)]
+    new = [100 if i == 7 else i % 3 for i in range(20)]
+    check(Run(flint, cuda, Cache(cached, new, 4, 2, 64, page_size, block, seed=23, after=1)).run())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("grow", [1e-4, 30.0, 6e4])
 @pytest.mark.parametrize("block", [1, 16])
 def test_scales_that_grow_and_extreme_rows(flint, cuda, grow, block):
