@@ -116,6 +116,8 @@ class Cache:
         for s in range(len(self.cached)):
             c, n = min(max(self.cached[s], 0), most), min(self.new[s], self.max_new)
             at = self.offsets[s]
+            if n == 0:
+                continue
             done[at:at + n] = True
             kept = [(p, self.page(s, p)) for p in range(c)]
             kept = [(p, page) for p, page in kept if page is not None]
