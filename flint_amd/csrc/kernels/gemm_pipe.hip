@@ -1117,11 +1117,11 @@ bool has_tail(const PipeConfig& c) { return c.same(PipeConfig{128, 192, 3, 64});
 // of each call showed in calls of a few us).
 size_t whole_k(const PipeConfig& c, size_t k) { return (k + c.bk - 1) & ~size_t(c.bk - 1); }
 
-// The gated products' configurations: those of which the tile choice takes one for
-// an epilogue like theirs (no loader waves or 64-wide tiles), but for 256 x 256,
-// whose epilogue does not fit the registers beside its accumulators.
-constexpr bool gated_config(int bn, int waves, int loaders) {
-    return bn >= 128 && bn < 256 && waves == 4 && loaders == 0;
+// The gated products' configurations: no 64-wide tiles, and not 256 x 256, whose
+// epilogue does not fit the registers beside its accumulators; loader waves for the
+// forward product alone (see pipe_eff).
+constexpr bool gated_config(Store st, int bn, int waves, int loaders) {
+    return bn >= 128 && bn < 256 && waves == 4 && (loaders == 0 || is_gated(st));
 }
 
 // Whether a configuration can run an epilogue over k: it fits in LDS and k is
@@ -1131,7 +1131,7 @@ constexpr bool gated_config(int bn, int waves, int loaders) {
 bool usable(const PipeConfig& c, Store st, size_t k, Layout l, bool views) {
     const bool tail = st == Store::kTn || (l != Layout::kTN && !views && has_tail(c));
     if ((is_gated(st) || st == Store::kDGated) &&
-        !gated_config(c.bn, c.waves, c.loaders))
+        !gated_config(st, c.bn, c.waves, c.loaders))
         return false;
     return lds_bytes(c, st) <= kPipeMaxLds && (whole_k(c, k) == k || tail) &&
            (c.waves == 4 || l == Layout::kNT);
@@ -1159,8 +1159,12 @@ double pipe_eff(const PipeConfig& c, Store st, Layout l) {
     // large). Other NT and NN epilogues ran as fast or slower (MLP down +
     // residual 43.8 -> 52.3 us: its residual no longer loads at tile start;
     // MLP up + GELU 54.7 -> 55.0; NN 8192 x 768 x 3072 38.2 -> 43.8), so
-    // there they are taken only when forced.
+    // there they are taken only when forced. The gated product's, too, store on a
+    // counter of their own: its projections' 96 KB a tile no longer hold up the next
+    // tile's k-steps (8192 x 768 -> 2 x 2048 with the projections 75.9 -> 71.7 us, x 2048
+    // -> 2 x 5504 381 -> 352 at 256 x 128; 2053 x 2048 -> 2 x 5504 127 -> 124 at 128 x 192).
     if (c.loaders) {
+        if (is_gated(st)) return c.bm == 256 ? 1.02 : 0.86;
         if (st == Store::kTn || st == Store::kTnHalf) return 1.0;
         if (st == Store::kBias && c.bm == 128) return 1.1;
         if (st == Store::kNone && l == Layout::kNT) return c.bm == 128 ? 1.1 : 1.15;
@@ -1226,7 +1230,8 @@ PipeConfig pick_pipe(size_t m, size_t n, size_t k, size_t slices, int cus, Store
         if (c.waves == 8 && (st != Store::kNone || rounds < kPipe8MinRounds)) continue;
         // The 256 x 128 loader tile: plain NT only on the logits' size of
         // output (8192 x 3072 x 768: 42.7 against 42.1 us for 128 x 192).
-        if (c.loaders && c.bm == 256 && l != Layout::kTN && double(m) * double(n) < 1e8)
+        if (c.loaders && c.bm == 256 && l != Layout::kTN && !is_gated(st) &&
+            double(m) * double(n) < 1e8)
             continue;
         const double cost =
             rounds * double(c.bm) * double(c.bn) * priced_k(c, l, k) / pipe_eff(c, st, l);
@@ -1301,14 +1306,16 @@ hipError_t launch_pipe(const PipeConfig& c, const Operands& op, size_t slices, i
     if (total == 0 || total > 0x7fffffffu) return hipErrorInvalidValue;
     // Persistent: one workgroup per CU (a multiple of 8, so each keeps its
     // XCD's share of the tiles), each walking ids blockIdx.x, + gridDim.x, ...
+    // With a tile or less a CU every tile has its own: cut to a multiple of 8, a few
+    // workgroups would walk two (180 tiles of 256 x 192, k 1,600: 60 us, 176 of them 34).
     size_t gx = std::min(total, size_t(cus));
-    if (gx >= 8) gx -= gx % 8;
+    if (gx >= 8 && total > gx) gx -= gx % 8;
     const dim3 grid(unsigned(gx), 1, 1);
     // Only the k-tail instances and TN's FP32 output have a partial last k-step:
     // any other would drop the k past the whole ones.
     const bool whole = ST == Store::kTn || whole_k(c, size_t(op.k)) == size_t(op.k);
 #define FLINT_PIPE_CASE(BM_, BN_, S_, BK_, NW_, LD_)                                           \
-    if constexpr (!kGatedOp || gated_config(BN_, NW_, LD_))                                    \
+    if constexpr (!kGatedOp || gated_config(ST, BN_, NW_, LD_))                                \
     if constexpr (pipe_lds_bytes<BM_, BN_, S_, BK_, L, ST, NW_>() <= kPipeMaxLds) {            \
         if (c.same(PipeConfig{BM_, BN_, S_, BK_, NW_, LD_})) {                                 \
             if (hv && !whole) return hipErrorInvalidValue;                                     \

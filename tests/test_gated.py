@@ -159,7 +159,8 @@ def test_backward_is_the_gradient(flint, cuda, act):
           bound + torch.cat([off, off], 1))
 
 
-PIPE = ["256,192,4", "128,192,4", "128,192,3,64", "256,128,3,64", "256,192,2,64"]
+PIPE = ["256,192,4", "128,192,4", "128,192,3,64", "256,128,3,64", "256,192,2,64",
+        "128,192,3,64,4,1", "256,128,3,64,4,1"]
 SMALL = ["32,32,5,8,2", "32,64,4,6,2", "64,64,8,6,2", "64,64,4,4,1", "128,64,8,3,1"]
 
 
