@@ -4,12 +4,13 @@
 // Bound by HBM: every value is read and written once, 4 bytes against some 3
 // operations. An angle is shared by all heads of its token, so a workgroup takes
 // the sines and cosines of a few tokens first (one a thread, in LDS) and then the
-// tokens' heads in 16-byte chunks: 8 values of either half of the pairs, or 4
+// tokens' heads, 32 bytes an item: 8 values of either half of the pairs, or 8
 // neighbouring pairs.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common/common.h"
 #include "kernels/kernels.h"
@@ -18,7 +19,9 @@ namespace flint {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kAhead = 4;   // items of a thread that load before the angles are there
 constexpr unsigned kMaxGrid = 1u << 20;
+constexpr size_t kMostTurns = 1024;   // sines and cosines in LDS, of a workgroup
 
 template <int N>
 struct Vec {
@@ -58,18 +61,74 @@ struct RotaryArgs {
 };
 
 // HALVES: an item turns V pairs (V values of either half), else V neighbouring
-// pairs. V is the widest that the width's alignment allows; the values that do
-// not turn are copied 2 V at a time.
+// pairs, in two vectors of V. V is the widest that the width's alignment allows; the
+// values that do not turn are copied 2 V at a time.
 template <bool HALVES, int V>
 __global__ void __launch_bounds__(kThreads) rotary(RotaryArgs a) {
     using H = typename Vec<V>::T;
-    using W = typename Vec<2 * V>::T;
     extern __shared__ float2 turns[];   // [token][pair]: cos, sin
     const unsigned pairs = a.width / 2, heads = a.heads + a.kv_heads;
     const float magnitude = float(a.plan[0]);
     const unsigned items = heads * a.chunks;
+    // An item: 2 V values of a row, V at `to` and V `gap` further on (the pairs' halves, or
+    // their neighbours), and where its token's angles lie; copied with `turn` kCopied.
+    struct Item {
+        _Float16* to;
+        unsigned turn;
+        H u, v;
+    };
+    constexpr unsigned kCopied = ~0u;
+    const unsigned half = HALVES ? pairs : V;
+    auto load = [&](unsigned t0, unsigned i) __attribute__((always_inline)) {
+        const unsigned t = i / items, in = i - t * items;
+        const unsigned head = in / a.chunks, chunk = in - head * a.chunks;
+        const bool is_q = head < a.heads, turned = chunk < a.turned;
+        const unsigned at = (is_q ? head : head - a.heads) * a.head_width +
+                            (turned ? chunk * (HALVES ? V : 2 * V)
+                                    : a.width + (chunk - a.turned) * 2 * V);
+        const _Float16* from =
+            (is_q ? a.q : a.k) + size_t(t0 + t) * (is_q ? a.q_stride : a.k_stride) + at;
+        Item x;
+        x.to = (is_q ? a.q_out : a.k_out) +
+               size_t(t0 + t) * (is_q ? a.q_out_stride : a.k_out_stride) + at;
+        x.turn = turned ? t * pairs + chunk * V : kCopied;
+        x.u = *reinterpret_cast<const H*>(from);
+        x.v = *reinterpret_cast<const H*>(from + (turned ? half : V));
+        return x;
+    };
+    auto finish = [&](const Item& it) __attribute__((always_inline)) {
+        H u = it.u, v = it.v;
+        if (it.turn != kCopied) {
+            // The 2 V values, in the order of their pairs.
+            float x[2 * V];
+            auto value = [&](int i) -> float {
+                if constexpr (V == 1) return float(i == 0 ? it.u : it.v);
+                else return float(i < V ? it.u[i % V] : it.v[i % V]);
+            };
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const int first = HALVES ? e : 2 * e, second = HALVES ? V + e : 2 * e + 1;
+                const float a0 = value(first), b0 = value(second);
+                const float c = turns[it.turn + e].x, s = turns[it.turn + e].y;
+                x[first] = __builtin_fmaf(a0, c, -b0 * s);
+                x[second] = __builtin_fmaf(a0, s, b0 * c);
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                if constexpr (V == 1) u = _Float16(x[0]), v = _Float16(x[1]);
+                else u[e] = _Float16(x[e]), v[e] = _Float16(x[V + e]);
+            }
+        }
+        *reinterpret_cast<H*>(it.to) = u;
+        *reinterpret_cast<H*>(it.to + (it.turn != kCopied ? half : V)) = v;
+    };
     for (unsigned t0 = blockIdx.x * a.block; t0 < a.tokens; t0 += gridDim.x * a.block) {
-        const unsigned block = min(a.block, a.tokens - t0);
+        const unsigned block = min(a.block, a.tokens - t0), n = block * items;
+        // The first items of a thread are on their way under the sines.
+        Item ahead[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (threadIdx.x + j * kThreads < n) ahead[j] = load(t0, threadIdx.x + j * kThreads);
         for (unsigned i = threadIdx.x; i < block * pairs; i += kThreads) {
             const unsigned t = i / pairs, pair = i - t * pairs;
             // Whole turns drop out in FP64; what is left is off by 2^-26 turns in FP32.
@@ -80,58 +139,11 @@ __global__ void __launch_bounds__(kThreads) rotary(RotaryArgs a) {
             turns[i] = float2{c * magnitude, (a.backward ? -s : s) * magnitude};
         }
         __syncthreads();
-        for (unsigned i = threadIdx.x; i < block * items; i += kThreads) {
-            const unsigned t = i / items, in = i - t * items;
-            const unsigned head = in / a.chunks, chunk = in - head * a.chunks;
-            const bool is_q = head < a.heads;
-            const unsigned at = (is_q ? head : head - a.heads) * a.head_width;
-            const _Float16* from = (is_q ? a.q : a.k) +
-                                   size_t(t0 + t) * (is_q ? a.q_stride : a.k_stride) + at;
-            _Float16* to = (is_q ? a.q_out : a.k_out) +
-                           size_t(t0 + t) * (is_q ? a.q_out_stride : a.k_out_stride) + at;
-            if (chunk >= a.turned) {
-                const unsigned d = a.width + (chunk - a.turned) * 2 * V;
-                *reinterpret_cast<W*>(to + d) = *reinterpret_cast<const W*>(from + d);
-                continue;
-            }
-            const float2* turn = turns + t * pairs + chunk * V;
-            float x[V], y[V];
-            if constexpr (HALVES) {
-                const H u = *reinterpret_cast<const H*>(from + chunk * V);
-                const H v = *reinterpret_cast<const H*>(from + pairs + chunk * V);
 #pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if constexpr (V == 1) x[e] = float(u), y[e] = float(v);
-                    else x[e] = float(u[e]), y[e] = float(v[e]);
-                }
-            } else {
-                const W w = *reinterpret_cast<const W*>(from + chunk * 2 * V);
-#pragma unroll
-                for (int e = 0; e < V; ++e) x[e] = float(w[2 * e]), y[e] = float(w[2 * e + 1]);
-            }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                const float c = turn[e].x, s = turn[e].y;
-                const float re = __builtin_fmaf(x[e], c, -y[e] * s);
-                y[e] = __builtin_fmaf(x[e], s, y[e] * c);
-                x[e] = re;
-            }
-            if constexpr (HALVES) {
-                H u, v;
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    if constexpr (V == 1) u = _Float16(x[e]), v = _Float16(y[e]);
-                    else u[e] = _Float16(x[e]), v[e] = _Float16(y[e]);
-                }
-                *reinterpret_cast<H*>(to + chunk * V) = u;
-                *reinterpret_cast<H*>(to + pairs + chunk * V) = v;
-            } else {
-                W w;
-#pragma unroll
-                for (int e = 0; e < V; ++e) w[2 * e] = _Float16(x[e]), w[2 * e + 1] = _Float16(y[e]);
-                *reinterpret_cast<W*>(to + chunk * 2 * V) = w;
-            }
-        }
+        for (int j = 0; j < kAhead; ++j)
+            if (threadIdx.x + j * kThreads < n) finish(ahead[j]);
+        for (unsigned i = threadIdx.x + kAhead * kThreads; i < n; i += kThreads)
+            finish(load(t0, i));
         __syncthreads();
     }
 }
@@ -148,9 +160,11 @@ hipError_t launch_rotary(void* q_out, void* k_out, const void* q, const void* k,
                          const void* positions, const void* plan, const flint_rotary_shape& s,
                          bool backward, hipStream_t stream) {
     const bool halves = s.layout == FLINT_ROTARY_HALVES;
-    // V values of both halves, aligned to their size; or 4 pairs, 16 bytes.
-    const size_t v = halves ? (s.width % 16 == 0 ? 8 : s.width % 8 == 0 ? 4 : 1)
-                            : (s.width % 8 == 0 ? 4 : 1);
+    // Vectors of V values, aligned to their size.
+    const size_t v = s.width % 16 == 0 && s.head_width % 16 == 0 ? 8
+                     : s.width % 8 == 0                          ? 4
+                     : s.width % 4 == 0                          ? 2
+                                                                 : 1;
     RotaryArgs a{static_cast<_Float16*>(q_out), static_cast<_Float16*>(k_out),
                  static_cast<const _Float16*>(q), static_cast<const _Float16*>(k),
                  static_cast<const int*>(positions), static_cast<const double*>(plan),
@@ -161,14 +175,21 @@ hipError_t launch_rotary(void* q_out, void* k_out, const void* q, const void* k,
     // In place nothing is copied.
     const bool copies = (s.heads != 0 && q_out != q) || (s.kv_heads != 0 && k_out != k);
     a.chunks = a.turned + (copies ? unsigned((s.head_width - s.width) / (2 * v)) : 0u);
-    // A sine and a cosine a thread; fewer tokens where that leaves CUs without any.
-    a.block = unsigned(std::max<size_t>(1, kThreads / (s.width / 2)));
-    a.block = unsigned(std::min<size_t>(a.block, std::max<size_t>(1, s.tokens / 1024)));
+    // As many tokens as the threads' first items hold; fewer where that leaves CUs without.
+    const size_t items = (s.heads + s.kv_heads) * a.chunks;
+    const size_t block = std::min(kAhead * kThreads / items, kMostTurns / (s.width / 2));
+    a.block = unsigned(std::clamp<size_t>(std::min(block, s.tokens / 1024), 1, kMostTurns));
     a.backward = backward;
     const unsigned grid =
         unsigned(std::min<size_t>(kMaxGrid, (s.tokens + a.block - 1) / a.block));
-    auto* const kernel = halves ? (v == 8 ? rotary<true, 8> : v == 4 ? rotary<true, 4> : rotary<true, 1>)
-                                : (v == 4 ? rotary<false, 4> : rotary<false, 1>);
+    auto pick = [v](auto form) {
+        constexpr bool kHalves = decltype(form)::value;
+        return v == 8   ? rotary<kHalves, 8>
+               : v == 4 ? rotary<kHalves, 4>
+               : v == 2 ? rotary<kHalves, 2>
+                        : rotary<kHalves, 1>;
+    };
+    auto* const kernel = halves ? pick(std::true_type{}) : pick(std::false_type{});
     hipLaunchKernelGGL(kernel, dim3(grid), dim3(kThreads), a.block * (s.width / 2) * sizeof(float2),
                        stream, a);
     return hipGetLastError();
