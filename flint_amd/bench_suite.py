@@ -555,6 +555,68 @@ def run(f, torch, dev, path, only=None):
         del sets
         torch.cuda.empty_cache()
 
+    def section_paged8():
+        # The same step over a cache of 8-bit values, a scale a page and head.
+        S, P, W = 64, 16, T // 16
+        lengths = [33 + 990 * i // (S - 1) for i in range(S)]
+        shape = f.paged_shape(S, S, 1, H, H, C // H, 3 * C, 3 * C, C, S * W, P, W)
+        ws = torch.empty(max(16, f.attention_paged8_workspace(shape, P)), dtype=torch.uint8,
+                         device=dev)
+        order = torch.randperm(S * W, generator=torch.Generator().manual_seed(120))
+        table = order.to(torch.int32).reshape(S, W).to(dev)
+        cached = torch.tensor(lengths, dtype=torch.int32, device=dev)
+        offsets = torch.arange(S + 1, dtype=torch.int32, device=dev)
+        o = torch.empty((S, C), dtype=torch.float16, device=dev)
+        per = 2 * sum(lengths) * C
+        sets = []
+        for r in range(_nsets(per)):
+            qkv = uniform((S, 3 * C), 121 + r).to(dev)
+            pages = [torch.randn(S * W, H, P, C // H, device=dev).mul_(100.0).to(
+                torch.float8_e4m3fn).view(torch.uint8) for _ in range(2)]
+            scales = [torch.full((S * W, H, 1), 120, dtype=torch.uint8, device=dev) for _ in range(2)]
+            sets.append((qkv[:, :C], qkv[:, C:2 * C], qkv[:, 2 * C:], *pages, *scales))
+        ms = _time_gpu(torch, lambda st: f.attention_paged8(
+            o, st[3], st[5], st[4], st[6], st[0], st[1], st[2], offsets, cached, table, shape, P,
+            0.125, workspace=ws), sets, per_round=16)
+        record("flint_attention_paged8 64 sequences, 1 new token, 33-1023 cached, 12x64", "red",
+               per + 2 * sum(-(-n // P) for n in lengths) * H + 4 * S * C * 2 + 2 * S * C, ms,
+               note="K and V of the cached positions and their scales read once")
+        del sets
+        torch.cuda.empty_cache()
+
+    def section_rotary():
+        # q and k of 8,192 tokens turned out of the qkv matrix, 12 + 12 heads of 64.
+        qkv = uniform((M, 3 * C), 130).to(dev)
+        outs = [torch.empty((M, C), dtype=torch.float16, device=dev) for _ in range(2)]
+        positions = torch.arange(M, dtype=torch.int32, device=dev) % T
+        plan = torch.empty(f.rotary_plan_bytes(C // H), dtype=torch.uint8, device=dev)
+        f.rotary_plan(plan, f.rotary_angles(C // H))
+        shape = f.rotary_shape(M, H, H, C // H, C // H, False, 3 * C, 3 * C, C, C)
+        ms = _time_gpu(torch, lambda _: f.rotary(outs[0], outs[1], qkv[:, :C], qkv[:, C:2 * C],
+                                                 positions, plan, shape), [0], per_round=8)
+        record("flint_rotary 8192 tokens, 12+12x64", "red", 4 * M * C * 2 + M * 4, ms,
+               note="q and k read and written once")
+
+    def section_gated():
+        # A gated block of width 768 and 2,048 hidden values (as many weights as the
+        # ungated MLP's), 8,192 tokens: forward with the projections kept, and their
+        # gradient.
+        N = 2048
+        x, dout = uniform((M, C), 140).to(dev), uniform((M, C), 141).to(dev)
+        w, down = uniform((2 * N, C), 142).to(dev), uniform((C, N), 143).to(dev)
+        y = torch.empty((M, N), dtype=torch.float16, device=dev)
+        pre, dpre = (torch.empty((M, 2 * N), dtype=torch.float16, device=dev) for _ in range(2))
+        if want("flint_gemm_nt_gated"):
+            ms = _time_gpu(torch, lambda _: f.gemm_nt_gated(y, pre, x, w, None, M, N, C), [0],
+                           per_round=8)
+            record("flint_gemm_nt_gated 8192x768 -> 2x2048, projections kept", "gemm",
+                   4 * M * N * C, ms)
+        if want("flint_gemm_nn_dgated"):
+            f.gemm_nt_gated(y, pre, x, w, None, M, N, C)
+            ms = _time_gpu(torch, lambda _: f.gemm_nn_dgated(dpre, dout, down, pre, M, N, C), [0],
+                           per_round=8)
+            record("flint_gemm_nn_dgated 8192x768 -> 2x2048", "gemm", 2 * M * N * C, ms)
+
     def section_logprobs():
         # Log probabilities and entropy 8192 x 50304 (vocab 50257), and the
         # gradient of the logits.
@@ -595,6 +657,12 @@ def run(f, torch, dev, path, only=None):
         section_packed()
     if want("flint_attention_paged"):
         section_paged()
+    if want("flint_attention_paged8"):
+        section_paged8()
+    if want("flint_rotary"):
+        section_rotary()
+    if want("flint_gemm_nt_gated") or want("flint_gemm_nn_dgated"):
+        section_gated()
     if want("flint_logprobs_forward") or want("flint_logprobs_backward"):
         section_logprobs()
     if want("gpt2_124m_train_step stored") or want("gpt2_124m_train_step fused"):
