@@ -12,7 +12,10 @@
 // are decoded as they become operands, V's behind a transposing read of bytes. Where
 // rows are many, a tile's four waves decode a quarter of it each, to halves in LDS. The
 // new rows, FP16 as they were given, lie in tiles of their own in front of the cached
-// ones, so that no tile mixes the two.
+// ones, so that no tile mixes the two. Measured, one new token a sequence: 64 sequences to
+// 8,192 positions, 32 heads on 8 of 128, 127.5 us (4.7 TB/s; the FP16 cache 240), 3 of
+// 131,072, 12 heads of 64, 82 us (168), 64 to 1,023, 12 of 64, 21.8 (31.6). With K and V
+// decoded to halves in LDS and 32-row products (one wave a SIMD) the first took 238.
 //
 // The rows are stored behind the attention by the launch that joins the parts: a block's
 // scale may grow with a new row, which rewrites rows that the attention reads.

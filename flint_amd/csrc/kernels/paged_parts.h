@@ -20,8 +20,9 @@ constexpr int kFewWaves = 2, kFewThreads = 64 * kFewWaves;
 constexpr int kGroups = 2;      // of 4 waves, where rows are many
 constexpr int kFewRows = 32, kManyRows = 128;
 // Workgroups aimed at: what the GPU holds at once at width 64 (few rows: four a
-// CU, many: two), half of it at 128; and the fewest tiles that a part of a
-// sequence takes.
+// CU, or six over 8-bit values, where 1,024 made 64 sequences to 8,192 positions of 8
+// heads of 128 take 157 us instead of 129; many: two), half of it at 128; and the fewest
+// tiles that a part of a sequence takes.
 constexpr int kFewTarget = 1024, kFewOwnTarget = 1536, kManyTarget = 512;
 constexpr int kFewTiles = 4, kManyTiles = 4;
 // From this many tiles a workgroup on, few rows are cut for two rounds of

@@ -5,7 +5,12 @@
 // operations. An angle is shared by all heads of its token, so a workgroup takes
 // the sines and cosines of a few tokens first (one a thread, in LDS) and then the
 // tokens' heads, 32 bytes an item: 8 values of either half of the pairs, or 8
-// neighbouring pairs.
+// neighbouring pairs. A thread's first items load before the sines are taken, since a
+// workgroup's only other loads, positions and frequencies, stand in a chain in front of
+// them (16,411 tokens, 32 + 8 heads of 128, half turned: 87 -> 71 us, 4.7 TB/s; a copy of
+// the same bytes takes 56). Recomputing the angles for every head, or reading a table of
+// them a layer, would cost more than this sharing. 8,192 tokens of 12 + 12 heads of 64
+// take 9.5 us (5.3 TB/s), one to 512 tokens a launch's 5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

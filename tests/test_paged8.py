@@ -220,6 +220,10 @@ SHAPES = [
     ([260, 12], [33, 129], 3, 1, 128, 8, 4),
     ([4000], [1], 2, 1, 64, 32, 32),
     ([3000, 50], [1, 1], 4, 1, 128, 16, 16),
+    ([40, 100], [20, 7], 1, 1, 64, 16, 4),
+    ([77, 400], [6, 1], 4, 1, 128, 8, 1),
+    ([200, 3], [2, 2], 8, 1, 128, 65536, 128),
+    ([1000], [1], 1, 1, 64, 8, 8),
 ]
 
 
@@ -265,6 +269,41 @@ def test_scales_that_grow_and_extreme_rows(flint, cuda, grow, block):
     kv = c.qkv[:, c.heads * c.width:]
     kv.copy_((kv.float() * grow).clamp(-65504, 65504).half())
     check(Run(flint, cuda, c).run())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [3.0, -3.0, 0.0, 1e-30])
+@pytest.mark.parametrize("heads,new,width", [(4, 1, 64), (32, 1, 128), (24, 1, 64), (4, 70, 128)])
+def test_scales_of_the_scores(flint, cuda, heads, new, width, scale):
+    """Scores of deviation 24 and more move the softmax's reference again and again."""
+    check(Run(flint, cuda, Cache([700, 33], [new, 1], heads, 1, width, 16, 16, seed=24,
+                                 scale=scale)).run())
+
+
+@pytest.mark.gpu
+def test_pages_past_4_gib(flint, cuda):
+    """The last pages of a pool of 5 GB, of K and of V."""
+    c = Cache([150, 64], [1, 3], 8, 8, 128, 64, 32, seed=25)
+    per = c.kv_heads * c.page_size * c.width
+    shift = (5 << 30) // per
+    small = Run(flint, cuda, c)
+    big = Run(flint, cuda, c)
+    for name in ("codes", "bytes"):
+        pools = []
+        for x in getattr(small, name):
+            pool = torch.zeros((shift + len(x),) + x.shape[1:], dtype=torch.uint8, device=cuda)
+            pool[shift:] = x
+            pools.append(pool)
+        setattr(big, name, pools)
+    big.table = torch.where(small.table >= 0, small.table + shift, -1)
+    big.shape.pages = shift + c.pages
+    small.run()
+    big.run()
+    check(small)
+    assert torch.equal(big.o, small.o)
+    for a, b in zip(big.codes + big.bytes, small.codes + small.bytes):
+        assert torch.equal(a[shift:], b)
+        assert int(a[:shift].count_nonzero()) == 0
 
 
 @pytest.mark.gpu
