@@ -73,6 +73,28 @@ __device__ __forceinline__ f16x8 decode(const i32x2& codes, const float (&scale)
     return out;
 }
 
+// Four transposing reads of bytes: of 16 lanes, 2i and 2i + 1 address the halves of row i,
+// 16 bytes, of 8; lane c gets column c of them. (The builtin waits for every load under way
+// into LDS. The wait stands in the same asm, so that no register is touched before it is
+// filled.)
+template <int OFFSET>
+__device__ __forceinline__ void read_transposed(unsigned a, unsigned b, unsigned c, unsigned d,
+                                                i32x2* to) {
+    i32x2 r0, r1, r2, r3;
+    asm volatile(
+        "ds_read_b64_tr_b8 %0, %4 offset:%8\n"
+        "ds_read_b64_tr_b8 %1, %5 offset:%8\n"
+        "ds_read_b64_tr_b8 %2, %6 offset:%8\n"
+        "ds_read_b64_tr_b8 %3, %7 offset:%8\n"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(r0), "=&v"(r1), "=&v"(r2), "=&v"(r3)
+        : "v"(a), "v"(b), "v"(c), "v"(d), "i"(OFFSET));
+    to[0] = r0;
+    to[1] = r1;
+    to[2] = r2;
+    to[3] = r3;
+}
+
 // Reads the cached rows of one sequence and kv head in tiles of KEYS positions. Codes
 // lie in LDS as rows of HD bytes, 16-byte chunk c of row r at position c ^ key(r). Two
 // reads have to spread over the banks, 32 lanes at a time: one chunk of 16 consecutive
@@ -475,21 +497,18 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 4 / RB : 2) paged8_few
         const int keys = valid[slot] >> g & 1 ? min(max(left - 8 * g, 0), 8) : 0;
         const unsigned low = keys >= 4 ? ~0u : (1u << 8 * keys) - 1;
         const unsigned high = keys >= 8 ? ~0u : keys <= 4 ? 0u : (1u << 8 * (keys - 4)) - 1;
-        // V's are read under the softmax, where they have registers that long.
+        // V's codes, four columns' operands at a time: all of them before the softmax,
+        // where they have registers that long.
         constexpr bool kEarly = HD * RB <= 128;
-        constexpr int kTogether = kEarly ? R::DB : 4;
-        i32x2 raw[kTogether];
-        auto read_v = [&](int first_db) __attribute__((always_inline)) {
-#pragma unroll
-            for (int i = 0; i < kTogether; ++i) {
-                const unsigned at = v_at[first_db + i];
-                i32x2 r;
-                asm volatile("ds_read_b64_tr_b8 %0, %1 offset:%2"
-                             : "=v"(r) : "v"(at), "i"((2 * slot + 1) * kCodes));
-                raw[i] = r;
-            }
+        i32x2 raw[kEarly ? R::DB : 4];
+        auto read_v = [&](int db, i32x2* to) __attribute__((always_inline)) {
+            read_transposed<(2 * slot + 1) * kCodes>(v_at[db], v_at[db + 1], v_at[db + 2],
+                                                     v_at[db + 3], to);
         };
-        if constexpr (kEarly) read_v(0);
+        if constexpr (kEarly) {
+#pragma unroll
+            for (int db = 0; db < R::DB; db += 4) read_v(db, raw + db);
+        }
         float k_scale[2], v_scale[FINE ? 8 : 1];
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
@@ -506,11 +525,9 @@ __global__ void __launch_bounds__(kFewThreads, HD == 64 ? 4 / RB : 2) paged8_few
             const i32x2 c = *at;
             return decode(c, k_scale[kb]);
         }, [&](int db) __attribute__((always_inline)) {
-            if (db % kTogether == 0) {
-                if constexpr (!kEarly) read_v(db);
-                wait_lds();
-            }
-            const i32x2 r = raw[db % kTogether];
+            if constexpr (!kEarly)
+                if (db % 4 == 0) read_v(db, raw);
+            const i32x2 r = raw[kEarly ? db : db % 4];
             const i32x2 c = {int(unsigned(r[0]) & low), int(unsigned(r[1]) & high)};
             if constexpr (!FINE) return decode(c, v_scale[0]);
             else return decode(c, v_scale);
