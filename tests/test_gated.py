@@ -229,6 +229,26 @@ def test_past_the_pipelines_sizes(flint, cuda, m, n, k):
 
 
 @pytest.mark.gpu
+def test_projections_past_2_to_the_32_values(flint, cuda):
+    """The last rows of 550,000 x 8,192 projections, and of their gradients."""
+    m, n, k = 550000, 4096, 8
+    g = torch.Generator(device="cuda").manual_seed(4)
+    x = torch.randn((m, k), generator=g, device=cuda, dtype=torch.float16)
+    w = torch.randn((2 * n, k), generator=g, device=cuda, dtype=torch.float16) * k ** -0.5
+    y = torch.empty((m, n), dtype=torch.float16, device=cuda)
+    pre = torch.empty((m, 2 * n), dtype=torch.float16, device=cuda)
+    flint.gemm_nt_gated(y, pre, x, w, None, m, n, k, "gelu")
+    wd = w.view(-1)[:k * n].view(k, n)
+    dpre = torch.empty((m, 2 * n), dtype=torch.float16, device=cuda)
+    flint.gemm_nn_dgated(dpre, x, wd, pre, m, n, k, "gelu")
+    for rows in (slice(0, 2), slice(m // 2, m // 2 + 2), slice(m - 2, m)):
+        y_ref, y_bound, pre_ref, pre_bound = forward_reference(x[rows].cpu(), w.cpu(), None, "gelu")
+        close(y[rows], y_ref, y_bound)
+        close(pre[rows], pre_ref, pre_bound)
+        close(dpre[rows], *backward_reference(x[rows].cpu(), wd.cpu(), pre[rows].cpu(), "gelu"))
+
+
+@pytest.mark.gpu
 def test_non_finite_values_stay_in_their_rows_and_columns(flint, cuda):
     m, n, k = 40, 48, 64
     x, w, _ = forward_inputs(m, n, k, False)

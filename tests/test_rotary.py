@@ -142,6 +142,22 @@ def test_far_and_negative_positions(flint, cuda, position):
 
 
 @pytest.mark.gpu
+def test_rows_past_2_to_the_32_values(flint, cuda):
+    """Rows as far apart as they may be, in place; the values beside them stay."""
+    tokens, stride = 520, 1 << 23
+    x = torch.empty((tokens, stride), dtype=torch.float16, device=cuda)
+    x[:, :136] = SENTINEL
+    rows = normal((tokens, 128), 5, 1.0, torch.float16)
+    x[:, :128] = rows.to(cuda)
+    positions = torch.arange(tokens, dtype=torch.int32) * 1000
+    plan = make_plan(flint, cuda, 64)
+    shape = flint.rotary_shape(tokens, 1, 1, 64, 64, False, stride, stride)
+    flint.rotary(x, x[:, 64:], x, x[:, 64:], positions.to(cuda), plan, shape)
+    close(x[:, :128], reference(rows, positions, frequencies(64, 10000.0), 2, 64, 64, False))
+    assert torch.all(x[:, 128:136] == SENTINEL)
+
+
+@pytest.mark.gpu
 def test_non_finite_values_stay_in_their_pair(flint, cuda):
     x = normal((4, 2 * 64), 4, 1.0, torch.float16)
     clean = x.clone()
