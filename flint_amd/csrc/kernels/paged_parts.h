@@ -31,6 +31,13 @@ constexpr int kFewTiles = 4, kManyTiles = 4;
 // take 258 us in two rounds and 309 in one; 32 of 3,000 positions, 12 heads of 64
 // (35 tiles), 65 and 62.
 constexpr int kTwoRounds = 64;
+// Many rows over 8-bit values are cut for two rounds where one would leave a sixth of its
+// time idle and take this many tiles: a block's parts are equal, and seldom as many as the
+// workgroups. 3,000 new tokens over 30,000, 12 heads on 4 of 64 (one round of 284 workgroups
+// for 512), take 704 us in one round and 475 in two, 2,000 over 16,384, 12 of 64, 213 and
+// 185; where a round is full, two cost their joins: 64 over 131,072, 32 on 8 of 128, 197 and
+// 215; and at 21 tiles 53 and 58.
+constexpr int kManyTwoRounds = 32;
 
 template <int HD, bool MANY>
 struct Plan {
@@ -115,15 +122,24 @@ __device__ __forceinline__ bool find_item(const PagedArgs& a, int idx, int lane,
     total = ((long long)(wave_sum(int(total >> 24))) << 24) + wave_sum(int(total & 0xffffff));
     constexpr long long kMost = 1 << 30;   // more tiles than any sequence has
     const bool twice = !MANY && total >= (long long)(kTwoRounds) * a.target;
-    const int target = twice ? 2 * a.target : a.target;
+    int target = twice ? 2 * a.target : a.target;
     int each = max(P::kLeast, int(min(kMost, (total + target - 1) / target)));
     // The target is what the GPU holds at once: parts that round up past it would
     // run behind the others. (One step of sequences only; the parts of more are
     // many anyway.)
-    for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
-        const int parts = (tiles_of(q) + each - 1) / each;
-        if (wave_sum(blocks_of(q) * parts) <= target || __ballot(parts > 1) == 0) break;
-        each += (each + 7) / 8;
+    auto fit = [&] {
+        for (int i = 0; i < 8 && a.sequences <= 64; ++i) {
+            const int parts = (tiles_of(q) + each - 1) / each;
+            if (wave_sum(blocks_of(q) * parts) <= target || __ballot(parts > 1) == 0) break;
+            each += (each + 7) / 8;
+        }
+    };
+    fit();
+    if (MANY && OWN && total >= (long long)(kManyTwoRounds) * target &&
+        6 * total < 5 * (long long)(each) * target) {
+        target *= 2;
+        each = int(min(kMost, (total + target - 1) / target));
+        fit();
     }
     int before = 0, slots = 0;
     for (int s0 = 0; s0 < a.sequences; s0 += 64) {
@@ -523,7 +539,7 @@ inline Sizes sizes_of(const flint_paged_shape& s, bool own = false) {
     const size_t target =
         (many ? kManyTarget : own ? kFewOwnTarget : kFewTarget) * 64 / s.head_width;
     z.target = std::max<size_t>(1, target / s.kv_heads);
-    z.most = many ? z.target : 2 * z.target;
+    z.most = many && !own ? z.target : 2 * z.target;
     z.blocks = many ? std::min(s.sequences * ((new_rows + z.rows - 1) / z.rows),
                                s.tokens * group / z.rows + s.sequences)
                     : s.sequences;

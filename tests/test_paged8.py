@@ -241,6 +241,13 @@ def test_many_parts(flint, cuda, width, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv_heads,width", [(32, 64), (16, 128)])
+def test_two_rounds_of_parts(flint, cuda, kv_heads, width):
+    """Six blocks of rows of 102 tiles for 16 workgroups: 12 parts, or 30 in two rounds."""
+    check(Run(flint, cuda, Cache([5800], [700], kv_heads, kv_heads, width, 64, 64, seed=29)).run())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [1, 40])
 def test_many_sequences(flint, cuda, new):
     """More than one step of the search over sequences, some of them empty."""
