@@ -277,6 +277,11 @@ struct FewRows {
                                          const int (&seen)[RB], float c) {
         f16x8 p[RB];
         for (;;) {
+            // Two blocks of rows read K's operands again where the tile is done again: kept for
+            // it, they took 32 registers through the softmax and others went to scratch, whose
+            // loads wait for the tiles on their way (64 sequences of 8 new tokens over 4,096,
+            // 32 heads on 8 of 128: 192 -> 130 us; 64-wide heads 71 -> 55).
+            if constexpr (RB > 1) asm volatile("" ::: "memory");
             f32x4 s[RB][2] = {};
 #pragma unroll
             for (int kk = 0; kk < KK; ++kk)
