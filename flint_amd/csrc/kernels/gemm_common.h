@@ -230,6 +230,7 @@ struct Operands {
     HeadView wv, yv;       // batched NN / TN (not gemm.hip): w (k-major) and
                            // y as heads views
     int gelu;              // gated products (not gemm.hip): the tanh GELU, or SiLU
+    int cached;            // (the pipeline alone) pre, or dpre, is stored through L2
 };
 
 }  // namespace

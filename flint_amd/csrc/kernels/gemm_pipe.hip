@@ -982,8 +982,12 @@ gemm_pipe(Operands op, TileArgs ta) {
                             if (!pre_pass && q >= E::kYPerLane) continue;
                             const unsigned off = gated_chunk_at(j, h, q, pre_pass, &r, &cc);
                             const f16x8 v = *reinterpret_cast<const f16x8*>(cst + r * E::kLdw + cc * 8);
-                            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v), rout,
-                                                                   off, 0, kStoreAux);
+                            if (pre_pass && op.cached)
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v),
+                                                                       rout, off, 0, 0);
+                            else
+                                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(i32x4, v),
+                                                                       rout, off, 0, kStoreAux);
                         } else if constexpr (ST == Store::kDGated) {
                             // Gate: RN16(sum u act'(g)), up: RN16(sum act(g)).
                             const unsigned off = chunk_at(j, h, q, 2, &r, &cc);
@@ -1135,6 +1139,17 @@ bool usable(const PipeConfig& c, Store st, size_t k, Layout l, bool views) {
         return false;
     return lds_bytes(c, st) <= kPipeMaxLds && (whole_k(c, k) == k || tail) &&
            (c.waves == 4 || l == Layout::kNT);
+}
+
+// Whether the gated product's projections are stored without the non-temporal bit: where a
+// wave's pieces of their rows start or end inside 64 bytes (n not whole 32s, or 192-wide
+// tiles: 48 columns of either), whose halves then meet in L2 and not in memory. One round of
+// tiles has its dirty lines to write back at its end, and past the 256 MB of the last-level
+// cache the rounds wait for them.
+bool stores_cached(const PipeConfig& c, Store st, size_t m, size_t n, int cus) {
+    const size_t tiles = ((m + c.bm - 1) / c.bm) * ((gated_width(n) + c.bn - 1) / c.bn);
+    return st == Store::kGatedPre && (n % 32 != 0 || c.bn % 128 != 0) && tiles > size_t(cus) &&
+           6 * m * n <= (size_t{1} << 28);
 }
 
 // Relative throughput per unit of tile area, measured on the GPT-2 shapes at
@@ -1598,6 +1613,7 @@ hipError_t launch_gemm_pipe(GemmLayout gl, Epilogue e, void* y, const void* x, c
     if (!pipe_forced(&c, &disabled) || !usable(c, st, k, l, views))
         c = pick_pipe(m, is_gated(st) ? gated_width(n) : n, k, slices, cus, st, l, views,
                       op.causal != 0);
+    op.cached = stores_cached(c, st, m, n, cus);
     switch (l) {
     case Layout::kNT: return dispatch_pipe<Layout::kNT>(c, st, op, slices, split_len, cus, stream);
     case Layout::kNN: return dispatch_pipe<Layout::kNN>(c, st, op, slices, split_len, cus, stream);
