@@ -1143,9 +1143,11 @@ bool usable(const PipeConfig& c, Store st, size_t k, Layout l, bool views) {
 
 // Whether the gated product's projections are stored without the non-temporal bit: where a
 // wave's pieces of their rows start or end inside 64 bytes (n not whole 32s, or 192-wide
-// tiles: 48 columns of either), whose halves then meet in L2 and not in memory. One round of
-// tiles has its dirty lines to write back at its end, and past the 256 MB of the last-level
-// cache the rounds wait for them.
+// tiles: 48 columns of either), whose halves then meet in L2 and not in memory (8192 x 768 ->
+// 2 x 2056 103 -> 80 us, x 2304 in 128 x 192 tiles 94 -> 80; 4096 x 1024 -> 2 x 2824 85 -> 69).
+// Whole pieces are faster past L2 (8192 x 768 -> 2 x 2048 77 and 81); one round of tiles
+// writes its dirty lines back at its end (1000 x 1600 -> 2 x 4288 38 and 43); and past the 256
+// MB of the last-level cache the rounds wait for them (8192 x 2048 -> 2 x 5480 387 and 403).
 bool stores_cached(const PipeConfig& c, Store st, size_t m, size_t n, int cus) {
     const size_t tiles = ((m + c.bm - 1) / c.bm) * ((gated_width(n) + c.bn - 1) / c.bn);
     return st == Store::kGatedPre && (n % 32 != 0 || c.bn % 128 != 0) && tiles > size_t(cus) &&
