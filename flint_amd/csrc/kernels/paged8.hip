@@ -1,6 +1,5 @@
 // Attention of new tokens over a paged cache of 8-bit values for gfx950, and their
-// storing: paged.hip's work items and tiles, with the cached rows decoded on their way
-// into LDS.
+// storing: paged.hip's work items and tiles, with the cached rows decoded on the chip.
 //
 // A value of the cache is an e4m3 number times a power of two from 2^-15 to 2^8, which
 // FP16 holds exactly: its subnormals reach 2^-24 = 2^-9 2^-15, and rows are stored with
