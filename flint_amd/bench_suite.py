@@ -586,15 +586,18 @@ def run(f, torch, dev, path, only=None):
 
     def section_rotary():
         # q and k of 8,192 tokens turned out of the qkv matrix, 12 + 12 heads of 64.
-        qkv = uniform((M, 3 * C), 130).to(dev)
-        outs = [torch.empty((M, C), dtype=torch.float16, device=dev) for _ in range(2)]
         positions = torch.arange(M, dtype=torch.int32, device=dev) % T
         plan = torch.empty(f.rotary_plan_bytes(C // H), dtype=torch.uint8, device=dev)
         f.rotary_plan(plan, f.rotary_angles(C // H))
         shape = f.rotary_shape(M, H, H, C // H, C // H, False, 3 * C, 3 * C, C, C)
-        ms = _time_gpu(torch, lambda _: f.rotary(outs[0], outs[1], qkv[:, :C], qkv[:, C:2 * C],
-                                                 positions, plan, shape), [0], per_round=8)
-        record("flint_rotary 8192 tokens, 12+12x64", "red", 4 * M * C * 2 + M * 4, ms,
+        per = 4 * M * C * 2
+        sets = []
+        for r in range(_nsets(per)):
+            qkv = uniform((M, 3 * C), 150 + r).to(dev)
+            outs = [torch.empty((M, C), dtype=torch.float16, device=dev) for _ in range(2)]
+            sets.append((*outs, qkv[:, :C], qkv[:, C:2 * C]))
+        ms = _time_gpu(torch, lambda st: f.rotary(*st, positions, plan, shape), sets, per_round=8)
+        record("flint_rotary 8192 tokens, 12+12x64", "red", per + M * 4, ms,
                note="q and k read and written once")
 
     def section_gated():
@@ -602,20 +605,31 @@ def run(f, torch, dev, path, only=None):
         # ungated MLP's), 8,192 tokens: forward with the projections kept, and their
         # gradient.
         N = 2048
-        x, dout = uniform((M, C), 140).to(dev), uniform((M, C), 141).to(dev)
         w, down = uniform((2 * N, C), 142).to(dev), uniform((C, N), 143).to(dev)
-        y = torch.empty((M, N), dtype=torch.float16, device=dev)
-        pre, dpre = (torch.empty((M, 2 * N), dtype=torch.float16, device=dev) for _ in range(2))
+        sets = []
+        for r in range(_nsets((M * C + 3 * M * N) * 2)):
+            x = uniform((M, C), 170 + r).to(dev)     # the output's gradient, too
+            y = torch.empty((M, N), dtype=torch.float16, device=dev)
+            pre, dpre = (torch.empty((M, 2 * N), dtype=torch.float16, device=dev) for _ in range(2))
+            sets.append((x, y, pre, dpre))
+
+        def forward(st):
+            f.gemm_nt_gated(st[1], st[2], st[0], w, None, M, N, C)
+
+        def gradient(st):
+            f.gemm_nn_dgated(st[3], st[0], down, st[2], M, N, C)
+
         if want("flint_gemm_nt_gated"):
-            ms = _time_gpu(torch, lambda _: f.gemm_nt_gated(y, pre, x, w, None, M, N, C), [0],
-                           per_round=8)
+            ms = _time_gpu(torch, forward, sets, per_round=8)
             record("flint_gemm_nt_gated 8192x768 -> 2x2048, projections kept", "gemm",
                    4 * M * N * C, ms)
         if want("flint_gemm_nn_dgated"):
-            f.gemm_nt_gated(y, pre, x, w, None, M, N, C)
-            ms = _time_gpu(torch, lambda _: f.gemm_nn_dgated(dpre, dout, down, pre, M, N, C), [0],
-                           per_round=8)
+            for st in sets:
+                forward(st)
+            ms = _time_gpu(torch, gradient, sets, per_round=8)
             record("flint_gemm_nn_dgated 8192x768 -> 2x2048", "gemm", 2 * M * N * C, ms)
+        del sets
+        torch.cuda.empty_cache()
 
     def section_logprobs():
         # Log probabilities and entropy 8192 x 50304 (vocab 50257), and the
