@@ -228,6 +228,66 @@ def test_past_the_pipelines_sizes(flint, cuda, m, n, k):
     close(dpre[rows][:, at], *ref)
 
 
+def check_rows(y, pre, dpre, x, w, dout, wd, pre_in, rows, act):
+    """Whole rows of either pass against float64."""
+    x, dout, w, wd = x[rows].cpu(), dout[rows].cpu(), w.cpu(), wd.cpu()
+    y_ref, y_bound, pre_ref, pre_bound = forward_reference(x, w, None, act)
+    close(y[rows], y_ref, y_bound)
+    close(pre[rows], pre_ref, pre_bound)
+    close(dpre[rows], *backward_reference(dout, wd, pre_in[rows].cpu(), act))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("k", [320, 328])
+def test_several_tiles_a_workgroup_of_several_steps(flint, cuda, tune, k):
+    """25 x 22 tiles of 256 x 192 for 256 CUs, and more of every other tile, of 5 steps and
+    more: a workgroup's second and third tiles begin under the stores of the one before.
+    Whole outputs are the same bits from every tile (k = 328 on the tile that takes partial
+    steps), with the projections' stores through L2 and past it."""
+    m, n, nd, act = 6151, 2056, 4104, "silu"
+    g = torch.Generator(device="cuda").manual_seed(5)
+
+    def random(rows, columns, std=1.0):
+        return (torch.randn((rows, columns), generator=g, device=cuda) * std).half()
+
+    x, w = random(m, k), random(2 * n, k, k ** -0.5)
+    dout, wd, pre_in = random(m, k, 0.5), random(k, nd, k ** -0.5), random(m, 2 * nd, 2.0)
+    rows = [0, 1, 31, 127, 128, 255, 256, 2999, m // 2, 4095, 4096, m - 9, m - 8, m - 7, m - 2, m - 1]
+
+    def all_of():
+        y, pre = run_forward(flint, cuda, x, w, None, act, True)
+        alone, _ = run_forward(flint, cuda, x, w, None, act, False)
+        return y, pre, alone, run_backward(flint, cuda, dout, wd, pre_in, act)
+
+    want = all_of()
+    check_rows(want[0], want[1], want[3], x, w, dout, wd, pre_in, rows, act)
+    assert torch.equal(want[0], want[2])
+    for name, plans in (("gemm_pipe", PIPE if k % 64 == 0 else ["128,192,3,64"]),
+                        ("gemm_small", SMALL[3:])):
+        for plan in plans:
+            tune(name, plan)
+            got = all_of()
+            tune(name, None)
+            for i, (a, b) in enumerate(zip(got, want)):
+                assert torch.equal(a, b), (name, plan, i)
+
+
+@pytest.mark.gpu
+def test_outputs_past_the_pipelines_in_several_steps(flint, cuda):
+    """Projections and gradients of 2.3 GB, past the pipeline's 2^31 bytes, k a whole step
+    and a partial one: the first, middle and last rows."""
+    m, n, k, act = 70001, 8192, 72, "gelu"
+    assert m * 2 * n * 2 >= 1 << 31
+    g = torch.Generator(device="cuda").manual_seed(6)
+    x, dout = (torch.randn((m, k), generator=g, device=cuda, dtype=torch.float16) for _ in range(2))
+    w = torch.randn((2 * n, k), generator=g, device=cuda, dtype=torch.float16) * k ** -0.5
+    wd = w.view(-1)[:k * n].view(k, n)
+    y, pre = run_forward(flint, cuda, x, w, None, act, True)
+    dpre = run_backward(flint, cuda, dout, wd, pre, act)
+    rows = [0, m // 2, m // 2 + 1, m - 2, m - 1]
+    check_rows(y, pre, dpre, x, w, dout, wd, pre, rows, act)
+
+
 @pytest.mark.gpu
 def test_projections_past_2_to_the_32_values(flint, cuda):
     """The last rows of 550,000 x 8,192 projections, and of their gradients."""
