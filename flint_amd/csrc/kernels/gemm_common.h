@@ -161,7 +161,7 @@ struct TileArgs {
 
 // Maps logical tile id `id` (< tiles_per_slice * slices) to (slice, tile_m,
 // tile_n). Workgroups run persistently: workgroup b takes ids b, b + G, b + 2G,
-// ... (G = grid size, a multiple of 8 when there are at least 8 ids), so id % 8
+// ... (G = grid size, a multiple of 8 where there are more than G ids), so id % 8
 // is the XCD the workgroup runs on (XCDs take workgroups round-robin). The
 // remap gives XCD x the contiguous range [x * total/8, (x+1) * total/8) of
 // tiles when total is a multiple of 8; within a slice, tiles go in groups of
@@ -230,7 +230,7 @@ struct Operands {
     HeadView wv, yv;       // batched NN / TN (not gemm.hip): w (k-major) and
                            // y as heads views
     int gelu;              // gated products (not gemm.hip): the tanh GELU, or SiLU
-    int cached;            // (the pipeline alone) pre, or dpre, is stored through L2
+    int cached;            // (the pipeline's kGatedPre alone) pre is stored through L2
 };
 
 }  // namespace

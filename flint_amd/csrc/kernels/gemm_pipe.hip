@@ -291,8 +291,8 @@ gemm_pipe(Operands op, TileArgs ta) {
     const int y_ld = HV ? op.yv.ld : (ST == Store::kDGated ? 2 * n : n);
     _Float16* const cst = lds + kStageHalves + wave * E::kHalves;
 
-    // This workgroup's tiles: ids blockIdx.x, + gridDim.x, ... (gridDim.x is a
-    // multiple of 8 when there are 8 or more tiles, so they stay on one XCD).
+    // This workgroup's tiles: ids blockIdx.x, + gridDim.x, ... (Where workgroups take
+    // several tiles, gridDim.x is a multiple of 8, so they stay on one XCD.)
     const unsigned total = unsigned(ta.tiles_per_slice) * unsigned(ta.slices);
     const int n_tiles = int((total - 1 - blockIdx.x) / gridDim.x) + 1;
     struct Tile {
