@@ -12,9 +12,19 @@
 // rows are many, a tile's four waves decode a quarter of it each, to halves in LDS. The
 // new rows, FP16 as they were given, lie in tiles of their own in front of the cached
 // ones, so that no tile mixes the two. Measured, one new token a sequence: 64 sequences to
-// 8,192 positions, 32 heads on 8 of 128, 127.5 us (4.7 TB/s; the FP16 cache 240), 3 of
-// 131,072, 12 heads of 64, 82 us (168), 64 to 1,023, 12 of 64, 21.8 (31.6). With K and V
-// decoded to halves in LDS and 32-row products (one wave a SIMD) the first took 238.
+// 8,192 positions, 32 heads on 8 of 128, 136 us (4.65 TB/s; the FP16 cache 259), 3 of 50,000
+// to 131,072, 12 heads of 64, 82 us (164), 64 to 1,023, 12 of 64, 21 to 22.5 (32 to 33). With
+// K and V decoded to halves in LDS and 32-row products (one wave a SIMD) the first took 238.
+//
+// Probabilities enter the product with V as FP16, as in paged.hip; their sum is of the FP32
+// values. o is then 2.9e-4 of itself from float64 (root mean squares), where storing it in
+// FP16 alone leaves 2.1e-4; the cache's e4m3 values are off by up to 2^-4 of theirs. A
+// second product, with what the rounding left of each probability, brings 2.1e-4 and takes
+// the first of these from 136 to 138 us, the last from 22.1 to 23.4, 8 new tokens each over
+// to 4,096 positions, 32 heads on 8 of 128, from 97 to 104, and where rows are many chunks of
+// 500 over to 4,096, 12 heads on 4 of 64, from 39 to 52, 2,000 over 16,384, 12 of 64, from 181
+// to 278 (it spills there): left out for all, so that a token's result is as exact in a batch
+// of either kind.
 //
 // The rows are stored behind the attention by the launch that joins the parts: a block's
 // scale may grow with a new row, which rewrites rows that the attention reads.
