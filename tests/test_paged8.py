@@ -267,6 +267,31 @@ def test_one_prompt_among_many_single_tokens(flint, cuda, block, page_size):
 
 
 @pytest.mark.gpu
+def test_single_tokens_and_a_prompt_called_apart(flint, cuda):
+    """Two calls over one cache and one set of rows, each with its own sequences: what one
+    call gives, and neither touches the other's rows or blocks."""
+    c = Cache([700, 33, 0, 129, 64, 300], [1, 1, 1, 1, 70, 41], 8, 2, 64, 16, 16, seed=30, after=1)
+    ref = c.reference()
+    r = Run(flint, cuda, c)
+    for first, last, most in ((0, 4, 1), (4, 6, 70)):
+        before = r.o.clone()
+        part = slice(first, last)
+        # (Clones of their own: a slice may begin off 16 bytes.)
+        offsets, cached, table = (x.clone() for x in (r.offsets[first:last + 1], r.cached[part],
+                                                      r.table[part]))
+        s = flint.paged_shape(c.tokens, last - first, most, c.heads, c.kv_heads, c.width,
+                              r.shape.q_stride, r.shape.kv_stride, r.shape.o_stride, c.pages,
+                              c.page_size, c.table.shape[1])
+        q, k, v = c.parts(r.qkv)
+        flint.attention_paged8(r.o, r.codes[0], r.bytes[0], r.codes[1], r.bytes[1], q, k, v,
+                               offsets, cached, table, s, c.block, c.scale)
+        mine = torch.zeros(c.tokens, dtype=torch.bool)
+        mine[c.offsets[first]:c.offsets[last]] = True
+        assert torch.equal(r.o[~mine.to(cuda)], before[~mine.to(cuda)])
+    check(r, ref)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("grow", [1e-4, 30.0, 6e4])
 @pytest.mark.parametrize("block", [1, 16])
 def test_scales_that_grow_and_extreme_rows(flint, cuda, grow, block):
