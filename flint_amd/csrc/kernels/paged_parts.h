@@ -20,9 +20,12 @@ constexpr int kFewWaves = 2, kFewThreads = 64 * kFewWaves;
 constexpr int kGroups = 2;      // of 4 waves, where rows are many
 constexpr int kFewRows = 32, kManyRows = 128;
 // Workgroups aimed at: what the GPU holds at once at width 64 (few rows: four a
-// CU, or six over 8-bit values, where 1,024 made 64 sequences to 8,192 positions of 8
-// heads of 128 take 157 us instead of 129; many: two), half of it at 128; and the fewest
-// tiles that a part of a sequence takes.
+// CU, or six over 8-bit values; many: two), half of it at 128; and the fewest tiles that
+// a part of a sequence takes. With 1,024 and with 1,536 over 8-bit values, one new token:
+// 64 sequences to 8,192 positions, 8 heads of K and V of 128, 170 and 136 us, 64 to 1,023,
+// 12 of 64, 24.7 and 22.1; 17 to 32 rows (32 heads on 8): 64 sequences of 8 new tokens to
+// 4,096 at width 128 108 and 97, at 64 53 and 50, 16 of 5 at 128 37 and 33, but 200 of 2 to
+// 1,000, 32 heads on 2 of 128, 31 and 38.
 constexpr int kFewTarget = 1024, kFewOwnTarget = 1536, kManyTarget = 512;
 constexpr int kFewTiles = 4, kManyTiles = 4;
 // From this many tiles a workgroup on, few rows are cut for two rounds of
