@@ -892,9 +892,9 @@ hipError_t launch_gemm_nn(void* y, const void* x, const void* w, const void* aux
 // size where the pipeline does not. As one product of 2n columns the forward pass is
 // bound as a plain one is: by the MFMAs and the load path where rows are many (8,192 x
 // 768 -> 2 x 2,048 50 to 54 us, 960 to 1,040 TFLOP/s; with the projections kept, 96 KB a
-// tile more to store, 66 to 79), by reading w where they are few (1 x 4,096 -> 2 x 8,192
+// tile more to store, 66 to 80), by reading w where they are few (1 x 4,096 -> 2 x 8,192
 // 27.6 us, 4.9 TB/s). The gradient reads and writes 8 bytes an output beside its product
-// and does that after the k-steps: 8,192 x 768 x 2,048 51 to 55 us, the plain product 33
+// and does that after the k-steps: 8,192 x 768 x 2,048 51 to 56 us, the plain product 33
 // to 35 and a copy of pre and dpre 21.5. Its activations cost 3 us of it; pre loaded four
 // blocks ahead, and 128 x 128 tiles two a CU, gain nothing (all workgroups are in step).
 hipError_t launch_gemm_nt_gated(void* y, void* pre, const void* x, const void* w, const void* bias,

@@ -10,7 +10,7 @@
 // them (16,411 tokens, 32 + 8 heads of 128, half turned: 87 -> 71 us, 4.7 TB/s; a copy of
 // the same bytes takes 56). Recomputing the angles for every head, or reading a table of
 // them a layer, would cost more than this sharing. 8,192 tokens of 12 + 12 heads of 64
-// take 9.5 us (5.3 TB/s), one to 512 tokens a launch's 5.
+// take 12.7 us (4.0 TB/s; 10.1 to 13 in the kernel), one to 512 tokens a launch's 5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
